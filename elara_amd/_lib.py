@@ -94,6 +94,19 @@ SIGNATURES = {
     'elr_step_exec_dev': (ctypes.c_int, [c_vp, c_vp, c_vp, c_i64, c_vp, c_vp]),
     'elr_step_dev_bytes': (c_i64, [c_vp]),
     'elr_step_dev': (ctypes.c_int, [c_vp, c_vp, c_i64, c_vp, c_vp]),
+    'elr_token_logprobs_scratch_bytes': (c_i64, [c_i64, c_i64, ctypes.c_int]),
+    'elr_token_logprobs': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, ctypes.c_int, ctypes.c_int]
+                           + [c_vp] * 6 + [c_i64, c_vp]),
+    'elr_token_logprobs_backward': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, ctypes.c_int]
+                                    + [c_vp] * 6 + [c_i64, c_vp]),
+    'elr_rms_norm': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, ctypes.c_int, c_i64, c_vp,
+                                    ctypes.c_int, c_f32, c_vp, ctypes.c_int, c_i64, c_vp, c_vp, c_vp, c_vp]),
+    'elr_rms_norm_backward_scratch_bytes': (c_i64, [c_i64, c_i64, ctypes.c_int]),
+    'elr_rms_norm_backward': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, ctypes.c_int, c_i64, c_vp,
+                                             c_i64, c_vp, ctypes.c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'elr_grad_norm_scratch_bytes': (c_i64, [c_vp, c_i64]),
+    'elr_grad_norm': (ctypes.c_int, [c_vp, c_i64, ctypes.c_int, c_vp, c_vp, c_i64, c_vp]),
+    'elr_clip_grad_norm': (ctypes.c_int, [c_vp, c_i64, ctypes.c_int, c_f32, c_f32, c_vp, c_vp, c_i64, c_vp]),
 }
 
 DIR_FIELDS = ('code', 'loc', 'ent', 'lstep', 'lfree', 'n_lfree', 'log_top', 'mat_top', 'live', 'adm_c0', 'rj',
@@ -205,8 +218,14 @@ class StepDevOut(ctypes.Structure):
     _fields_ = [(n, c_i64) for n in STEP_DEV_OUT_FIELDS] + [('exec', ExecOut)]
 
 
+class Grad(ctypes.Structure):
+    """elr_grad: one tensor of a gradient norm, and where its clipped values go."""
+    _fields_ = [('data', c_vp), ('out', c_vp)] + [(n, c_i64) for n in ('rows', 'cols', 'ld', 'cs', 'out_ld', 'out_cs')] + [
+        ('type', c_i32), ('out_type', c_i32)]
+
+
 ABI_STRUCTS = (DirState, DirParams, PlanIn, PlanOut, AssembleArgs, SlotsArgs, UpdateArgs, ExecArgs, ExecOut, PlanCtl,
-               StepDevArgs, StepDevOut)
+               StepDevArgs, StepDevOut, Grad)
 
 
 def lib():
@@ -331,3 +350,5 @@ def split_empty(dev, dtype, sizes):
 
 
 ESIZE = {torch.int8: 1, torch.bool: 1, torch.uint8: 1, torch.int32: 4, torch.int64: 8, torch.float32: 4}
+# element types of include/elara_amd.h
+ETYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}

@@ -1,0 +1,117 @@
+// Element types (fp32, fp16, bf16) in 16-byte vectors, and wave reductions, for the operators between the looked-up rows
+// and their update (log probabilities, norms, gradient clipping).  All arithmetic is fp32: an element is widened when it
+// is loaded and rounded once, to nearest even, when it is stored.
+#pragma once
+
+#include "elr_common.h"
+
+namespace elr {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// A 16-byte vector at any element's address: gfx950 takes such accesses in one instruction (a row of an odd number of
+// 16-bit elements then needs no peeled head; only the memory lines at its ends are touched twice).
+typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+
+// VE elements in 16 bytes; widen() and narrow() convert a whole vector.
+template <class E>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int VE = 4, kType = ELR_F32;
+  typedef f32x4 vec;
+};
+template <>
+struct Elem<_Float16> {
+  static constexpr int VE = 8, kType = ELR_F16;
+  typedef f16x8 vec;
+};
+template <>
+struct Elem<__bf16> {
+  static constexpr int VE = 8, kType = ELR_BF16;
+  typedef bf16x8 vec;
+};
+
+template <class E>
+struct Frag {
+  float v[Elem<E>::VE];
+};
+
+template <class E>
+__device__ __forceinline__ Frag<E> widen(u32x4 raw) {
+  constexpr int N = Elem<E>::VE;
+  typedef float fN __attribute__((ext_vector_type(N)));
+  const fN f = __builtin_convertvector(__builtin_bit_cast(typename Elem<E>::vec, raw), fN);
+  Frag<E> r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r.v[j] = f[j];
+  return r;
+}
+
+template <class E>
+__device__ __forceinline__ u32x4 narrow(const Frag<E>& a) {
+  constexpr int N = Elem<E>::VE;
+  typedef float fN __attribute__((ext_vector_type(N)));
+  fN f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = a.v[j];
+  return __builtin_bit_cast(u32x4, __builtin_convertvector(f, typename Elem<E>::vec));
+}
+
+// The raw vector at p of which `valid` elements (any number; <= 0: none) may be read; the others are `fill`.  NT: read
+// once, not kept in the caches.
+template <class E, bool NT>
+__device__ __forceinline__ u32x4 load_raw(const E* p, int64_t valid, float fill) {
+  constexpr int N = Elem<E>::VE;
+  if (valid >= N) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(p));
+    else return *reinterpret_cast<const u32x4_u*>(p);
+  }
+  typename Elem<E>::vec r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r[j] = j < valid ? p[j] : (E)fill;
+  return __builtin_bit_cast(u32x4, r);
+}
+
+template <class E, bool NT>
+__device__ __forceinline__ void store_raw(E* p, u32x4 x, int64_t valid) {
+  constexpr int N = Elem<E>::VE;
+  if (valid >= N) {
+    if constexpr (NT) __builtin_nontemporal_store((u32x4_u)x, reinterpret_cast<u32x4_u*>(p));
+    else *reinterpret_cast<u32x4_u*>(p) = (u32x4_u)x;
+    return;
+  }
+  const typename Elem<E>::vec r = __builtin_bit_cast(typename Elem<E>::vec, x);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < valid) p[j] = r[j];
+}
+
+template <class E>
+__device__ __forceinline__ float to_f32(E x) { return (float)x; }
+
+// max(a, b) that is NaN if either is (torch's amax); __builtin_fmaxf drops a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Sum and maximum over aligned groups of `width` lanes (a power of two up to 64); every lane gets the result.  The order
+// of the additions is fixed.
+__device__ __forceinline__ float lanes_sum(float x, int width) {
+  for (int o = 1; o < width; o <<= 1) x = x + __shfl_xor(x, o, 64);
+  return x;
+}
+__device__ __forceinline__ float lanes_max(float x, int width) {
+  for (int o = 1; o < width; o <<= 1) x = __builtin_fmaxf(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ float lanes_max_nan(float x, int width) {
+  for (int o = 1; o < width; o <<= 1) x = max_nan(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+inline int64_t elem_size(int type) { return type == ELR_F32 ? 4 : 2; }
+inline bool elem_type_ok(int type) { return type == ELR_F32 || type == ELR_F16 || type == ELR_BF16; }
+inline bool elem_aligned(const void* p, int type) { return ((uintptr_t)p & (uintptr_t)(elem_size(type) - 1)) == 0; }
+
+}  // namespace elr

@@ -636,7 +636,8 @@ extern "C" int elr_abi_sizes(int64_t* out, int n) {
                         (int64_t)sizeof(elr_plan_out), (int64_t)sizeof(elr_assemble_args),
                         (int64_t)sizeof(elr_slots_args), (int64_t)sizeof(elr_update_args),
                         (int64_t)sizeof(elr_exec_args), (int64_t)sizeof(elr_exec_out), (int64_t)sizeof(elr_plan_ctl),
-                        (int64_t)sizeof(elr_step_dev_args), (int64_t)sizeof(elr_step_dev_out)};
+                        (int64_t)sizeof(elr_step_dev_args), (int64_t)sizeof(elr_step_dev_out),
+                        (int64_t)sizeof(elr_grad)};
   const int m = (int)(sizeof(sz) / sizeof(sz[0]));
   const int k = n < m ? n : m;
   for (int i = 0; i < k; ++i) out[i] = sz[i];

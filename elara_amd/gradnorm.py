@@ -1,0 +1,115 @@
+"""The global norm of many gradients, and clipping by it, before the row-sparse and the dense Adam.  No counterpart in the
+reference, whose step updates unclipped.
+
+    grad_norm(grads, norm_type=2.0) -> norm                              float32 scalar on the GPU
+    clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None) -> norm   grads scaled by min(1, max_norm / (norm + eps))
+
+They run the HIP kernels behind elr_grad_norm and elr_clip_grad_norm (elara_amd/csrc/gradnorm.hip) on torch's current
+stream: two launches for up to 144 tensors, and no host synchronisation.  A batch's summed row gradients
+(dedup.embedding_dense_backward, dedup.segment_sum_plan) are one of the tensors.
+"""
+import math
+
+import torch
+
+from . import _lib
+
+_KINDS = {1.0: 1, 2.0: 2, math.inf: 0}
+
+
+def _two_strides(t, o):
+    """(rows, cols, ld, cs, out_ld, out_cs) of t's elements and o's in the same order, neighbouring dimensions merged."""
+    dims = []
+    for d in sorted(range(t.dim()), key=lambda i: (-t.stride(i), -t.shape[i])):
+        if t.shape[d] == 1:
+            continue
+        ts, os = t.stride(d), o.stride(d)
+        if dims and dims[-1][1] == ts * t.shape[d] and dims[-1][2] == os * t.shape[d]:
+            dims[-1] = (dims[-1][0] * t.shape[d], ts, os)
+        else:
+            dims.append((t.shape[d], ts, os))
+    while len(dims) < 2:
+        dims.insert(0, (1, 0, 0))
+    if len(dims) > 2:
+        raise RuntimeError(f'a gradient of shape {tuple(t.shape)} and strides {t.stride()} does not reduce to two strides')
+    (rows, ld, old), (cols, cs, ocs) = dims
+    return rows, cols, ld, cs, old, ocs
+
+
+def _describe(grads, out):
+    grads = list(grads)
+    if not grads:
+        raise RuntimeError('grads must hold at least one tensor')
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise RuntimeError(f'out must hold {len(grads)} tensors, got {len(outs)}')
+    dev = grads[0].device
+    arr = (_lib.Grad * len(grads))()
+    for i, (t, o) in enumerate(zip(grads, outs)):
+        if not (t.is_cuda and t.device == dev and t.dtype in _lib.ETYPE and t.layout == torch.strided):
+            raise RuntimeError(f'gradient {i} must be a cuda float32, float16 or bfloat16 tensor on {dev}, got {t.dtype} '
+                               f'{t.device}')
+        if o is not t and not (o.is_cuda and o.device == dev and o.dtype in (t.dtype, torch.float32)
+                               and o.shape == t.shape and o.layout == torch.strided):
+            raise RuntimeError(f'out {i} must be a cuda {t.dtype} or float32 tensor of shape {tuple(t.shape)} on {dev}')
+        n = t.numel()
+        if t.is_contiguous() and (o is t or o.is_contiguous()):
+            shape = (1, n, n, 1, n, 1)
+        else:
+            shape = _two_strides(t, o) if n else (0, 0, 0, 0, 0, 0)
+        arr[i] = (t.data_ptr(), o.data_ptr(), *shape, _lib.ETYPE[t.dtype], _lib.ETYPE[o.dtype])
+    return grads, outs, dev, arr
+
+
+def _kind(norm_type):
+    try:
+        return _KINDS[float(norm_type)]
+    except (KeyError, TypeError, ValueError):
+        raise RuntimeError(f'norm_type must be 1, 2 or inf, got {norm_type!r}') from None
+
+
+def _run(grads, out, kind, clip):
+    grads, outs, dev, arr = _describe(grads, out)
+    if clip:
+        seen = set()
+        for i, o in enumerate(outs):
+            if o.numel() and (o.data_ptr() in seen or _self_overlap(o)):
+                raise RuntimeError(f'output {i} overlaps itself or another: each element is scaled once')
+            if o.numel():
+                seen.add(o.data_ptr())
+    L = _lib.lib()
+    n = len(arr)
+    nbytes = L.elr_grad_norm_scratch_bytes(arr, n)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(max(nbytes, 8) // 8, dtype=torch.float64, device=dev)
+    with _lib.on_device(dev):
+        if clip:
+            rc = L.elr_clip_grad_norm(arr, n, kind, *clip, norm.data_ptr(), scratch.data_ptr(), nbytes,
+                                      _lib.raw_stream(dev))
+        else:
+            rc = L.elr_grad_norm(arr, n, kind, norm.data_ptr(), scratch.data_ptr(), nbytes, _lib.raw_stream(dev))
+    _lib.check(rc, 'elr_clip_grad_norm' if clip else 'elr_grad_norm')
+    return norm
+
+
+def _self_overlap(t):
+    """Whether some dimension of more than one element has stride 0 (an expanded tensor)."""
+    return any(s == 0 and d > 1 for s, d in zip(t.stride(), t.shape))
+
+
+def grad_norm(grads, norm_type=2.0):
+    """(sum |g|^p)^(1/p) over every element of every tensor of grads (p = norm_type: 1, 2 or inf), as a float32 scalar on
+    the GPU.  grads: cuda float32, float16 or bfloat16 tensors of one device, of any shapes and of strides that reduce to
+    two.  Summed in float64; the order of the additions depends on the sizes alone."""
+    return _run(grads, None, _kind(norm_type), None)
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None):
+    """Scales grads so that their global norm is at most max_norm, and returns the norm before that (grad_norm's).
+    In place, or into out: a list of tensors of grads' shapes, each of its gradient's type or float32 (16-bit gradients
+    straight into the float32 rows that gpu_adam reads).  In place a norm of at most max_norm costs no write.  A NaN makes
+    the norm and every gradient NaN; an infinite norm scales by 0."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise RuntimeError(f'max_norm must be at least 0, got {max_norm}')
+    return _run(grads, out, _kind(norm_type), (max_norm, float(eps)))

@@ -33,6 +33,11 @@ extern "C" {
 #define ELR_EUNSUPPORTED (-2) /* valid for the reference but outside this build's limits (e.g. K > 8) */
 #define ELR_ECAPACITY (-3)   /* caller-provided scratch or output too small */
 
+/* Element types of the operators below that take more than fp32. */
+#define ELR_F32 0
+#define ELR_F16 1
+#define ELR_BF16 2
+
 /* Text for a return code (static storage). */
 const char* elr_error_string(int code);
 
@@ -726,6 +731,82 @@ int elr_glog_take(float* logs, int64_t nlogs, const int64_t* ids, const float* g
  * distinct.  Rows out of range are skipped. */
 int elr_mark_rows(const int64_t* rows, const int64_t* n_dev, int64_t n_max, int32_t value, int32_t* out,
                   int64_t out_rows, uint32_t* bits, uint32_t bit, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Log probabilities of given tokens (no counterpart in the reference, whose models end in a sigmoid): the loss of a
+ * model that predicts one of V ids, or its scores when it serves.  For each of n rows x of V logits:
+ *   lse = log sum e^x;  logprob = x[token] - lse;  entropy = -sum p log p, p = e^(x - lse);
+ *   top_id / top_logprob [n, k]: the k largest logits, larger first, ties by the lower id, -0 equal to +0 (0 <= k <=
+ *   min(V, ELR_TOPK_MAX)).
+ * A token outside [0, V) marks a row without one: its logprob is 0.  A row of nothing but -inf has lse and logprob
+ * -inf and entropy 0; a NaN or +inf in a row makes its fp32 results NaN, and a NaN ranks as -inf among the top ids.
+ *   logits of `type` (ELR_F32, ELR_F16, ELR_BF16), row i at logits + i * ld elements (ld may exceed V, or be 0);
+ *   tokens int32 (idx64 = 0) or int64 (1) [n]; logprob, lse, entropy fp32 [n]; scratch of
+ *   elr_token_logprobs_scratch_bytes(n, V, k) bytes, 8-byte aligned (may be 0; -1: bad argument).
+ * ------------------------------------------------------------------------------------------------------- */
+#define ELR_TOPK_MAX 32
+int64_t elr_token_logprobs_scratch_bytes(int64_t n, int64_t V, int k);
+int elr_token_logprobs(const void* logits, int type, int64_t n, int64_t V, int64_t ld, const void* tokens, int idx64,
+                       int k, float* logprob, float* lse, float* entropy, float* top_logprob, int64_t* top_id,
+                       void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Its gradient to the logits: d_logits[v] = [v = token] g + p_v (z - g - h (log p_v + entropy)), with g, h, z the
+ * gradients of logprob, entropy and lse (each fp32 [n] or NULL: zero), lse and entropy from the forward (entropy may be
+ * NULL without d_entropy).  A row without a token has g = 0, a row with lse below -2^100 (nothing
+ * but -inf, or nothing but fp32's or bf16's lowest value) no gradient.  d_logits has
+ * `type` and the row stride out_ld >= V; it may be the logits themselves (same stride). */
+int elr_token_logprobs_backward(const void* logits, int type, int64_t n, int64_t V, int64_t ld, const void* tokens,
+                                int idx64, const float* lse, const float* entropy, const float* d_logprob,
+                                const float* d_entropy, const float* d_lse, void* d_logits, int64_t out_ld,
+                                void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Root-mean-square norm with the residual's addition (no counterpart in the reference).  For each of n rows of D:
+ *   h = x + residual (h = x without one);  rstd = 1 / sqrt(mean h^2 + eps);  y = h rstd weight,
+ * sums in fp32, the norm of the unrounded h.  fp8 = 0: y has x's type.  fp8 = 1: y holds e4m3 bytes of y / scale, with
+ * scale = max|y| / 448 (1 where that is 0) over each row (group = 0; scale fp32 [n]) or over each `group` of 32, 64,
+ * 128 or 256 columns that divides D (scale fp32 [n, D / group]).
+ *   x of `type`, residual (or NULL) and h of res_type = type or ELR_F32, weight (or NULL: ones) of w_type = type or
+ *   ELR_F32; rows of x and residual x_ld and res_ld elements apart; y, h, rstd [n] contiguous.  h is written only with a
+ *   residual and must not overlap x or the residual.
+ * ------------------------------------------------------------------------------------------------------- */
+int elr_rms_norm(const void* x, int type, int64_t n, int64_t D, int64_t x_ld, const void* residual, int res_type,
+                 int64_t res_ld, const void* weight, int w_type, float eps, void* y, int fp8, int64_t group,
+                 float* scale, void* h, float* rstd, void* stream);
+
+/* Its backward.  dy (of `type`) is y's gradient, h and rstd the forward's, dh (or NULL) the gradient that arrives on h:
+ *   dx = rstd (u - xh mean(u xh)) + dh, u = weight dy, xh = h rstd: the gradient of x and of the residual alike;
+ *   dweight (fp32 [D], or NULL) = sum over the rows of dy xh, in an order that depends on the sizes alone.
+ * h, dh and dx have h_type = type or ELR_F32; dx is contiguous and may be dh or h where that is contiguous too.  scratch
+ * of elr_rms_norm_backward_scratch_bytes(n, D, type) bytes, 4-byte aligned, only with dweight. */
+int64_t elr_rms_norm_backward_scratch_bytes(int64_t n, int64_t D, int type);
+int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_t D, int64_t dy_ld, const void* h, int h_type,
+                          int64_t h_ld, const void* dh, int64_t dh_ld, const void* weight, int w_type,
+                          const float* rstd, void* dx, float* dweight, void* scratch, int64_t scratch_bytes,
+                          void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * The global norm of many gradients, and clipping by it (no counterpart in the reference).
+ *   norm = (sum |g|^p)^(1/p) over all elements of all n tensors, p = 1, 2, or 0 for the largest |g| (summed in fp64);
+ *   clip: out = g min(1, max_norm / (norm + eps)) for each tensor.
+ * A NaN makes the norm NaN, and then the outputs; an infinite norm scales by 0.
+ * ------------------------------------------------------------------------------------------------------- */
+typedef struct elr_grad {
+  const void* data;
+  void* out;            /* clip: the data itself (in place; then nothing is written if the scale is 1), or another array */
+  int64_t rows, cols;   /* element (i, j) at data + i * ld + j * cs and out + i * out_ld + j * out_cs */
+  int64_t ld, cs, out_ld, out_cs;
+  int32_t type;         /* ELR_F32, ELR_F16 or ELR_BF16 */
+  int32_t out_type;     /* the same, or ELR_F32 */
+} elr_grad;
+
+/* grads: a host array, read during the call.  norm: device fp32 [1].  scratch: elr_grad_norm_scratch_bytes(grads, n)
+ * bytes, 8-byte aligned (-1: bad argument).  Outputs must not overlap one another or other tensors' data. */
+int64_t elr_grad_norm_scratch_bytes(const elr_grad* grads, int64_t n);
+int elr_grad_norm(const elr_grad* grads, int64_t n, int p, float* norm, void* scratch, int64_t scratch_bytes,
+                  void* stream);
+int elr_clip_grad_norm(const elr_grad* grads, int64_t n, int p, float max_norm, float eps, float* norm, void* scratch,
+                       int64_t scratch_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Exhaustive check of the step-constant division (no counterpart in the reference).  The Adam kernels compute
