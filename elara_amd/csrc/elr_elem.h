@@ -14,6 +14,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // A 16-byte vector at any element's address: gfx950 takes such accesses in one instruction (a row of an odd number of
 // 16-bit elements then needs no peeled head; only the memory lines at its ends are touched twice).
 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
 
 // VE elements in 16 bytes; widen() and narrow() convert a whole vector.
 template <class E>
@@ -87,6 +89,60 @@ __device__ __forceinline__ void store_raw(E* p, u32x4 x, int64_t valid) {
 #pragma unroll
   for (int j = 0; j < N; ++j)
     if (j < valid) p[j] = r[j];
+}
+
+// The raw vector at p[e], where elements outside [0, len) are `fill` and not read (e may be negative: a row or tensor walked
+// from the memory line that it starts in, so that every wave's accesses are whole lines).
+template <class E, bool NT>
+__device__ __forceinline__ u32x4 load_part(const E* p, int64_t e, int64_t len, float fill) {
+  constexpr int N = Elem<E>::VE;
+  if (e >= 0 && e + N <= len) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(p + e));
+    else return *reinterpret_cast<const u32x4_u*>(p + e);
+  }
+  typename Elem<E>::vec r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r[j] = e + j >= 0 && e + j < len ? p[e + j] : (E)fill;
+  return __builtin_bit_cast(u32x4, r);
+}
+template <class E, bool NT>
+__device__ __forceinline__ void store_part(E* p, int64_t e, int64_t len, u32x4 x) {
+  constexpr int N = Elem<E>::VE;
+  if (e >= 0 && e + N <= len) {
+    if constexpr (NT) __builtin_nontemporal_store((u32x4_u)x, reinterpret_cast<u32x4_u*>(p + e));
+    else *reinterpret_cast<u32x4_u*>(p + e) = (u32x4_u)x;
+    return;
+  }
+  const typename Elem<E>::vec r = __builtin_bit_cast(typename Elem<E>::vec, x);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (e + j >= 0 && e + j < len) p[e + j] = r[j];
+}
+// Elements between p and the line of `bytes` that it lies in.
+template <class E>
+__host__ __device__ inline int line_shift(const void* p, int bytes) {
+  return (int)(((uintptr_t)p & (uintptr_t)(bytes - 1)) / sizeof(E));
+}
+
+// Four elements (8 bytes of a 16-bit type, 16 of fp32) at p[e], where those outside [0, len) are 0 and not read.
+template <class E, bool NT>
+__device__ __forceinline__ f32x4 load4(const E* p, int64_t e, int64_t len) {
+  typedef E v4 __attribute__((ext_vector_type(4)));
+  if (e >= 0 && e + 4 <= len) {
+    if constexpr (sizeof(E) == 4) {
+      const u32x4_u* q = reinterpret_cast<const u32x4_u*>(p + e);
+      const u32x4 r = NT ? __builtin_nontemporal_load(q) : *q;
+      return __builtin_bit_cast(f32x4, r);
+    } else {
+      const u32x2_u* q = reinterpret_cast<const u32x2_u*>(p + e);
+      const u32x2 r = NT ? __builtin_nontemporal_load(q) : *q;
+      return __builtin_convertvector(__builtin_bit_cast(v4, r), f32x4);
+    }
+  }
+  f32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = e + j >= 0 && e + j < len ? (float)p[e + j] : 0.0f;
+  return r;
 }
 
 template <class E>

@@ -4,36 +4,49 @@
 //   N = (sum |g|^p)^(1/p) over every element of every tensor, p = 1, 2 or inf;  c = min(1, max_norm / (N + eps));
 //   out = c g.
 //
-// Two launches: the first leaves one partial sum per block, the second adds the partials (every block the same ones in the
-// same order, so there is no launch between that does only this) and scales.  In place with c = 1 the second ends there
-// and writes nothing.  No atomics: the order of the additions depends on the sizes alone.
+// The first launches leave one partial sum per block.  A list of few chunks is then scaled by one launch whose blocks each
+// add the same partials in the same order; a longer one has a launch for the addition and then a block per chunk.  In place
+// with c = 1 the scaling ends there and writes nothing.  No atomics: the order of the additions depends on the sizes and
+// alignments alone.
 //
-// Sums are fp64 (fp64 fma runs at fp32's rate on this chip): no overflow or underflow of squares, and the norm is exact to
-// its one rounding to fp32.  A NaN gives a NaN norm; a norm of +inf gives c = 0 (so inf * 0 = NaN where a gradient was
-// inf), as dividing by it does.
+// Sums are fp64: no overflow or underflow of squares, and the norm is exact to its one rounding to fp32.  It costs nothing
+// (fp32 sums: 131 us against 133 for 717 MB).  A NaN gives a NaN norm; a norm of +inf gives c = 0 (so inf * 0 = NaN where a
+// gradient was inf), as dividing by it does.
 //
 // The tensors travel in the kernel arguments, kList of them a launch: nothing is copied to the device ahead, and a captured
-// graph holds its own list.  Each is cut into chunks of 16 KB; a block finds its chunk's tensor by binary search.
+// graph holds its own list.  Each is cut into chunks of 16 KB.
+//
+// Measured: 641 MB of bf16 gradients packed next to one another and 77 MB of fp32 rows, into fp32 (240 tensors): sum 125 us
+// (5.7 TB/s), scaling 322 us (6.4 TB/s; the sum's last reads are still in the last-level cache when the scaling, which goes
+// backwards, begins).  What brought it there from 928 us: whole memory lines (451 -> 385 us of scaling with aligned stores
+// and a chunk a block), lines of 256 bytes for the widened output (-> 365), and a chunk's bounds tested once instead of at
+// each access (-> 322).
 #include "elr_elem.h"
 
 #include <algorithm>
 
 namespace elr {
 
-constexpr int kList = 144;
+constexpr int kList = 136;
 constexpr int kGradThreads = 256;
 constexpr int kGradVecs = 4;                 // 16-byte vectors of a thread in a chunk
-constexpr int64_t kPartBlocks = 2048;        // blocks (and partial sums) over all launches of a call, about
+constexpr int64_t kPartBlocks = 8192;        // blocks (and partial sums) over all launches of a call, about (2048: 12 % slower)
+constexpr int64_t kScaleBlocks = 1 << 22;    // blocks of one scaling launch, at most
+constexpr int64_t kOwnBlocks = 1024;         // chunks up to which the scaling's blocks add the partials themselves
 constexpr int64_t kMostElems = (int64_t)1 << 31;   // elements of one list entry
 
+// Entries of 4 and 8 bytes only.  With a byte array here the compiler formed (arguments + i) + 7 i as the address of in[i]
+// for a scalar load, which drops the two low bits of each part and so read half of one pointer and half of the next (a
+// memory violation): every part of such an address has to be a multiple of four.
 struct GradList {
   const void* in[kList];
   void* out[kList];
   uint32_t len[kList];           // elements
   uint32_t end[kList];           // chunks up to and with this tensor
-  uint8_t type[kList];           // input's element type | 4 if the output is fp32 and the input is not
+  uint32_t type[kList];          // input's element type | 4 if the output is fp32 and the input is not
   int32_t count;
 };
+static_assert(sizeof(GradList) + 64 <= 4096, "kernel arguments");
 
 template <class E>
 constexpr int chunk_elems() { return kGradThreads * kGradVecs * Elem<E>::VE; }
@@ -76,25 +89,37 @@ __device__ __forceinline__ Acc<P> block_merge(Acc<P> x, Acc<P>* lds) {
   return x;
 }
 
-// The list entry that holds chunk c (wave-uniform).
+// The list entry that holds chunk c: every lane compares its share of the chunk ends (one load's latency, where a binary
+// search would be eight loads, one after another).
 __device__ __forceinline__ int entry_of(const GradList& g, uint32_t c) {
-  int lo = 0, hi = g.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (c < g.end[mid]) hi = mid;
-    else lo = mid + 1;
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+#pragma unroll
+  for (int q = 0; q < (kList + 63) / 64; ++q) {
+    const int i = q * 64 + lane;
+    const uint32_t end = i < g.count ? g.end[i] : UINT32_MAX;
+    n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= c));
   }
-  return lo;
+  return n;
 }
 
+// Chunks are laid from a memory line's start, the sum's from the input's and the scaling's from the output's: with a wave's
+// 16-byte accesses off the lines by the tensor's own offset, tensors packed next to one another were 5 to 18 % slower than
+// padded ones (160 M bf16 elements into fp32: 163 and 177 us against 150).
+constexpr int kInLine = 128, kOutLine = 256;   // (256: 16-bit input then starts on 128 too when it widens to fp32)
+
 template <int P, class E>
-__device__ __forceinline__ Acc<P> chunk_sum(const E* p, int64_t left, Acc<P> acc) {
+__device__ __forceinline__ Acc<P> chunk_sum(const void* in, int64_t chunk, int64_t len, Acc<P> acc) {
   constexpr int VE = Elem<E>::VE;
+  const E* p = (const E*)in;
+  const int64_t c0 = chunk * chunk_elems<E>() - line_shift<E>(in, kInLine), e0 = c0 + (int)threadIdx.x * VE;
   u32x4 raw[kGradVecs];
+  if (c0 >= 0 && c0 + chunk_elems<E>() <= len) {
 #pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int e = (u * kGradThreads + (int)threadIdx.x) * VE;
-    raw[u] = load_raw<E, false>(p + e, left - e, 0.0f);
+    for (int u = 0; u < kGradVecs; ++u) raw[u] = load_raw<E, false>(p + e0 + u * kGradThreads * VE, VE, 0.0f);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kGradVecs; ++u) raw[u] = load_part<E, false>(p, e0 + u * kGradThreads * VE, len, 0.0f);
   }
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
@@ -113,14 +138,11 @@ __global__ __launch_bounds__(kGradThreads) void k_grad_sum(GradList g, double* p
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int i = entry_of(g, c);
     const int64_t in = c - (i ? g.end[i - 1] : 0u);
-    const int type = g.type[i] & 3;
-    if (type == ELR_F32) {
-      const int64_t e = in * chunk_elems<float>();
-      acc = chunk_sum<P>((const float*)g.in[i] + e, (int64_t)g.len[i] - e, acc);
-    } else {
-      const int64_t e = in * chunk_elems<__bf16>();
-      if (type == ELR_F16) acc = chunk_sum<P>((const _Float16*)g.in[i] + e, (int64_t)g.len[i] - e, acc);
-      else acc = chunk_sum<P>((const __bf16*)g.in[i] + e, (int64_t)g.len[i] - e, acc);
+    const int64_t len = g.len[i];
+    switch (g.type[i] & 3u) {
+      case ELR_F32: acc = chunk_sum<P, float>(g.in[i], in, len, acc); break;
+      case ELR_F16: acc = chunk_sum<P, _Float16>(g.in[i], in, len, acc); break;
+      default: acc = chunk_sum<P, __bf16>(g.in[i], in, len, acc); break;
     }
   }
   acc = block_merge<P>(acc, lds);
@@ -173,64 +195,76 @@ __global__ __launch_bounds__(kGradThreads) void k_grad_norm(const double* part, 
 
 struct Clip {
   const double* part;
-  int parts;
+  int parts;             // 0: *norm is there already
   float max_norm, eps;
   float* norm;
   int write;             // outputs other than the inputs: written also where c = 1
 };
 
-// c of every thread; the first block of the first launch writes the norm.
+// c of every thread.  With parts, each block adds them up and the first writes the norm.
 template <int P>
 __device__ __forceinline__ float coef_of(const Clip& k, Acc<P>* lds) {
-  const float x = norm_of<P>(k.part, k.parts, lds);
-  if (k.norm && blockIdx.x == 0 && threadIdx.x == 0) *k.norm = x;
+  float x;
+  if (k.parts) {
+    x = norm_of<P>(k.part, k.parts, lds);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *k.norm = x;
+  } else {
+    x = *k.norm;
+  }
   const float c = k.max_norm / (x + k.eps);
   return c > 1.0f ? 1.0f : c;    // NaN stays
 }
 
-template <class E, class O>
-__device__ __forceinline__ void chunk_scale(const E* p, O* o, int64_t left, float c) {
-  constexpr int VE = Elem<E>::VE, VO = Elem<O>::VE;
-  u32x4 raw[kGradVecs];
+template <class E, class O, bool ALL>
+__device__ __forceinline__ void scale_vecs(const E* p, O* o, int64_t e0, int64_t len, float c) {
+  constexpr int N = Elem<O>::VE, V = chunk_elems<E>() / (kGradThreads * N);   // elements of a store, stores of a thread
+  Frag<O> x[V];
 #pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int e = (u * kGradThreads + (int)threadIdx.x) * VE;
-    raw[u] = load_raw<E, true>(p + e, left - e, 0.0f);
+  for (int v = 0; v < V; ++v) {
+    const int64_t e = e0 + v * kGradThreads * N;
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+      const f32x4 a = load4<E, true>(p + (ALL ? e + 4 * q : 0), ALL ? 0 : e + 4 * q, ALL ? 4 : len);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[v].v[4 * q + j] = a[j];
+    }
   }
 #pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int e = (u * kGradThreads + (int)threadIdx.x) * VE;
-    const Frag<E> x = widen<E>(raw[u]);
+  for (int v = 0; v < V; ++v) {
+    const int64_t e = e0 + v * kGradThreads * N;
 #pragma unroll
-    for (int q = 0; q < VE / VO; ++q) {
-      Frag<O> y;
-#pragma unroll
-      for (int j = 0; j < VO; ++j) y.v[j] = x.v[q * VO + j] * c;
-      store_raw<O, true>(o + e + q * VO, narrow<O>(y), left - e - q * VO);
-    }
+    for (int j = 0; j < N; ++j) x[v].v[j] = x[v].v[j] * c;
+    if constexpr (ALL) store_raw<O, true>(o + e, narrow<O>(x[v]), N);
+    else store_part<O, true>(o, e, len, narrow<O>(x[v]));
   }
 }
 
-// The chunks in the reverse of the first launch's order: what it read last may still be in the last-level cache.
+template <class E, class O>
+__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t chunk, int64_t len, float c) {
+  const int64_t c0 = chunk * chunk_elems<E>() - line_shift<O>(out, kOutLine);
+  const int64_t e0 = c0 + (int)threadIdx.x * Elem<O>::VE;
+  if (c0 >= 0 && c0 + chunk_elems<E>() <= len) scale_vecs<E, O, true>((const E*)in, (O*)out, e0, len, c);
+  else scale_vecs<E, O, false>((const E*)in, (O*)out, e0, len, c);
+}
+
+// The chunks in the reverse of the sum's order (the lists come reversed): what it read last may still be in the last-level
+// cache.
 template <int P>
 __global__ __launch_bounds__(kGradThreads) void k_grad_scale(GradList g, Clip k) {
   __shared__ Acc<P> lds[kGradThreads / 64];
   const float c = coef_of<P>(k, lds);
   if (c == 1.0f && !k.write) return;
   const uint32_t chunks = g.end[g.count - 1];
-  for (uint32_t b = blockIdx.x; b < chunks; b += gridDim.x) {
-    const uint32_t at = chunks - 1 - b;
+  for (uint32_t at = blockIdx.x; at < chunks; at += gridDim.x) {
     const int i = entry_of(g, at);
-    const int64_t in = at - (i ? g.end[i - 1] : 0u);
-    const int type = g.type[i];
-    const int64_t e = in * ((type & 3) == ELR_F32 ? chunk_elems<float>() : chunk_elems<__bf16>());
-    const int64_t left = (int64_t)g.len[i] - e;
-    switch (type) {
-      case ELR_F32: chunk_scale((const float*)g.in[i] + e, (float*)g.out[i] + e, left, c); break;
-      case ELR_F16: chunk_scale((const _Float16*)g.in[i] + e, (_Float16*)g.out[i] + e, left, c); break;
-      case ELR_BF16: chunk_scale((const __bf16*)g.in[i] + e, (__bf16*)g.out[i] + e, left, c); break;
-      case ELR_F16 | 4: chunk_scale((const _Float16*)g.in[i] + e, (float*)g.out[i] + e, left, c); break;
-      default: chunk_scale((const __bf16*)g.in[i] + e, (float*)g.out[i] + e, left, c); break;
+    const int64_t in = g.end[i] - 1 - at;
+    const int64_t len = g.len[i];
+    switch (g.type[i]) {
+      case ELR_F32: chunk_scale<float, float>(g.in[i], g.out[i], in, len, c); break;
+      case ELR_F16: chunk_scale<_Float16, _Float16>(g.in[i], g.out[i], in, len, c); break;
+      case ELR_BF16: chunk_scale<__bf16, __bf16>(g.in[i], g.out[i], in, len, c); break;
+      case ELR_F16 | 4: chunk_scale<_Float16, float>(g.in[i], g.out[i], in, len, c); break;
+      default: chunk_scale<__bf16, float>(g.in[i], g.out[i], in, len, c); break;
     }
   }
 }
@@ -258,34 +292,39 @@ static bool one_run(const elr_grad& g) {
 }
 
 // The call's launches: lists of contiguous tensors (filled one at a time) and strided ones.  visit(list or NULL,
-// strided or NULL, chunks) for each.
+// strided or NULL, chunks) for each.  back: from the last tensor to the first.
 template <class F>
-static void each_launch(const elr_grad* g, int64_t n, const F& visit) {
+static void each_launch(const elr_grad* g, int64_t n, bool back, const F& visit) {
   GradList l;
   l.count = 0;
   uint32_t chunks = 0;
   auto flush = [&] {
-    if (l.count) visit(&l, (const Strided*)nullptr, (int64_t)chunks);
+    if (l.count) visit((const GradList*)&l, (const Strided*)nullptr, (int64_t)chunks);
     l.count = 0;
     chunks = 0;
   };
-  for (int64_t i = 0; i < n; ++i) {
-    const elr_grad& t = g[i];
+  for (int64_t q = 0; q < n; ++q) {
+    const elr_grad& t = g[back ? n - 1 - q : q];
     const int64_t total = t.rows * t.cols;
     if (total == 0) continue;
     const int64_t ie = elem_size(t.type), oe = elem_size(t.out_type);
     if (!one_run(t)) {
       const Strided s{t.data, t.out, t.rows, t.cols, t.ld, t.cs, t.out_ld, t.out_cs, t.type, t.out_type == ELR_F32};
-      visit((GradList*)nullptr, &s, (total + chunk_of(t.type) - 1) / chunk_of(t.type));
+      visit((const GradList*)nullptr, &s, (total + chunk_of(t.type) - 1) / chunk_of(t.type));
       continue;
     }
-    for (int64_t a = 0; a < total; a += kMostElems) {
-      const int64_t m = std::min(total - a, kMostElems), c = (m + chunk_of(t.type) - 1) / chunk_of(t.type);
+    const int64_t parts = (total + kMostElems - 1) / kMostElems;
+    for (int64_t p = 0; p < parts; ++p) {
+      const int64_t a = (back ? parts - 1 - p : p) * kMostElems, m = std::min(total - a, kMostElems);
+      const char* out = t.out ? (const char*)t.out + a * oe : nullptr;
+      const char* in = (const char*)t.data + a * ie;
+      const int64_t shift = std::max(line_shift<char>(in, kInLine) / ie, line_shift<char>(out, kOutLine) / oe);
+      const int64_t c = (m + shift + chunk_of(t.type) - 1) / chunk_of(t.type);
       if (l.count == kList || (int64_t)chunks + c > INT32_MAX) flush();
-      l.in[l.count] = (const char*)t.data + a * ie;
-      l.out[l.count] = t.out ? (char*)t.out + a * oe : nullptr;
+      l.in[l.count] = in;
+      l.out[l.count] = (void*)out;
       l.len[l.count] = (uint32_t)m;
-      l.type[l.count] = (uint8_t)(t.type | (t.out_type == ELR_F32 && t.type != ELR_F32 ? 4 : 0));
+      l.type[l.count] = (uint32_t)(t.type | (t.out_type == ELR_F32 && t.type != ELR_F32 ? 4 : 0));
       chunks += (uint32_t)c;
       l.end[l.count++] = chunks;
     }
@@ -318,7 +357,7 @@ struct GradPlan {
 };
 static GradPlan grad_plan(const elr_grad* g, int64_t n) {
   GradPlan p;
-  each_launch(g, n, [&](const GradList*, const Strided*, int64_t c) { p.chunks += c, p.launches += 1; });
+  each_launch(g, n, false, [&](const GradList*, const Strided*, int64_t c) { p.chunks += c, p.launches += 1; });
   return p;
 }
 
@@ -329,22 +368,21 @@ static int run_grads(const elr_grad* g, int64_t n, bool scale, int write, float 
   double* part = (double*)scratch;
   if (bytes < plan.parts() * 8 || (plan.chunks && !scratch) || ((uintptr_t)scratch & 7u)) return ELR_ECAPACITY;
   int64_t at = 0;
-  each_launch(g, n, [&](const GradList* l, const Strided* s, int64_t c) {
+  each_launch(g, n, false, [&](const GradList* l, const Strided* s, int64_t c) {
     const unsigned b = (unsigned)plan.blocks(c);
     if (l) k_grad_sum<P><<<b, kGradThreads, 0, st>>>(*l, part + at);
     else k_grad_sum_strided<P><<<b, kGradThreads, 0, st>>>(*s, part + at);
     at += b;
   });
-  if (!scale || plan.launches == 0) {
-    k_grad_norm<P><<<1, kGradThreads, 0, st>>>(part, (int)at, norm);
-    return launch_status();
-  }
-  Clip k{part, (int)at, max_norm, eps, norm, write};
-  each_launch(g, n, [&](const GradList* l, const Strided* s, int64_t c) {
-    const unsigned b = (unsigned)plan.blocks(c);
+  // One launch of few blocks adds the partials up by itself; otherwise that is a launch, and a block has one chunk.
+  const bool own = scale && plan.launches == 1 && plan.chunks <= kOwnBlocks;
+  if (!own) k_grad_norm<P><<<1, kGradThreads, 0, st>>>(part, (int)at, norm);
+  if (!scale) return launch_status();
+  const Clip k{part, own ? (int)at : 0, max_norm, eps, norm, write};
+  each_launch(g, n, true, [&](const GradList* l, const Strided* s, int64_t c) {
+    const unsigned b = (unsigned)std::min(c, kScaleBlocks);
     if (l) k_grad_scale<P><<<b, kGradThreads, 0, st>>>(*l, k);
     else k_grad_scale_strided<P><<<b, kGradThreads, 0, st>>>(*s, k);
-    k.norm = nullptr;
   });
   return launch_status();
 }

@@ -18,8 +18,6 @@ namespace elr {
 
 constexpr float kFp8Max = 448.0f;
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 struct NormArgs {
   const void *x, *r, *w;       // r: residual or NULL; w: weight or NULL
   int64_t x_ld, r_ld;

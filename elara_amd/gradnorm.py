@@ -5,7 +5,7 @@ reference, whose step updates unclipped.
     clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None) -> norm   grads scaled by min(1, max_norm / (norm + eps))
 
 They run the HIP kernels behind elr_grad_norm and elr_clip_grad_norm (elara_amd/csrc/gradnorm.hip) on torch's current
-stream: two launches for up to 144 tensors, and no host synchronisation.  A batch's summed row gradients
+stream: two launches for up to 136 tensors, and no host synchronisation.  A batch's summed row gradients
 (dedup.embedding_dense_backward, dedup.segment_sum_plan) are one of the tensors.
 """
 import math
