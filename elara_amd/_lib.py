@@ -251,14 +251,14 @@ NOT_TAKEN = -1000   # _hostcall's answer for arguments the Python path has to lo
 
 class _NoHost:
     """Stands in for _hostcall where it is not built for this interpreter's torch: the Python path takes every call."""
-    adam = init = replay = staticmethod(lambda *a: NOT_TAKEN)
+    adam = init = replay = logprobs = logprobs_back = norm = norm_back = clip = staticmethod(lambda *a: NOT_TAKEN)
 
 
 _host = None
 
 
 def host():
-    """The native argument checks of the row ops (csrc/hostcall.cpp), bound to the loaded library.  Without the module,
+    """The native argument checks of the row ops and of the operators (csrc/hostcall.cpp), bound to the loaded library.  Without the module,
     or with one built for another torch or Python, a warning says so once and the Python path takes every call."""
     global _host
     if _host is None:
@@ -269,6 +269,10 @@ def host():
                 raise ImportError(f'built for torch {h.TORCH}, this is {torch.__version__}')
             h.bind(*(ctypes.cast(f, c_vp).value for f in (L.elr_adam_scalars, L.elr_adam_rows, L.elr_init_rows,
                                                           L.elr_replay_rows)))
+            h.bind_ops(*(ctypes.cast(getattr(L, 'elr_' + f), c_vp).value for f in (
+                'token_logprobs_scratch_bytes', 'token_logprobs', 'token_logprobs_backward', 'rms_norm',
+                'rms_norm_backward_scratch_bytes', 'rms_norm_backward', 'grad_norm_scratch_bytes', 'grad_norm',
+                'clip_grad_norm')))
         except ImportError as e:
             warnings.warn(f'elara_amd._hostcall is not used (small row-op calls take several microseconds longer): {e}',
                           stacklevel=3)

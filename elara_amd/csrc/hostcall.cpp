@@ -1,6 +1,6 @@
 // Host side of the row ops' Python entry points: the argument checks and the C-ABI call of ops.gpu_adam,
-// gpu_ops.init_rows and gpu_ops.replay_rows in one native call, for the arguments a training loop passes (plain
-// contiguous GPU tensors of the expected types on the current device).  Everything else -- other types, strides or
+// gpu_ops.init_rows and gpu_ops.replay_rows in one native call, and of the operators in logprobs, norms and gradnorm, for
+// the arguments a training loop passes (plain contiguous GPU tensors of the expected types on the current device).  Everything else -- other types, strides or
 // devices, arenas in host memory, wrapped tensors, errors -- is answered with NOT_TAKEN, and the Python path then
 // converts, raises or runs as it always has, so the two accept and refuse the same calls.
 //
@@ -11,7 +11,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
 #include <cstring>
+#include <vector>
 
 #include <ATen/ops/empty.h>
 #include <c10/core/DefaultDtype.h>
@@ -201,6 +203,296 @@ PyObject* replay(PyObject*, PyObject* const* a, Py_ssize_t na) {
   }
 }
 
+// ---- logprobs, norms, gradnorm
+
+decltype(&elr_token_logprobs_scratch_bytes) f_lp_bytes = nullptr;
+decltype(&elr_token_logprobs) f_lp = nullptr;
+decltype(&elr_token_logprobs_backward) f_lp_back = nullptr;
+decltype(&elr_rms_norm) f_norm = nullptr;
+decltype(&elr_rms_norm_backward_scratch_bytes) f_norm_bytes = nullptr;
+decltype(&elr_rms_norm_backward) f_norm_back = nullptr;
+decltype(&elr_grad_norm_scratch_bytes) f_grad_bytes = nullptr;
+decltype(&elr_grad_norm) f_grad_norm = nullptr;
+decltype(&elr_clip_grad_norm) f_clip = nullptr;
+
+template <class F>
+void set_address(F& f, unsigned long long a) {
+  f = reinterpret_cast<F>(a);
+}
+
+PyObject* bind_ops(PyObject*, PyObject* args) {
+  unsigned long long a[9];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8)) return nullptr;
+  set_address(f_lp_bytes, a[0]), set_address(f_lp, a[1]), set_address(f_lp_back, a[2]);
+  set_address(f_norm, a[3]), set_address(f_norm_bytes, a[4]), set_address(f_norm_back, a[5]);
+  set_address(f_grad_bytes, a[6]), set_address(f_grad_norm, a[7]), set_address(f_clip, a[8]);
+  Py_RETURN_NONE;
+}
+
+int elem_type(const at::Tensor& t) {   // ELR_F32, ELR_F16, ELR_BF16, or -1
+  switch (t.scalar_type()) {
+    case at::kFloat: return ELR_F32;
+    case at::kHalf: return ELR_F16;
+    case at::kBFloat16: return ELR_BF16;
+    default: return -1;
+  }
+}
+
+// None (sets t to nullptr) or a plain tensor; false: anything else.
+bool maybe(PyObject* o, const at::Tensor*& t) {
+  t = nullptr;
+  return o == Py_None || (t = plain(o)) != nullptr;
+}
+
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
+  return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+}
+
+// The scratch of a call (8-byte elements), undefined for none.
+at::Tensor scratch_on(const at::Tensor& like, int64_t bytes) {
+  return bytes > 0 ? empty_on(like, {(bytes + 7) / 8}, at::kDouble) : at::Tensor();
+}
+void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float* floats(const at::Tensor* t) { return t ? static_cast<const float*>(t->data_ptr()) : nullptr; }
+
+PyObject* wrap_or_none(const at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+
+// logprobs(logits, tokens, k) -> (return code, logprob, lse, entropy, top_logprob, top_id), or NOT_TAKEN
+PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 3 || !f_lp) return not_taken();
+  const at::Tensor *x = plain(a[0]), *tok = plain(a[1]);
+  int64_t k;
+  if (!x || !tok || !integer(a[2], k) || x->dim() < 1 || x->numel() == 0) return not_taken();
+  const int type = elem_type(*x);
+  const auto it = tok->scalar_type();
+  const int64_t V = x->size(-1), n = x->numel() / V;
+  if (type < 0 || (it != at::kInt && it != at::kLong) || tok->device() != x->device() ||
+      tok->sizes() != x->sizes().slice(0, x->dim() - 1) || k < 0 || k > V || k > ELR_TOPK_MAX)
+    return not_taken();
+  try {
+    at::Tensor lp, id, lse, ent, val;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x, st)) {
+        std::vector<int64_t> shape(tok->sizes().begin(), tok->sizes().end());
+        val = empty_on(*x, shape, at::kFloat), lse = empty_on(*x, shape, at::kFloat);
+        ent = empty_on(*x, shape, at::kFloat);
+        if (k) {
+          shape.push_back(k);
+          lp = empty_on(*x, shape, at::kFloat), id = empty_on(*x, shape, at::kLong);
+        }
+        const int64_t bytes = f_lp_bytes(n, V, static_cast<int>(k));
+        const at::Tensor scratch = scratch_on(*x, bytes);
+        rc = f_lp(x->data_ptr(), type, n, V, V, tok->data_ptr(), it == at::kLong, static_cast<int>(k),
+                  static_cast<float*>(val.data_ptr()), static_cast<float*>(lse.data_ptr()),
+                  static_cast<float*>(ent.data_ptr()), static_cast<float*>(data_or_null(lp)),
+                  static_cast<int64_t*>(data_or_null(id)), data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iNNNNN)", rc, THPVariable_Wrap(val), THPVariable_Wrap(lse), THPVariable_Wrap(ent),
+                         wrap_or_none(lp), wrap_or_none(id));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// logprobs_back(logits, tokens, lse, entropy, d_logprob, d_entropy, d_lse, out) -> (return code, out), or NOT_TAKEN
+PyObject* logprobs_back(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 8 || !f_lp_back) return not_taken();
+  const at::Tensor *x = plain(a[0]), *tok = plain(a[1]), *lse = plain(a[2]), *r[4], *out;
+  for (int i = 0; i < 4; ++i)
+    if (!maybe(a[3 + i], r[i])) return not_taken();
+  if (!x || !tok || !lse || !maybe(a[7], out) || x->dim() < 1 || x->numel() == 0) return not_taken();
+  const int type = elem_type(*x);
+  const auto it = tok->scalar_type();
+  const int64_t V = x->size(-1), n = x->numel() / V;
+  if (type < 0 || (it != at::kInt && it != at::kLong) || tok->device() != x->device() ||
+      tok->sizes() != x->sizes().slice(0, x->dim() - 1) || (r[2] && !r[0]))
+    return not_taken();
+  for (const at::Tensor* t : {lse, r[0], r[1], r[2], r[3]})
+    if (t && (t->scalar_type() != at::kFloat || t->device() != x->device() || t->sizes() != tok->sizes()))
+      return not_taken();
+  if (out && (out->scalar_type() != x->scalar_type() || out->device() != x->device() || out->sizes() != x->sizes()))
+    return not_taken();
+  try {
+    at::Tensor made;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x, st)) {
+        if (!out) made = empty_on(*x, x->sizes(), x->scalar_type());
+        rc = f_lp_back(x->data_ptr(), type, n, V, V, tok->data_ptr(), it == at::kLong, floats(lse),
+                       r[2] ? floats(r[0]) : nullptr, floats(r[1]), floats(r[2]), floats(r[3]),
+                       out ? out->data_ptr() : made.data_ptr(), V, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    if (!out) return Py_BuildValue("(iN)", rc, THPVariable_Wrap(made));
+    return Py_BuildValue("(iO)", rc, a[7]);
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// A weight of D elements for inputs of type `like` (None: ones); its type in `type`.
+bool weight_ok(const at::Tensor* w, const at::Tensor& like, int64_t D, int& type) {
+  type = elem_type(w ? *w : like);
+  return !w || ((w->scalar_type() == like.scalar_type() || w->scalar_type() == at::kFloat) && w->dim() == 1 &&
+                w->size(0) == D && w->device() == like.device());
+}
+
+// norm(x, weight, eps, residual, fp8, group) -> (return code, y, scale, h, rstd), or NOT_TAKEN
+PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 6 || !f_norm) return not_taken();
+  const at::Tensor *x = plain(a[0]), *w, *r;
+  double eps;
+  int64_t fp8, group;
+  if (!x || !maybe(a[1], w) || !real(a[2], eps) || !maybe(a[3], r) || !integer(a[4], fp8) || !integer(a[5], group) ||
+      x->dim() < 1 || x->numel() == 0)
+    return not_taken();
+  const int type = elem_type(*x);
+  const int64_t D = x->size(-1), n = x->numel() / D;
+  int wt, rt = type;
+  if (type < 0 || group < 0 || !weight_ok(w, *x, D, wt)) return not_taken();
+  if (r) {
+    rt = elem_type(*r);
+    if (r->sizes() != x->sizes() || r->device() != x->device() || (rt != type && rt != ELR_F32)) return not_taken();
+  }
+  try {
+    at::Tensor y, scale, h, rstd;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x, st)) {
+        std::vector<int64_t> lead(x->sizes().begin(), x->sizes().end() - 1);
+        y = empty_on(*x, x->sizes(), fp8 ? at::kFloat8_e4m3fn : x->scalar_type());
+        rstd = empty_on(*x, lead, at::kFloat);
+        if (r) h = empty_on(*x, x->sizes(), r->scalar_type());
+        if (fp8) {
+          lead.push_back(group ? D / group : 1);
+          scale = empty_on(*x, lead, at::kFloat);
+        }
+        rc = f_norm(x->data_ptr(), type, n, D, D, r ? r->data_ptr() : nullptr, rt, D, w ? w->data_ptr() : nullptr, wt,
+                    static_cast<float>(eps), y.data_ptr(), fp8 != 0, group, static_cast<float*>(data_or_null(scale)),
+                    data_or_null(h), static_cast<float*>(rstd.data_ptr()), st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    PyObject* ho = r ? THPVariable_Wrap(h) : (Py_INCREF(a[0]), a[0]);
+    return Py_BuildValue("(iNNNN)", rc, THPVariable_Wrap(y), wrap_or_none(scale), ho, THPVariable_Wrap(rstd));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// norm_back(dy, h, weight, rstd, dh, need_dweight) -> (return code, dx, dweight), or NOT_TAKEN
+PyObject* norm_back(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 6 || !f_norm_back) return not_taken();
+  const at::Tensor *dy = plain(a[0]), *h = plain(a[1]), *w, *rstd = plain(a[3]), *dh;
+  int64_t need;
+  if (!dy || !h || !rstd || !maybe(a[2], w) || !maybe(a[4], dh) || !integer(a[5], need) || dy->dim() < 1 ||
+      dy->numel() == 0)
+    return not_taken();
+  const int type = elem_type(*dy), ht = elem_type(*h);
+  const int64_t D = dy->size(-1), n = dy->numel() / D;
+  int wt;
+  if (type < 0 || (ht != type && ht != ELR_F32) || h->sizes() != dy->sizes() || h->device() != dy->device() ||
+      !weight_ok(w, *dy, D, wt) || rstd->scalar_type() != at::kFloat || rstd->device() != dy->device() ||
+      rstd->sizes() != dy->sizes().slice(0, dy->dim() - 1))
+    return not_taken();
+  if (dh && (dh->sizes() != h->sizes() || dh->scalar_type() != h->scalar_type() || dh->device() != h->device()))
+    return not_taken();
+  try {
+    at::Tensor dx, dw;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*dy, st)) {
+        dx = empty_on(*dy, h->sizes(), h->scalar_type());
+        at::Tensor scratch;
+        int64_t bytes = 0;
+        if (need) {
+          dw = empty_on(*dy, {D}, at::kFloat);
+          bytes = f_norm_bytes(n, D, type);
+          scratch = scratch_on(*dy, bytes);
+        }
+        rc = f_norm_back(dy->data_ptr(), type, n, D, D, h->data_ptr(), ht, D, dh ? dh->data_ptr() : nullptr, D,
+                         w ? w->data_ptr() : nullptr, wt, floats(rstd), dx.data_ptr(),
+                         static_cast<float*>(data_or_null(dw)), data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(dx), wrap_or_none(dw));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// clip(grads, out or None, kind, max_norm or None, eps) -> (return code, norm), or NOT_TAKEN; max_norm None: the norm alone
+PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 5 || !f_clip) return not_taken();
+  if (!(PyList_CheckExact(a[0]) || PyTuple_CheckExact(a[0])) ||
+      !(a[1] == Py_None || PyList_CheckExact(a[1]) || PyTuple_CheckExact(a[1])))
+    return not_taken();
+  int64_t kind;
+  double max_norm = 0, eps = 0;
+  const bool scale = a[3] != Py_None;
+  if (!integer(a[2], kind) || (scale && (!real(a[3], max_norm) || !real(a[4], eps)))) return not_taken();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(a[0]);
+  const bool outs = a[1] != Py_None;
+  if (n == 0 || (outs && PySequence_Fast_GET_SIZE(a[1]) != n)) return not_taken();
+  try {
+    std::vector<elr_grad> list(static_cast<size_t>(n));
+    std::vector<const void*> written;
+    written.reserve(static_cast<size_t>(n));
+    const at::Tensor* first = nullptr;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* to = PySequence_Fast_GET_ITEM(a[0], i);
+      PyObject* oo = outs ? PySequence_Fast_GET_ITEM(a[1], i) : to;
+      const at::Tensor *t = plain(to), *o = oo == to ? t : plain(oo);
+      if (!t || !o) return not_taken();
+      if (!first) first = t;
+      const int type = elem_type(*t), ot = elem_type(*o);
+      if (type < 0 || (ot != type && ot != ELR_F32) || t->device() != first->device() || o->device() != first->device() ||
+          (o != t && o->sizes() != t->sizes()))
+        return not_taken();
+      const int64_t m = t->numel();
+      list[static_cast<size_t>(i)] = elr_grad{t->data_ptr(), o->data_ptr(), 1, m, m, 1, m, 1, type, ot};
+      if (m) written.push_back(o->data_ptr());
+    }
+    std::sort(written.begin(), written.end());
+    if (scale && std::adjacent_find(written.begin(), written.end()) != written.end()) return not_taken();
+    at::Tensor norm;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*first, st)) {
+        norm = empty_on(*first, {}, at::kFloat);
+        const int64_t bytes = f_grad_bytes(list.data(), n);
+        const at::Tensor scratch = scratch_on(*first, bytes);
+        float* np = static_cast<float*>(norm.data_ptr());
+        rc = scale ? f_clip(list.data(), n, static_cast<int>(kind), static_cast<float>(max_norm),
+                            static_cast<float>(eps), np, data_or_null(scratch), bytes, st)
+                   : f_grad_norm(list.data(), n, static_cast<int>(kind), np, data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(norm));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
 #define ELR_STR1(x) #x
 #define ELR_STR(x) ELR_STR1(x)
 #define ELR_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -208,6 +500,12 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "Addresses of the library'
                          {"adam", ELR_FAST(adam), METH_FASTCALL, "elr_adam_rows with gpu_adam's checks."},
                          {"init", ELR_FAST(init), METH_FASTCALL, "elr_init_rows into a new tensor."},
                          {"replay", ELR_FAST(replay), METH_FASTCALL, "elr_replay_rows into a new tensor."},
+                         {"bind_ops", bind_ops, METH_VARARGS, "Addresses of the operators' entry points."},
+                         {"logprobs", ELR_FAST(logprobs), METH_FASTCALL, "elr_token_logprobs into new tensors."},
+                         {"logprobs_back", ELR_FAST(logprobs_back), METH_FASTCALL, "elr_token_logprobs_backward."},
+                         {"norm", ELR_FAST(norm), METH_FASTCALL, "elr_rms_norm into new tensors."},
+                         {"norm_back", ELR_FAST(norm_back), METH_FASTCALL, "elr_rms_norm_backward into new tensors."},
+                         {"clip", ELR_FAST(clip), METH_FASTCALL, "elr_clip_grad_norm or elr_grad_norm."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -69,6 +69,10 @@ def _kind(norm_type):
 
 
 def _run(grads, out, kind, clip):
+    r = (_lib._host or _lib.host()).clip(grads, out, kind, *(clip or (None, None)))
+    if r != _lib.NOT_TAKEN:
+        _lib.check(r[0], 'elr_clip_grad_norm' if clip else 'elr_grad_norm')
+        return r[1]
     grads, outs, dev, arr = _describe(grads, out)
     if clip:
         seen = set()

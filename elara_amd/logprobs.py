@@ -54,6 +54,11 @@ def token_logprobs(logits, tokens, k=0, check=False):
     check=True raises IndexError for a token >= V first, at the cost of a host synchronisation.  A row of nothing but -inf
     has logprob and lse -inf and entropy 0.  k (at most 32 and at most V): that many largest logits' ids, larger first and
     ties by the lower id, with their log probabilities."""
+    if not check:
+        r = (_lib._host or _lib.host()).logprobs(logits, tokens, k)
+        if r != _lib.NOT_TAKEN:
+            _lib.check(r[0], 'elr_token_logprobs')
+            return TokenLogprobs(*r[1:])
     x = _logits2d(logits, 'logits')
     tok = _tokens(tokens, logits)
     n, V = x.shape
@@ -95,6 +100,10 @@ def token_logprobs_backward(logits, tokens, lse, entropy, d_logprob, d_entropy=N
     float32's or bfloat16's lowest value, get 0.  out: where to write
     it, a tensor of the logits' shape and type whose rows lie apart by a fixed stride; the logits themselves are allowed,
     and are then overwritten."""
+    r = (_lib._host or _lib.host()).logprobs_back(logits, tokens, lse, entropy, d_logprob, d_entropy, d_lse, out)
+    if r != _lib.NOT_TAKEN:
+        _lib.check(r[0], 'elr_token_logprobs_backward')
+        return r[1]
     x = _logits2d(logits, 'logits')
     tok = _tokens(tokens, logits)
     n, V = x.shape

@@ -53,6 +53,10 @@ def _weight(w, x):
 
 
 def _norm(x, weight, eps, residual, fp8, group):
+    r = (_lib._host or _lib.host()).norm(x, weight, eps, residual, int(fp8), group)
+    if r != _lib.NOT_TAKEN:
+        _lib.check(r[0], 'elr_rms_norm')
+        return r[1:]
     xr = _rows(x, 'x', tuple(_lib.ETYPE))
     n, D = xr.shape
     dev, dt = x.device, x.dtype
@@ -99,6 +103,10 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dweight=True):
     """dy: y's gradient, in x's type; h, rstd: the forward's; dh (h's type and shape, or None): the gradient that arrives
     on the residual stream.  Returns (dx, dweight): dx in h's type, the gradient of x and of the residual alike (dh added);
     dweight float32 [D], summed in an order that depends on the sizes alone (None with need_dweight=False)."""
+    r = (_lib._host or _lib.host()).norm_back(dy, h, weight, rstd, dh, int(need_dweight))
+    if r != _lib.NOT_TAKEN:
+        _lib.check(r[0], 'elr_rms_norm_backward')
+        return r[1:]
     dyr = _rows(dy, 'dy', tuple(_lib.ETYPE))
     if h.shape != dy.shape or h.device != dy.device:
         raise RuntimeError(f'h must have shape {tuple(dy.shape)} on {dy.device}')
