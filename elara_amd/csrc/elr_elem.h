@@ -166,6 +166,35 @@ __device__ __forceinline__ float lanes_max_nan(float x, int width) {
   return x;
 }
 
+// Over the whole wave with data-parallel moves within it (no LDS), the same value in every lane; fixed order.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_or(float x, float none) {   // x of the lane that CTRL names; `none` where there is none
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(none), (int)__float_as_uint(x), CTRL,
+                                                               ROWS, 0xF, false));
+}
+__device__ __forceinline__ float last_lane(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = x + dpp_or<0x111, 0xF>(x, 0.0f);   // row_shr 1, 2, 4, 8: each row of 16 lanes into its last
+  x = x + dpp_or<0x112, 0xF>(x, 0.0f);
+  x = x + dpp_or<0x114, 0xF>(x, 0.0f);
+  x = x + dpp_or<0x118, 0xF>(x, 0.0f);
+  x = x + dpp_or<0x142, 0xA>(x, 0.0f);   // row_bcast 15 into rows 1 and 3
+  x = x + dpp_or<0x143, 0xC>(x, 0.0f);   // row_bcast 31 into rows 2 and 3
+  return last_lane(x);
+}
+__device__ __forceinline__ float wave_max(float x) {   // (a NaN is dropped)
+  constexpr float none = -__builtin_inff();
+  x = __builtin_fmaxf(x, dpp_or<0x111, 0xF>(x, none));
+  x = __builtin_fmaxf(x, dpp_or<0x112, 0xF>(x, none));
+  x = __builtin_fmaxf(x, dpp_or<0x114, 0xF>(x, none));
+  x = __builtin_fmaxf(x, dpp_or<0x118, 0xF>(x, none));
+  x = __builtin_fmaxf(x, dpp_or<0x142, 0xA>(x, none));
+  x = __builtin_fmaxf(x, dpp_or<0x143, 0xC>(x, none));
+  return last_lane(x);
+}
+
 inline int64_t elem_size(int type) { return type == ELR_F32 ? 4 : 2; }
 inline bool elem_type_ok(int type) { return type == ELR_F32 || type == ELR_F16 || type == ELR_BF16; }
 inline bool elem_aligned(const void* p, int type) { return ((uintptr_t)p & (uintptr_t)(elem_size(type) - 1)) == 0; }

@@ -11,11 +11,12 @@
 // fp32), so that e * (x - m) is 0 there too and not 0 * inf.  A row of nothing but -inf has s = 0: lse and logprob are
 // -inf, entropy 0, and no gradient.  A NaN (or +inf) anywhere gives NaN, as the formula does: the clamp keeps a NaN.
 //
-// The k likeliest (k <= 32) need no second pass over the row.  Each thread remembers the maximum of each of its chunks (in
-// LDS).  Among the 64 maxima of disjoint parts of the row the k-th largest is a lower bound of the row's k-th largest
-// element, so only chunks whose maximum reaches it are read again (about 64 ln(64 / (64 - k)) elements of a random row
-// reach it), and their elements that reach it are ranked.  Rows with more such elements than the lists hold (many
-// equal values, few unmasked ones) take the radix selection below: four counting passes, then the ties in index order.
+// The k likeliest (k <= 32) need no second pass over the row.  Among the maxima of 64 disjoint parts of it (the lanes', taken
+// anyway) the k-th largest is a lower bound of the row's k-th largest element; about 64 ln(64 / (64 - k)) elements of a
+// random row reach it.  A part that fits the block's registers is searched there.  A longer one keeps the maximum of each
+// thread's chunks in LDS, and only chunks whose maximum reaches the bound are read again, a vector per lane.  The elements
+// found are ranked.  Rows with more of them than the lists hold (many equal values, few unmasked ones) take the radix
+// selection below: four counting passes, then the ties in index order.
 // Order: larger first, ties by the lower id; -0 equals +0; a NaN ranks as -inf.
 #include "elr_elem.h"
 
@@ -29,6 +30,7 @@ constexpr int kMaxTop = ELR_TOPK_MAX;
 constexpr int kVecs = 4;        // 16-byte vectors a thread loads at a time (one chunk's step)
 constexpr int kChunks = 16;     // chunk maxima a thread keeps
 constexpr int kAbove = 448, kTies = 64;   // candidate lists
+constexpr int kHits = 256;      // chunks read again
 constexpr int kMaxSplits = 64;
 
 __device__ __forceinline__ float exp_nat(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
@@ -97,6 +99,10 @@ __device__ __forceinline__ int lane_rank(uint32_t key) {
   for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
   return rank;
 }
+__device__ __forceinline__ uint64_t lane_of(uint64_t x, int j) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), j) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)x, j);
+}
 
 // Candidates of one block: order and id packed so that a larger number comes first (ties: the lower id).
 __device__ __forceinline__ uint64_t pack_cand(uint32_t o, uint32_t id) { return (uint64_t)o << 32 | (uint32_t)~id; }
@@ -105,15 +111,18 @@ template <int T>
 struct TopShared {
   float gmax[T];                  // thread maxima
   uint64_t above[kAbove], ties[kTies];
-  int n_above, n_ties;
+  int n_above, n_ties, n_hits;
+  uint32_t thr;
+  uint32_t hits[kHits];           // chunk * T + thread
   uint32_t hist[256];
   int scan[T / 64 + 1];
 };
 
 template <class E, int T>
 struct RowPart {
-  const E* p;        // the split's first element
+  const E* p;           // the split's first element
   int32_t first, len;   // its place in the row and its length
+  int32_t shift;        // elements between the start of p's memory line and p: vectors are laid from there
 };
 
 // The elements of the part that satisfy `pred(order)`, counted over the whole block into *count, in no order.
@@ -187,56 +196,79 @@ __device__ uint32_t radix_kth(const RowPart<E, T>& r, TopShared<T>& sh, int k) {
   return prefix;
 }
 
-// The k likeliest of a part, in order, through out(rank, packed).  cm: the thread's chunk maxima (column threadIdx.x of
-// [kChunks][T]); m: the thread's maximum.
-template <class E, int T, class Out>
-__device__ void top_of(const LpArgs& a, const RowPart<E, T>& r, TopShared<T>& sh, const float* cm, int steps, float m,
-                       const Out& out) {
-  constexpr int VE = Elem<E>::VE;
-  const int k = a.k, lane = threadIdx.x & 63;
-  sh.gmax[threadIdx.x] = m;
-  if (threadIdx.x == 0) sh.n_above = sh.n_ties = 0;
-  __syncthreads();
-  float g = sh.gmax[lane];
+// The order of a lower bound of the block's k-th largest element (its low 6 bits cut off, which only lowers it), the same in
+// every thread, from the threads' maxima.
+template <int T>
+__device__ __forceinline__ uint32_t lower_bound(TopShared<T>& sh, float m, int k) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (T > 64) {
+    sh.gmax[threadIdx.x] = m;
+    __syncthreads();
+    if (threadIdx.x < 64) {
 #pragma unroll
-  for (int w = 1; w < T / 64; ++w) g = __builtin_fmaxf(g, sh.gmax[w * 64 + lane]);
-  // the low 6 bits make the keys distinct; what they cut off only lowers the bound
-  const uint32_t key = (order_of(g) & ~63u) | (uint32_t)(63 - lane);
-  const uint64_t at = __builtin_amdgcn_ballot_w64(lane_rank(key) == k - 1);
-  const uint32_t thr = (uint32_t)__builtin_amdgcn_readlane((int)key, __builtin_ctzll(at)) & ~63u;
-  const uint32_t floor_ord = 0x007FFFFFu;   // order_of(-inf)
-  const float thr_f = thr <= floor_ord ? -__builtin_inff() : value_of(thr);
-  for (int c = 0; c * a.per_chunk < steps; ++c) {
-    if (!(cm[c * T] >= thr_f)) continue;
-    const int end = min(steps, (c + 1) * a.per_chunk);
-    for (int it = c * a.per_chunk; it < end; ++it) {
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u) {
-        const int64_t e = ((int64_t)(it * kVecs + u) * T + threadIdx.x) * VE;
-        if (e >= r.len) break;
-        const Frag<E> x = widen<E>(load_raw<E, false>(r.p + e, r.len - e, 0.0f));
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const uint32_t o = order_of(x.v[j]);
-          if (o < thr || e + j >= r.len) continue;
-          if ((o & ~63u) > thr) {
-            const int i = atomicAdd(&sh.n_above, 1);
-            if (i < kAbove) sh.above[i] = pack_cand(o, (uint32_t)(r.first + e + j));
-          } else {
-            const int i = atomicAdd(&sh.n_ties, 1);
-            if (i < kTies) sh.ties[i] = pack_cand(o, (uint32_t)(r.first + e + j));
-          }
-        }
-      }
+      for (int w = 1; w < T / 64; ++w) m = __builtin_fmaxf(m, sh.gmax[w * 64 + lane]);
+    }
+  }
+  uint32_t thr = 0;
+  if (T == 64 || threadIdx.x < 64) {
+    const uint32_t key = (order_of(m) & ~63u) | (uint32_t)(63 - lane);   // distinct
+    const uint64_t at = __builtin_amdgcn_ballot_w64(lane_rank(key) == k - 1);
+    thr = (uint32_t)__builtin_amdgcn_readlane((int)key, __builtin_ctzll(at)) & ~63u;
+    if (lane == 0) {
+      sh.n_above = sh.n_ties = sh.n_hits = 0;
+      sh.thr = thr;
     }
   }
   __syncthreads();
+  return T > 64 ? sh.thr : thr;
+}
+
+// An element that reaches the bound into its list: above it, or in the bound's own class.
+template <int T>
+__device__ __forceinline__ void push_cand(TopShared<T>& sh, float x, uint32_t thr, int32_t id) {
+  const uint32_t o = order_of(x);
+  if ((o & ~63u) > thr) {
+    const int i = atomicAdd(&sh.n_above, 1);
+    if (i < kAbove) sh.above[i] = pack_cand(o, (uint32_t)id);
+  } else {
+    const int i = atomicAdd(&sh.n_ties, 1);
+    if (i < kTies) sh.ties[i] = pack_cand(o, (uint32_t)id);
+  }
+}
+
+// The nc candidates (distinct) of `at` ranked by one wave if they fit it, else by the block; out(rank, candidate) of the
+// first k.
+template <int T, class At, class Out>
+__device__ __forceinline__ void rank_cands(int nc, int k, const At& at, const Out& out) {
+  if (nc <= 64) {
+    if (threadIdx.x >= 64) return;
+    const uint64_t c = (int)threadIdx.x < nc ? at(threadIdx.x) : 0;
+    int rank = 0;
+    for (int j = 0; j < nc; ++j) rank += lane_of(c, j) > c;
+    if ((int)threadIdx.x < nc && rank < k) out(rank, c);
+    return;
+  }
+  for (int i = threadIdx.x; i < nc; i += T) {
+    const uint64_t c = at(i);
+    int rank = 0;
+    for (int j = 0; j < nc; ++j) rank += at(j) > c;
+    if (rank < k) out(rank, c);
+  }
+}
+
+// The k likeliest of a part from the lists, in order, through out(rank, packed); thr: the bound the lists were filled by.
+// lost: more chunks than the hit list holds reach the bound, and the lists are not whole.
+template <class E, int T, class Out>
+__device__ __forceinline__ void finish_top(int k, const RowPart<E, T>& r, TopShared<T>& sh, uint32_t thr, const Out& out) {
+  constexpr uint32_t floor_ord = 0x007FFFFFu;   // order_of(-inf)
+  __syncthreads();
   int na = sh.n_above, nt = sh.n_ties;
-  if (na > kAbove || nt > kTies) {
+  const bool lost = sh.n_hits > kHits;
+  if (lost || na > kAbove || nt > kTies) {
     // 16-bit types and -inf: the bound is one value, so its ties in index order complete the list
     const int want = min(k, r.len);
     uint32_t kth = thr < 0x80000000u ? thr | 63u : thr;   // (a negative value's order has ones there)
-    if (na > kAbove || (sizeof(E) == 4 && thr > floor_ord)) {
+    if (lost || na > kAbove || (sizeof(E) == 4 && thr > floor_ord)) {
       kth = radix_kth<E, T>(r, sh, want);
       if (threadIdx.x == 0) sh.n_above = 0;
       __syncthreads();
@@ -250,13 +282,7 @@ __device__ void top_of(const LpArgs& a, const RowPart<E, T>& r, TopShared<T>& sh
     nt = sh.n_ties;
   }
   const int nc = na + nt;
-  for (int i = threadIdx.x; i < nc; i += T) {
-    const uint64_t c = i < na ? sh.above[i] : sh.ties[i - na];
-    int rank = 0;
-    for (int j = 0; j < na; ++j) rank += sh.above[j] > c;
-    for (int j = 0; j < nt; ++j) rank += sh.ties[j] > c;
-    if (rank < k) out(rank, c);
-  }
+  rank_cands<T>(nc, k, [&](int i) { return i < na ? sh.above[i] : sh.ties[i - na]; }, out);
   for (int i = nc + threadIdx.x; i < k; i += T) out(i, (uint64_t)0);   // a part shorter than k
 }
 
@@ -267,35 +293,175 @@ __device__ __forceinline__ void write_top(const LpArgs& a, int64_t row, int rank
   a.top_id[row * a.k + rank] = (int64_t)(uint32_t)~(uint32_t)c;
 }
 
-// One block of T threads per (row, split).
+// A wave's lanes' sums put together, the same in every lane.
+__device__ __forceinline__ Sums wave_join(const Sums& q) {
+  Sums r;
+  r.m = wave_max(q.m);
+  const float d = clamp_low(q.m - exp_ref(r.m)), f = exp_nat(d);
+  r.s = wave_sum(q.s * f);
+  r.t = wave_sum((q.t + q.s * d) * f);
+  return r;
+}
+template <int T>
+__device__ __forceinline__ Sums block_join(Sums q, Sums* waves) {
+  q = wave_join(q);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = q;
+    __syncthreads();
+    q = waves[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) q = join(q, waves[w]);
+  }
+  return q;
+}
+
+template <class E, int T>
+__device__ __forceinline__ RowPart<E, T> part_of(const LpArgs& a, int64_t row, int split) {
+  RowPart<E, T> r;
+  r.first = split * a.seg;
+  r.len = min(a.seg, a.V - r.first);
+  r.p = (const E*)a.x + row * a.ld + r.first;
+  r.shift = line_shift<E>(r.p, 128);
+  return r;
+}
+
+// The part's results: the row's if it is not split.
+template <class E, int T, bool TOP, class Fill>
+__device__ __forceinline__ void part_done(const LpArgs& a, int64_t row, int64_t unit, const RowPart<E, T>& r,
+                                          TopShared<TOP ? T : 64>& sh, const Sums& q, bool has, float x_tok,
+                                          float mine, const Fill& fill) {
+  if (a.splits == 1) {
+    if (threadIdx.x == 0) write_row(a, row, q, has, x_tok);
+  } else if (threadIdx.x == 0) {
+    a.part[unit * 3] = q.m;
+    a.part[unit * 3 + 1] = q.s;
+    a.part[unit * 3 + 2] = q.t;
+  }
+  if constexpr (TOP) {
+    const uint32_t thr = lower_bound<T>(sh, mine, a.k);
+    const float thr_f = thr <= 0x007FFFFFu ? -__builtin_inff() : value_of(thr);
+    fill(thr, thr_f);
+    if (a.splits == 1) {
+      const float logs = __builtin_logf(q.s);
+      finish_top<E, T>(a.k, r, sh, thr, [&](int rank, uint64_t c) {
+        write_top(a, row, rank, c, q.m, logs, q.s == 0.0f);
+      });
+    } else {
+      finish_top<E, T>(a.k, r, sh, thr, [&](int rank, uint64_t c) { a.part_top[unit * a.k + rank] = c; });
+    }
+  }
+}
+
+// The row's token and its logit, loaded by the first thread while the row is on its way.
+template <class E>
+__device__ __forceinline__ bool token_logit(const LpArgs& a, int64_t row, float& x) {
+  x = 0.0f;
+  if (a.splits != 1 || threadIdx.x != 0) return false;
+  const int64_t tok = token_at(a, row);
+  if (tok < 0 || tok >= a.V) return false;
+  x = to_f32(((const E*)a.x)[row * a.ld + tok]);
+  return true;
+}
+
+// A part of up to T * NV vectors: it stays in registers, and no sum is rescaled.
+template <class E, int T, int NV, bool TOP>
+__global__ __launch_bounds__(T) void k_lp_one(LpArgs a) {
+  constexpr int VE = Elem<E>::VE;
+  __shared__ Sums waves[T / 64];
+  __shared__ float wmax[T / 64];
+  __shared__ TopShared<TOP ? T : 64> sh;
+  const int64_t unit = blockIdx.x;
+  const int64_t row = a.splits == 1 ? unit : unit / a.splits;
+  const RowPart<E, T> r = part_of<E, T>(a, row, a.splits == 1 ? 0 : (int)(unit - row * a.splits));
+  const int64_t e0 = (int64_t)threadIdx.x * VE - r.shift;
+  u32x4 raw[NV];
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+    raw[u] = load_part<E, true>(r.p, e0 + (int64_t)u * T * VE, r.len, -__builtin_inff());
+  float x_tok;
+  const bool has = token_logit<E>(a, row, x_tok);
+  Frag<E> x[NV];
+  Sums q{-__builtin_inff(), 0.0f, 0.0f};
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    x[u] = widen<E>(raw[u]);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) q.m = __builtin_fmaxf(q.m, x[u].v[j]);
+  }
+  const float mine = q.m;
+  q.m = wave_max(q.m);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = q.m;
+    __syncthreads();
+    q.m = wmax[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) q.m = __builtin_fmaxf(q.m, wmax[w]);
+  }
+  const float ref = exp_ref(q.m);
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float d = clamp_low(x[u].v[j] - ref);
+      const float e = exp_nat(d);
+      q.s = q.s + e;
+      q.t = __builtin_fmaf(e, d, q.t);
+    }
+  q.s = wave_sum(q.s);
+  q.t = wave_sum(q.t);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = q;
+    __syncthreads();
+    q = waves[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) {
+      q.s = q.s + waves[w].s;
+      q.t = q.t + waves[w].t;
+    }
+  }
+  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, [&](uint32_t thr, float thr_f) {
+    if constexpr (TOP) {
+      if (!(mine >= thr_f)) return;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          const int64_t e = e0 + (int64_t)u * T * VE + j;
+          const float v = x[u].v[j];
+          if ((v >= thr_f || (v != v && thr <= 0x007FFFFFu)) && e >= 0 && e < r.len)
+            push_cand(sh, v, thr, r.first + (int32_t)e);
+        }
+    }
+  });
+}
+
+// A longer part, T * kVecs vectors at a time.
 template <class E, int T, bool TOP>
 __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
   constexpr int VE = Elem<E>::VE;
+  constexpr int64_t kStep = (int64_t)T * kVecs * VE;
   __shared__ float cmax[TOP ? kChunks * T : 1];
   __shared__ Sums waves[T / 64];
   __shared__ TopShared<TOP ? T : 64> sh;
   const int64_t unit = blockIdx.x;
   const int64_t row = a.splits == 1 ? unit : unit / a.splits;
-  const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
-  RowPart<E, T> r;
-  r.first = split * a.seg;
-  r.len = min(a.seg, a.V - r.first);
-  r.p = (const E*)a.x + row * a.ld + r.first;
-  const int steps = (int)(((int64_t)r.len + (int64_t)T * kVecs * VE - 1) / ((int64_t)T * kVecs * VE));
+  const RowPart<E, T> r = part_of<E, T>(a, row, a.splits == 1 ? 0 : (int)(unit - row * a.splits));
+  const int steps = (int)((r.len + r.shift + kStep - 1) / kStep);
+  float x_tok;
+  const bool has = token_logit<E>(a, row, x_tok);
   Sums q{-__builtin_inff(), 0.0f, 0.0f};
   float ck = -__builtin_inff();   // the current chunk's maximum
   int in_chunk = 0, chunk = 0;
   for (int it = 0; it < steps; ++it) {
-    const int64_t e0 = ((int64_t)it * kVecs * T + threadIdx.x) * VE;
+    const int64_t s0 = it * kStep - r.shift, e0 = s0 + (int64_t)threadIdx.x * VE;
     u32x4 raw[kVecs];
-    if ((int64_t)(it + 1) * kVecs * T * VE <= r.len) {
+    if (s0 >= 0 && s0 + kStep <= r.len) {
 #pragma unroll
       for (int u = 0; u < kVecs; ++u) raw[u] = load_raw<E, true>(r.p + e0 + (int64_t)u * T * VE, VE, 0.0f);
     } else {
 #pragma unroll
       for (int u = 0; u < kVecs; ++u)
-        raw[u] = load_raw<E, true>(r.p + e0 + (int64_t)u * T * VE, r.len - e0 - (int64_t)u * T * VE,
-                                   -__builtin_inff());
+        raw[u] = load_part<E, true>(r.p, e0 + (int64_t)u * T * VE, r.len, -__builtin_inff());
     }
     Frag<E> x[kVecs];
     float c = -__builtin_inff();
@@ -331,95 +497,83 @@ __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
     }
   }
   const float mine = q.m;
-  for (int o = 1; o < 64; o <<= 1) {
-    Sums b;
-    b.m = __shfl_xor(q.m, o, 64);
-    b.s = __shfl_xor(q.s, o, 64);
-    b.t = __shfl_xor(q.t, o, 64);
-    q = join(q, b);
-  }
-  if constexpr (T > 64) {
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = q;
-    __syncthreads();
-    q = waves[0];
-#pragma unroll
-    for (int w = 1; w < T / 64; ++w) q = join(q, waves[w]);
-  }
-  if (a.splits == 1) {
-    if (threadIdx.x == 0) {
-      const int64_t tok = token_at(a, row);
-      const bool has = tok >= 0 && tok < a.V;
-      write_row(a, row, q, has, has ? to_f32(((const E*)a.x)[row * a.ld + tok]) : 0.0f);
-    }
+  q = block_join<T>(q, waves);
+  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, [&](uint32_t thr, float thr_f) {
     if constexpr (TOP) {
-      const float logs = __builtin_logf(q.s);
-      top_of<E, T>(a, r, sh, cmax + threadIdx.x, steps, mine, [&](int rank, uint64_t c) {
-        write_top(a, row, rank, c, q.m, logs, q.s == 0.0f);
-      });
+      // the chunks that reach the bound ...
+      if (mine >= thr_f)
+        for (int c = 0; c < chunk; ++c)
+          if (cmax[c * T + threadIdx.x] >= thr_f) {
+            const int i = atomicAdd(&sh.n_hits, 1);
+            if (i < kHits) sh.hits[i] = (uint32_t)(c * T) + threadIdx.x;
+          }
+      __syncthreads();
+      const int nh = sh.n_hits;
+      if (nh > kHits) return;
+      // ... read again, one vector a thread at a time
+      const int per = a.per_chunk * kVecs, tasks = nh * per;
+      for (int i = threadIdx.x; i < tasks; i += T) {
+        const int h = i / per, v = i - h * per;
+        const uint32_t hit = sh.hits[h];
+        const int64_t vec = ((int64_t)(hit / T) * per + v) * T + hit % T;
+        const int64_t e = vec * VE - r.shift;
+        const Frag<E> x = widen<E>(load_part<E, false>(r.p, e, r.len, -__builtin_inff()));
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if ((x.v[j] >= thr_f || (x.v[j] != x.v[j] && thr <= 0x007FFFFFu)) && e + j >= 0 && e + j < r.len)
+            push_cand(sh, x.v[j], thr, r.first + (int32_t)(e + j));
+      }
     }
-  } else {
-    if (threadIdx.x == 0) {
-      a.part[unit * 3] = q.m;
-      a.part[unit * 3 + 1] = q.s;
-      a.part[unit * 3 + 2] = q.t;
-    }
-    if constexpr (TOP)
-      top_of<E, T>(a, r, sh, cmax + threadIdx.x, steps, mine,
-                   [&](int rank, uint64_t c) { a.part_top[unit * a.k + rank] = c; });
-  }
+  });
 }
 
-// The splits of a row joined: lane i holds split i's sums and its sorted candidates.  A candidate below the k-th largest
-// of the splits' first candidates cannot be among the row's k, which leaves at most k (k - 1) + 1.
+// The splits of a row joined: lane i holds split i's sums and its first candidate.  A candidate below the k-th largest of
+// the splits' first ones cannot be among the row's k, which leaves at most k (k - 1) + 1.
 constexpr int kJoinThreads = 256;
 template <class E>
 __global__ __launch_bounds__(kJoinThreads) void k_lp_join(LpArgs a) {
-  __shared__ uint64_t cand[kMaxTop * (kMaxTop - 1) + 1];
-  __shared__ uint64_t heads[kMaxSplits];
+  constexpr int kMost = kMaxTop * (kMaxTop - 1) + 1, kEach = kMaxSplits * kMaxTop / kJoinThreads;
+  __shared__ uint64_t cand[kMost];
   __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63, S = a.splits;
+  const int lane = threadIdx.x & 63, S = a.splits, all = S * a.k;
+  const uint64_t* top = a.part_top + row * S * a.k;
+  uint64_t mine[kEach], head = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = i * kJoinThreads + threadIdx.x;
+    mine[i] = j < all ? top[j] : 0;
+  }
+  if (a.k && lane < S) head = top[lane * a.k];
   Sums q{-__builtin_inff(), 0.0f, 0.0f};
   if (lane < S) {
     const float* p = a.part + (row * S + lane) * 3;
     q = Sums{p[0], p[1], p[2]};
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    Sums b;
-    b.m = __shfl_xor(q.m, o, 64);
-    b.s = __shfl_xor(q.s, o, 64);
-    b.t = __shfl_xor(q.t, o, 64);
-    q = join(q, b);
-  }
+  bool has = false;
+  float x_tok = 0.0f;
   if (threadIdx.x == 0) {
     const int64_t tok = token_at(a, row);
-    const bool has = tok >= 0 && tok < a.V;
-    write_row(a, row, q, has, has ? to_f32(((const E*)a.x)[row * a.ld + tok]) : 0.0f);
+    has = tok >= 0 && tok < a.V;
+    if (has) x_tok = to_f32(((const E*)a.x)[row * a.ld + tok]);
     count = 0;
   }
+  q = wave_join(q);
+  if (threadIdx.x == 0) write_row(a, row, q, has, x_tok);
   if (a.k == 0) return;
-  const uint64_t* top = a.part_top + row * S * a.k;
-  if (threadIdx.x < kMaxSplits) heads[threadIdx.x] = threadIdx.x < S ? top[(int64_t)threadIdx.x * a.k] : 0;
   __syncthreads();
-  const uint64_t mine = heads[lane];
-  int rank = 0;      // ties (absent heads are 0) by the lane
-  for (int j = 0; j < S; ++j) rank += heads[j] > mine || (heads[j] == mine && j < lane);
+  int rank = 0;      // heads of splits are distinct and not 0; the lanes past them are
+  for (int j = 0; j < S; ++j) rank += lane_of(head, j) > head;
   const uint64_t at = __builtin_amdgcn_ballot_w64(rank == a.k - 1 && lane < S);
-  const uint64_t thr = at ? heads[__builtin_ctzll(at)] : 0;   // fewer than k splits: every candidate
-  const int all = S * a.k;
-  for (int i = threadIdx.x; i < all; i += kJoinThreads) {
-    const uint64_t c = top[i];
-    if (c != 0 && c >= thr) cand[atomicAdd(&count, 1)] = c;
-  }
+  const uint64_t thr = at ? lane_of(head, __builtin_ctzll(at)) : 0;   // fewer than k splits: every candidate
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (mine[i] != 0 && mine[i] >= thr) cand[atomicAdd(&count, 1)] = mine[i];
   __syncthreads();
-  const int nc = count;
   const float logs = __builtin_logf(q.s);
-  for (int i = threadIdx.x; i < nc; i += kJoinThreads) {
-    const uint64_t c = cand[i];
-    int r = 0;
-    for (int j = 0; j < nc; ++j) r += cand[j] > c;
-    if (r < a.k) write_top(a, row, r, c, q.m, logs, q.s == 0.0f);
-  }
+  rank_cands<kJoinThreads>(count, a.k, [&](int i) { return cand[i]; }, [&](int r, uint64_t c) {
+    write_top(a, row, r, c, q.m, logs, q.s == 0.0f);
+  });
 }
 
 // d x_v = [v = a] g + p_v (z - g - h (log p_v + H)), p = e^(x - lse): one read and one write of the logits, in place too.
@@ -440,22 +594,18 @@ constexpr int kBackVecs = 4;
 // for log V and e^(x - lse) would be 1 for each of the V.  Such a row gets no gradient.
 constexpr float kEmptyLse = -0x1.0p+100f;
 
-template <class E, int U>
-__global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
+// A wave's vectors of a row, from element e0 of lane 0 on; ALL: every one lies within the row.
+template <class E, int U, bool ALL>
+__device__ __forceinline__ void back_vecs(const LpBackArgs& a, int64_t row, const E* x, E* out, int64_t s0) {
   constexpr int VE = Elem<E>::VE;
   const int lane = threadIdx.x & 63;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4u + (threadIdx.x >> 6)));
-  const uint32_t in = wave / (uint32_t)a.chunks;
-  const int chunk = (int)(wave - in * (uint32_t)a.chunks);
-  const int64_t row = row0 + in;
-  if (row >= a.n) return;
-  const E* x = (const E*)a.x + row * a.ld;
-  E* out = (E*)a.out + row * a.out_ld;
-  const int64_t e0 = (int64_t)chunk * 64 * U * VE + lane * VE;
+  const int64_t e0 = s0 + lane * VE;
   u32x4 raw[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    raw[u] = load_raw<E, true>(x + e0 + u * 64 * VE, a.V - e0 - u * 64 * VE, -__builtin_inff());
+  for (int u = 0; u < U; ++u) {
+    if constexpr (ALL) raw[u] = load_raw<E, true>(x + e0 + u * 64 * VE, VE, 0.0f);
+    else raw[u] = load_part<E, true>(x, e0 + u * 64 * VE, a.V, -__builtin_inff());
+  }
   const int64_t tok = a.idx64 ? ((const int64_t*)a.tokens)[row] : (int64_t)((const int32_t*)a.tokens)[row];
   const bool has = tok >= 0 && tok < a.V;
   const float g = has && a.d_logprob ? a.d_logprob[row] : 0.0f;
@@ -467,7 +617,6 @@ __global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t e = e0 + u * 64 * VE;
-    if (e >= a.V) break;
     Frag<E> y = widen<E>(raw[u]);
     const int at = has && tok >= e && tok < e + VE ? (int)(tok - e) : -1;
 #pragma unroll
@@ -476,12 +625,30 @@ __global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
       const float d = exp_nat(logp) * __builtin_fmaf(-h, logp, c0);
       y.v[j] = empty ? 0.0f : j == at ? d + g : d;
     }
-    store_raw<E, true>(out + e, narrow<E>(y), a.V - e);
+    if constexpr (ALL) store_raw<E, true>(out + e, narrow<E>(y), VE);
+    else store_part<E, true>(out, e, a.V, narrow<E>(y));
   }
+}
+
+// Chunks of 64 * U vectors, one wave each, laid from the memory line in which the output's row starts.
+template <class E, int U>
+__global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
+  constexpr int VE = Elem<E>::VE;
+  constexpr int64_t kChunk = 64 * U * VE;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4u + (threadIdx.x >> 6)));
+  const uint32_t in = wave / (uint32_t)a.chunks;
+  const int64_t row = row0 + in;
+  if (row >= a.n) return;
+  const E* x = (const E*)a.x + row * a.ld;
+  E* out = (E*)a.out + row * a.out_ld;
+  const int64_t s0 = (int64_t)(wave - in * (uint32_t)a.chunks) * kChunk - line_shift<E>(out, 128);
+  if (s0 >= 0 && s0 + kChunk <= a.V) back_vecs<E, U, true>(a, row, x, out, s0);
+  else back_vecs<E, U, false>(a, row, x, out, s0);
 }
 
 // ---- host side
 
+constexpr int kThreads = 256;
 constexpr int64_t kSplitMin = 8192;       // elements of a split, at least
 constexpr int64_t kSplitBlocks = 1024;    // blocks that splitting aims at
 
@@ -494,23 +661,29 @@ static int lp_splits(int64_t n, int64_t V) {
 
 constexpr int64_t kRowsPerLaunch = 1 << 22;
 
+template <class E, bool TOP>
+static void launch_part(const LpArgs& a, unsigned blocks, hipStream_t st) {
+  constexpr int64_t VE = Elem<E>::VE, line = 128 / sizeof(E) - 1;   // a part may start anywhere in a line
+  const int64_t most = (int64_t)a.seg + line;
+  if (most <= 64 * VE) k_lp_one<E, 64, 1, TOP><<<blocks, 64, 0, st>>>(a);
+  else if (most <= 128 * VE) k_lp_one<E, 64, 2, TOP><<<blocks, 64, 0, st>>>(a);
+  else if (most <= 256 * VE) k_lp_one<E, 64, 4, TOP><<<blocks, 64, 0, st>>>(a);
+  else if (most <= kThreads * 2 * VE) k_lp_one<E, kThreads, 2, TOP><<<blocks, kThreads, 0, st>>>(a);
+  else if (most <= kThreads * 4 * VE) k_lp_one<E, kThreads, 4, TOP><<<blocks, kThreads, 0, st>>>(a);
+  else k_lp_rows<E, kThreads, TOP><<<blocks, kThreads, 0, st>>>(a);
+}
+
 template <class E>
 static void launch_rows(LpArgs a, hipStream_t st) {
   constexpr int VE = Elem<E>::VE;
-  a.seg = ((a.V + a.splits - 1) / a.splits + VE - 1) / VE * VE;
+  constexpr int64_t line = 128 / sizeof(E);
+  a.seg = (int32_t)(((a.V + a.splits - 1) / a.splits + line - 1) / line * line);
   a.splits = (a.V + a.seg - 1) / a.seg;
-  const bool small = a.V <= 64 * VE * kVecs;
-  const int64_t T = small ? 64 : 256;
-  const int64_t steps = (a.seg + T * kVecs * VE - 1) / (T * kVecs * VE);
+  const int64_t steps = (a.seg + line + kThreads * kVecs * VE - 1) / (kThreads * kVecs * VE);
   a.per_chunk = (int)((steps + kChunks - 1) / kChunks);
   const unsigned blocks = (unsigned)(a.n * a.splits);
-  if (small) {
-    if (a.k) k_lp_rows<E, 64, true><<<blocks, 64, 0, st>>>(a);
-    else k_lp_rows<E, 64, false><<<blocks, 64, 0, st>>>(a);
-  } else {
-    if (a.k) k_lp_rows<E, 256, true><<<blocks, 256, 0, st>>>(a);
-    else k_lp_rows<E, 256, false><<<blocks, 256, 0, st>>>(a);
-  }
+  if (a.k) launch_part<E, true>(a, blocks, st);
+  else launch_part<E, false>(a, blocks, st);
   if (a.splits > 1) k_lp_join<E><<<(unsigned)a.n, kJoinThreads, 0, st>>>(a);
 }
 
@@ -518,9 +691,11 @@ template <class E>
 static void launch_back(const LpBackArgs& a0, hipStream_t st) {
   constexpr int VE = Elem<E>::VE;
   LpBackArgs a = a0;
-  const bool one = a.V <= 64 * VE;
+  const bool lines = a.out_ld * (int64_t)sizeof(E) % 128 == 0 && line_shift<E>(a.out, 128) == 0;
+  const int64_t most = (int64_t)a.V + (lines ? 0 : 128 / sizeof(E) - 1);
+  const bool one = most <= 64 * VE;
   const int64_t per = 64 * VE * (one ? 1 : kBackVecs);
-  a.chunks = (int32_t)((a.V + per - 1) / per);
+  a.chunks = (int32_t)((most + per - 1) / per);
   const int64_t rows = (int64_t)1 << 28;          // waves of a launch
   const int64_t step = rows / a.chunks < 1 ? 1 : rows / a.chunks;
   for (int64_t r = 0; r < a.n; r += step) {
