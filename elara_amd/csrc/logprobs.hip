@@ -29,8 +29,14 @@ constexpr float kExpFloor = -1e4f;
 constexpr int kMaxTop = ELR_TOPK_MAX;
 constexpr int kVecs = 4;        // 16-byte vectors a thread loads at a time (one chunk's step)
 constexpr int kChunks = 16;     // chunk maxima a thread keeps
-constexpr int kAbove = 448, kTies = 64;   // candidate lists
-constexpr int kHits = 256;      // chunks read again
+// Candidate lists, and vectors or chunks that hold candidates: of a block, and of a wave by itself (whose LDS bounds how many
+// run at once: 10.5 KB a wave was 4 waves a SIMD).
+template <int T>
+constexpr int kAbove = T > 64 ? 448 : 128;
+constexpr int kTies = 64;
+template <int T>
+constexpr int kHits = T > 64 ? 256 : 80;
+constexpr uint32_t kFloorOrd = 0x007FFFFFu;   // order_of(-inf)
 constexpr int kMaxSplits = 64;
 
 __device__ __forceinline__ float exp_nat(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
@@ -75,7 +81,7 @@ struct LpArgs {
   int idx64, k;
   float *logprob, *lse, *entropy, *top_logprob;
   int64_t* top_id;
-  float* part;                 // [n * splits][3] partial (m, s, t)
+  float* part;                 // [n * splits][4] partial (m, s, t) and the token's logit, if the split holds it
   uint64_t* part_top;          // [n * splits][k] candidates: order in the high half, ~id in the low
 };
 
@@ -92,12 +98,21 @@ __device__ __forceinline__ void write_row(const LpArgs& a, int64_t row, const Su
   a.logprob[row] = !has ? 0.0f : empty ? -__builtin_inff() : (x_tok - r.m) - logs;
 }
 
-// A rank among the 64 lanes' distinct keys (0: the largest).
-__device__ __forceinline__ int lane_rank(uint32_t key) {
-  int rank = 0;
+// Bits of an order that tell values of the type apart (the others are all 0 or all 1).
+template <class E>
+constexpr uint32_t kBits = sizeof(E) == 4 ? ~0u : Elem<E>::kType == ELR_BF16 ? 0xFFFF0000u : 0xFFFFE000u;
+
+// The k-th largest of the 64 lanes' orders, bit by bit (its low bits 0 where kBits has none).
+template <class E>
+__device__ __forceinline__ uint32_t wave_kth(uint32_t o, int k) {
+  uint32_t t = 0;
 #pragma unroll
-  for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j) > key;
-  return rank;
+  for (int b = 31; (kBits<E> >> b & 1u) != 0 && b >= 0; --b) {
+    const uint32_t c = t | 1u << b;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(o >= c)) >= k) t = c;
+    if (b == 0) break;
+  }
+  return t;
 }
 __device__ __forceinline__ uint64_t lane_of(uint64_t x, int j) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), j) << 32 |
@@ -110,11 +125,14 @@ __device__ __forceinline__ uint64_t pack_cand(uint32_t o, uint32_t id) { return 
 template <int T>
 struct TopShared {
   float gmax[T];                  // thread maxima
-  uint64_t above[kAbove], ties[kTies];
+  uint64_t above[kAbove<T>], ties[kTies];
   int n_above, n_ties, n_hits;
   uint32_t thr;
-  uint32_t hits[kHits];           // chunk * T + thread
-  uint32_t hist[256];
+  uint32_t hits[kHits<T>];        // a vector's number, or chunk * T + thread
+  union {
+    u32x4 vecs[kHits<T>];         // the vectors themselves (parts held in registers)
+    uint32_t hist[256];           // of the radix selection, when they are done with
+  };
   int scan[T / 64 + 1];
 };
 
@@ -196,43 +214,55 @@ __device__ uint32_t radix_kth(const RowPart<E, T>& r, TopShared<T>& sh, int k) {
   return prefix;
 }
 
-// The order of a lower bound of the block's k-th largest element (its low 6 bits cut off, which only lowers it), the same in
-// every thread, from the threads' maxima.
-template <int T>
-__device__ __forceinline__ uint32_t lower_bound(TopShared<T>& sh, float m, int k) {
+// The order of a lower bound of the block's k-th largest element (the bits of kBits), the same in every thread, from the
+// threads' maxima m; most: the block's maximum.
+template <class E, int T>
+__device__ __forceinline__ uint32_t lower_bound(TopShared<T>& sh, float m, float most, int k) {
   const int lane = threadIdx.x & 63;
-  if constexpr (T > 64) {
-    sh.gmax[threadIdx.x] = m;
-    __syncthreads();
-    if (threadIdx.x < 64) {
+  if (threadIdx.x == 0) sh.n_above = sh.n_ties = sh.n_hits = 0;
+  uint32_t thr = order_of(most) & kBits<E>;
+  if (k > 1) {
+    if constexpr (T > 64) {
+      sh.gmax[threadIdx.x] = m;
+      __syncthreads();
+      if (threadIdx.x < 64) {
 #pragma unroll
-      for (int w = 1; w < T / 64; ++w) m = __builtin_fmaxf(m, sh.gmax[w * 64 + lane]);
+        for (int w = 1; w < T / 64; ++w) m = __builtin_fmaxf(m, sh.gmax[w * 64 + lane]);
+      }
     }
-  }
-  uint32_t thr = 0;
-  if (T == 64 || threadIdx.x < 64) {
-    const uint32_t key = (order_of(m) & ~63u) | (uint32_t)(63 - lane);   // distinct
-    const uint64_t at = __builtin_amdgcn_ballot_w64(lane_rank(key) == k - 1);
-    thr = (uint32_t)__builtin_amdgcn_readlane((int)key, __builtin_ctzll(at)) & ~63u;
-    if (lane == 0) {
-      sh.n_above = sh.n_ties = sh.n_hits = 0;
-      sh.thr = thr;
+    if (T == 64 || threadIdx.x < 64) {
+      thr = wave_kth<E>(order_of(m), k);
+      if (T > 64 && lane == 0) sh.thr = thr;
     }
   }
   __syncthreads();
-  return T > 64 ? sh.thr : thr;
+  return T > 64 && k > 1 ? sh.thr : thr;
 }
 
-// An element that reaches the bound into its list: above it, or in the bound's own class.
-template <int T>
-__device__ __forceinline__ void push_cand(TopShared<T>& sh, float x, uint32_t thr, int32_t id) {
-  const uint32_t o = order_of(x);
-  if ((o & ~63u) > thr) {
-    const int i = atomicAdd(&sh.n_above, 1);
-    if (i < kAbove) sh.above[i] = pack_cand(o, (uint32_t)id);
-  } else {
-    const int i = atomicAdd(&sh.n_ties, 1);
-    if (i < kTies) sh.ties[i] = pack_cand(o, (uint32_t)id);
+// The elements of a vector that reach the bound (thr_f) into the lists: above the bound's order, or equal to it.  Every
+// place in a list is taken before the first is written, so that the waits for them overlap.
+template <class E, int T>
+__device__ __forceinline__ void push_vec(TopShared<T>& sh, const Frag<E>& x, uint32_t thr, float thr_f, int32_t id) {
+  constexpr int VE = Elem<E>::VE;
+  int at[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j) {
+    at[j] = -1;
+    if (x.v[j] >= thr_f) {
+      const uint32_t o = order_of(x.v[j]);
+      at[j] = atomicAdd((o & kBits<E>) > thr ? &sh.n_above : &sh.n_ties, 1);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VE; ++j) {
+    if (at[j] < 0) continue;
+    const uint32_t o = order_of(x.v[j]);
+    const uint64_t c = pack_cand(o, (uint32_t)(id + j));
+    if ((o & kBits<E>) > thr) {
+      if (at[j] < kAbove<T>) sh.above[at[j]] = c;
+    } else {
+      if (at[j] < kTies) sh.ties[at[j]] = c;
+    }
   }
 }
 
@@ -256,30 +286,34 @@ __device__ __forceinline__ void rank_cands(int nc, int k, const At& at, const Ou
   }
 }
 
-// The k likeliest of a part from the lists, in order, through out(rank, packed); thr: the bound the lists were filled by.
-// lost: more chunks than the hit list holds reach the bound, and the lists are not whole.
+// The k likeliest of a part from the lists, in order, through out(rank, packed); thr: the bound they were filled by.  With a
+// bound of -inf they hold what lies above it only.  More hits or ties than the lists hold: the bound is one value, so the
+// elements above it are collected again, if need be above a bound that at most k of them reach, and its ties follow in
+// index order.
 template <class E, int T, class Out>
 __device__ __forceinline__ void finish_top(int k, const RowPart<E, T>& r, TopShared<T>& sh, uint32_t thr, const Out& out) {
-  constexpr uint32_t floor_ord = 0x007FFFFFu;   // order_of(-inf)
   __syncthreads();
   int na = sh.n_above, nt = sh.n_ties;
-  const bool lost = sh.n_hits > kHits;
-  if (lost || na > kAbove || nt > kTies) {
-    // 16-bit types and -inf: the bound is one value, so its ties in index order complete the list
+  const bool lost = sh.n_hits > kHits<T>;
+  if (lost || na > kAbove<T> || nt > kTies || thr <= kFloorOrd) {
     const int want = min(k, r.len);
-    uint32_t kth = thr < 0x80000000u ? thr | 63u : thr;   // (a negative value's order has ones there)
-    if (lost || na > kAbove || (sizeof(E) == 4 && thr > floor_ord)) {
-      kth = radix_kth<E, T>(r, sh, want);
+    uint32_t kth = thr < 0x80000000u ? thr | ~kBits<E> : thr;   // (a negative value's order has ones there)
+    for (int pass = 0; pass < 2 && (na > kAbove<T> || (pass == 0 && lost)); ++pass) {
+      if (pass || !lost) kth = radix_kth<E, T>(r, sh, want);
+      __syncthreads();
       if (threadIdx.x == 0) sh.n_above = 0;
       __syncthreads();
-      each_elem<E, T>(r, [&](uint32_t o, uint32_t id) {   // fewer than k elements
-        if (o > kth) sh.above[atomicAdd(&sh.n_above, 1)] = pack_cand(o, id);
+      each_elem<E, T>(r, [&](uint32_t o, uint32_t id) {
+        if (o > kth) {
+          const int i = atomicAdd(&sh.n_above, 1);
+          if (i < kAbove<T>) sh.above[i] = pack_cand(o, id);
+        }
       });
       __syncthreads();
       na = sh.n_above;
     }
-    ordered_ties<E, T>(r, sh, kth, want);
-    nt = sh.n_ties;
+    if (na < want) ordered_ties<E, T>(r, sh, kth, want - na);
+    nt = na < want ? sh.n_ties : 0;
   }
   const int nc = na + nt;
   rank_cands<T>(nc, k, [&](int i) { return i < na ? sh.above[i] : sh.ties[i - na]; }, out);
@@ -333,13 +367,11 @@ __device__ __forceinline__ void part_done(const LpArgs& a, int64_t row, int64_t 
   if (a.splits == 1) {
     if (threadIdx.x == 0) write_row(a, row, q, has, x_tok);
   } else if (threadIdx.x == 0) {
-    a.part[unit * 3] = q.m;
-    a.part[unit * 3 + 1] = q.s;
-    a.part[unit * 3 + 2] = q.t;
+    *(f32x4*)(a.part + unit * 4) = (f32x4){q.m, q.s, q.t, x_tok};
   }
   if constexpr (TOP) {
-    const uint32_t thr = lower_bound<T>(sh, mine, a.k);
-    const float thr_f = thr <= 0x007FFFFFu ? -__builtin_inff() : value_of(thr);
+    const uint32_t thr = lower_bound<E, T>(sh, mine, q.m, a.k);
+    const float thr_f = thr <= kFloorOrd ? -0x1.fffffep+127f : value_of(thr);   // -inf: what is above it
     fill(thr, thr_f);
     if (a.splits == 1) {
       const float logs = __builtin_logf(q.s);
@@ -352,14 +384,14 @@ __device__ __forceinline__ void part_done(const LpArgs& a, int64_t row, int64_t 
   }
 }
 
-// The row's token and its logit, loaded by the first thread while the row is on its way.
-template <class E>
-__device__ __forceinline__ bool token_logit(const LpArgs& a, int64_t row, float& x) {
+// Whether the part holds the row's token, and its logit: loaded by the first thread while the row is on its way.
+template <class E, int T>
+__device__ __forceinline__ bool token_logit(const LpArgs& a, int64_t row, const RowPart<E, T>& r, float& x) {
   x = 0.0f;
-  if (a.splits != 1 || threadIdx.x != 0) return false;
-  const int64_t tok = token_at(a, row);
-  if (tok < 0 || tok >= a.V) return false;
-  x = to_f32(((const E*)a.x)[row * a.ld + tok]);
+  if (threadIdx.x != 0) return false;
+  const int64_t tok = token_at(a, row) - r.first;
+  if (tok < 0 || tok >= r.len) return false;
+  x = to_f32(r.p[tok]);
   return true;
 }
 
@@ -379,14 +411,17 @@ __global__ __launch_bounds__(T) void k_lp_one(LpArgs a) {
   for (int u = 0; u < NV; ++u)
     raw[u] = load_part<E, true>(r.p, e0 + (int64_t)u * T * VE, r.len, -__builtin_inff());
   float x_tok;
-  const bool has = token_logit<E>(a, row, x_tok);
+  const bool has = token_logit<E, T>(a, row, r, x_tok);
   Frag<E> x[NV];
+  float vmax[NV];
   Sums q{-__builtin_inff(), 0.0f, 0.0f};
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     x[u] = widen<E>(raw[u]);
+    vmax[u] = x[u].v[0];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) q.m = __builtin_fmaxf(q.m, x[u].v[j]);
+    for (int j = 1; j < VE; ++j) vmax[u] = __builtin_fmaxf(vmax[u], x[u].v[j]);
+    q.m = __builtin_fmaxf(q.m, vmax[u]);
   }
   const float mine = q.m;
   q.m = wave_max(q.m);
@@ -421,16 +456,21 @@ __global__ __launch_bounds__(T) void k_lp_one(LpArgs a) {
   }
   part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, [&](uint32_t thr, float thr_f) {
     if constexpr (TOP) {
-      if (!(mine >= thr_f)) return;
+      // the vectors that reach the bound to LDS, then a vector per thread
 #pragma unroll
       for (int u = 0; u < NV; ++u)
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const int64_t e = e0 + (int64_t)u * T * VE + j;
-          const float v = x[u].v[j];
-          if ((v >= thr_f || (v != v && thr <= 0x007FFFFFu)) && e >= 0 && e < r.len)
-            push_cand(sh, v, thr, r.first + (int32_t)e);
+        if (vmax[u] >= thr_f) {
+          const int i = atomicAdd(&sh.n_hits, 1);
+          if (i < kHits<T>) {
+            sh.hits[i] = (uint32_t)(u * T) + threadIdx.x;
+            sh.vecs[i] = raw[u];
+          }
         }
+      __syncthreads();
+      const int nh = sh.n_hits;
+      if (nh > kHits<T>) return;
+      for (int i = threadIdx.x; i < nh; i += T)
+        push_vec<E, T>(sh, widen<E>(sh.vecs[i]), thr, thr_f, r.first + (int32_t)sh.hits[i] * VE - r.shift);
     }
   });
 }
@@ -448,7 +488,7 @@ __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
   const RowPart<E, T> r = part_of<E, T>(a, row, a.splits == 1 ? 0 : (int)(unit - row * a.splits));
   const int steps = (int)((r.len + r.shift + kStep - 1) / kStep);
   float x_tok;
-  const bool has = token_logit<E>(a, row, x_tok);
+  const bool has = token_logit<E, T>(a, row, r, x_tok);
   Sums q{-__builtin_inff(), 0.0f, 0.0f};
   float ck = -__builtin_inff();   // the current chunk's maximum
   int in_chunk = 0, chunk = 0;
@@ -505,11 +545,11 @@ __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
         for (int c = 0; c < chunk; ++c)
           if (cmax[c * T + threadIdx.x] >= thr_f) {
             const int i = atomicAdd(&sh.n_hits, 1);
-            if (i < kHits) sh.hits[i] = (uint32_t)(c * T) + threadIdx.x;
+            if (i < kHits<T>) sh.hits[i] = (uint32_t)(c * T) + threadIdx.x;
           }
       __syncthreads();
       const int nh = sh.n_hits;
-      if (nh > kHits) return;
+      if (nh > kHits<T>) return;
       // ... read again, one vector a thread at a time
       const int per = a.per_chunk * kVecs, tasks = nh * per;
       for (int i = threadIdx.x; i < tasks; i += T) {
@@ -518,19 +558,16 @@ __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
         const int64_t vec = ((int64_t)(hit / T) * per + v) * T + hit % T;
         const int64_t e = vec * VE - r.shift;
         const Frag<E> x = widen<E>(load_part<E, false>(r.p, e, r.len, -__builtin_inff()));
-#pragma unroll
-        for (int j = 0; j < VE; ++j)
-          if ((x.v[j] >= thr_f || (x.v[j] != x.v[j] && thr <= 0x007FFFFFu)) && e + j >= 0 && e + j < r.len)
-            push_cand(sh, x.v[j], thr, r.first + (int32_t)(e + j));
+        push_vec<E, T>(sh, x, thr, thr_f, r.first + (int32_t)e);
       }
     }
   });
 }
 
-// The splits of a row joined: lane i holds split i's sums and its first candidate.  A candidate below the k-th largest of
-// the splits' first ones cannot be among the row's k, which leaves at most k (k - 1) + 1.
+// The splits of a row joined: lane i holds split i's sums.  The splits' sorted candidates fall into up to 64 runs, at least k,
+// and a candidate below the k-th largest of the runs' first ones cannot be among the row's k; of k candidates a run, that
+// leaves at most k (k - 1) + 1.
 constexpr int kJoinThreads = 256;
-template <class E>
 __global__ __launch_bounds__(kJoinThreads) void k_lp_join(LpArgs a) {
   constexpr int kMost = kMaxTop * (kMaxTop - 1) + 1, kEach = kMaxSplits * kMaxTop / kJoinThreads;
   __shared__ uint64_t cand[kMost];
@@ -539,33 +576,34 @@ __global__ __launch_bounds__(kJoinThreads) void k_lp_join(LpArgs a) {
   const int lane = threadIdx.x & 63, S = a.splits, all = S * a.k;
   const uint64_t* top = a.part_top + row * S * a.k;
   uint64_t mine[kEach], head = 0;
+  float x_tok = 0.0f;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int j = i * kJoinThreads + threadIdx.x;
     mine[i] = j < all ? top[j] : 0;
   }
-  if (a.k && lane < S) head = top[lane * a.k];
+  const int runs = kMaxSplits / S, each = (a.k + runs - 1) / runs;   // of a split
+  const int sp = lane / runs, in = (lane - sp * runs) * each;
+  if (sp < S && in < a.k) head = top[sp * a.k + in];
   Sums q{-__builtin_inff(), 0.0f, 0.0f};
   if (lane < S) {
-    const float* p = a.part + (row * S + lane) * 3;
+    const f32x4 p = *(const f32x4*)(a.part + (row * S + lane) * 4);
     q = Sums{p[0], p[1], p[2]};
+    x_tok = p[3];
   }
-  bool has = false;
-  float x_tok = 0.0f;
-  if (threadIdx.x == 0) {
-    const int64_t tok = token_at(a, row);
-    has = tok >= 0 && tok < a.V;
-    if (has) x_tok = to_f32(((const E*)a.x)[row * a.ld + tok]);
-    count = 0;
-  }
+  const int64_t tok = token_at(a, row);
+  const bool has = tok >= 0 && tok < a.V;
+  x_tok = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x_tok), has ? (int)(tok / a.seg) : 0));
+  if (threadIdx.x == 0) count = 0;
   q = wave_join(q);
   if (threadIdx.x == 0) write_row(a, row, q, has, x_tok);
   if (a.k == 0) return;
   __syncthreads();
-  int rank = 0;      // heads of splits are distinct and not 0; the lanes past them are
-  for (int j = 0; j < S; ++j) rank += lane_of(head, j) > head;
-  const uint64_t at = __builtin_amdgcn_ballot_w64(rank == a.k - 1 && lane < S);
-  const uint64_t thr = at ? lane_of(head, __builtin_ctzll(at)) : 0;   // fewer than k splits: every candidate
+  int rank = 0;      // distinct, but for those of no run, which are 0
+#pragma unroll 8
+  for (int j = 0; j < 64; ++j) rank += lane_of(head, j) > head;
+  const uint64_t at = __builtin_amdgcn_ballot_w64(rank == a.k - 1);
+  const uint64_t thr = at ? lane_of(head, __builtin_ctzll(at)) : 0;   // fewer than k runs: every candidate
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
     if (mine[i] != 0 && mine[i] >= thr) cand[atomicAdd(&count, 1)] = mine[i];
@@ -662,12 +700,12 @@ static int lp_splits(int64_t n, int64_t V) {
 constexpr int64_t kRowsPerLaunch = 1 << 22;
 
 template <class E, bool TOP>
-static void launch_part(const LpArgs& a, unsigned blocks, hipStream_t st) {
-  constexpr int64_t VE = Elem<E>::VE, line = 128 / sizeof(E) - 1;   // a part may start anywhere in a line
-  const int64_t most = (int64_t)a.seg + line;
+static void launch_part(const LpArgs& a, int64_t most, unsigned blocks, hipStream_t st) {
+  constexpr int64_t VE = Elem<E>::VE;
   if (most <= 64 * VE) k_lp_one<E, 64, 1, TOP><<<blocks, 64, 0, st>>>(a);
   else if (most <= 128 * VE) k_lp_one<E, 64, 2, TOP><<<blocks, 64, 0, st>>>(a);
-  else if (most <= 256 * VE) k_lp_one<E, 64, 4, TOP><<<blocks, 64, 0, st>>>(a);
+  else if (most <= 256 * VE && a.splits == 1) k_lp_one<E, 64, 4, TOP><<<blocks, 64, 0, st>>>(a);
+  else if (most <= kThreads * VE) k_lp_one<E, kThreads, 1, TOP><<<blocks, kThreads, 0, st>>>(a);
   else if (most <= kThreads * 2 * VE) k_lp_one<E, kThreads, 2, TOP><<<blocks, kThreads, 0, st>>>(a);
   else if (most <= kThreads * 4 * VE) k_lp_one<E, kThreads, 4, TOP><<<blocks, kThreads, 0, st>>>(a);
   else k_lp_rows<E, kThreads, TOP><<<blocks, kThreads, 0, st>>>(a);
@@ -679,12 +717,15 @@ static void launch_rows(LpArgs a, hipStream_t st) {
   constexpr int64_t line = 128 / sizeof(E);
   a.seg = (int32_t)(((a.V + a.splits - 1) / a.splits + line - 1) / line * line);
   a.splits = (a.V + a.seg - 1) / a.seg;
-  const int64_t steps = (a.seg + line + kThreads * kVecs * VE - 1) / (kThreads * kVecs * VE);
+  // a part's vectors start at its memory line: up to a line less one element more than its own
+  const bool lines = line_shift<E>(a.x, 128) == 0 && (a.n == 1 || a.ld % line == 0);
+  const int64_t most = a.seg + (lines ? 0 : line - 1);
+  const int64_t steps = (most + kThreads * kVecs * VE - 1) / (kThreads * kVecs * VE);
   a.per_chunk = (int)((steps + kChunks - 1) / kChunks);
   const unsigned blocks = (unsigned)(a.n * a.splits);
-  if (a.k) launch_part<E, true>(a, blocks, st);
-  else launch_part<E, false>(a, blocks, st);
-  if (a.splits > 1) k_lp_join<E><<<(unsigned)a.n, kJoinThreads, 0, st>>>(a);
+  if (a.k) launch_part<E, true>(a, most, blocks, st);
+  else launch_part<E, false>(a, most, blocks, st);
+  if (a.splits > 1) k_lp_join<<<(unsigned)a.n, kJoinThreads, 0, st>>>(a);
 }
 
 template <class E>
@@ -722,7 +763,7 @@ extern "C" int64_t elr_token_logprobs_scratch_bytes(int64_t n, int64_t V, int k)
   if (n == 0) return 0;
   const int64_t s = elr::lp_splits(n, V);
   if (s == 1) return 0;
-  return (n * s * 12 + 7) / 8 * 8 + n * s * k * 8;
+  return n * s * (16 + k * 8);
 }
 
 extern "C" int elr_token_logprobs(const void* logits, int type, int64_t n, int64_t V, int64_t ld, const void* tokens,
@@ -735,13 +776,13 @@ extern "C" int elr_token_logprobs(const void* logits, int type, int64_t n, int64
   if (n == 0) return ELR_OK;
   if (!tokens || !logprob || !lse || !entropy || (k && (!top_logprob || !top_id))) return ELR_EINVAL;
   const int64_t need = elr_token_logprobs_scratch_bytes(n, V, k);
-  if (need > 0 && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 7u))) return ELR_ECAPACITY;
+  if (need > 0 && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 15u))) return ELR_ECAPACITY;
   LpArgs a{};
   a.x = logits, a.ld = ld, a.n = n, a.V = (int32_t)V, a.splits = lp_splits(n, V);
   a.tokens = tokens, a.idx64 = idx64, a.k = k;
   a.logprob = logprob, a.lse = lse, a.entropy = entropy, a.top_logprob = top_logprob, a.top_id = top_id;
   a.part = (float*)scratch;
-  a.part_top = (uint64_t*)((char*)scratch + (n * a.splits * 12 + 7) / 8 * 8);
+  a.part_top = (uint64_t*)((char*)scratch + n * a.splits * 16);
   hipStream_t st = (hipStream_t)stream;
   for (int64_t r = 0; r < n; r += kRowsPerLaunch) {   // one launch unless n is huge (then a row is no longer split)
     a.n = n - r < kRowsPerLaunch ? n - r : kRowsPerLaunch;

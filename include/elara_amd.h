@@ -742,7 +742,7 @@ int elr_mark_rows(const int64_t* rows, const int64_t* n_dev, int64_t n_max, int3
  * -inf and entropy 0; a NaN or +inf in a row makes its fp32 results NaN, and a NaN ranks as -inf among the top ids.
  *   logits of `type` (ELR_F32, ELR_F16, ELR_BF16), row i at logits + i * ld elements (ld may exceed V, or be 0);
  *   tokens int32 (idx64 = 0) or int64 (1) [n]; logprob, lse, entropy fp32 [n]; scratch of
- *   elr_token_logprobs_scratch_bytes(n, V, k) bytes, 8-byte aligned (may be 0; -1: bad argument).
+ *   elr_token_logprobs_scratch_bytes(n, V, k) bytes, 16-byte aligned (may be 0; -1: bad argument).
  * ------------------------------------------------------------------------------------------------------- */
 #define ELR_TOPK_MAX 32
 int64_t elr_token_logprobs_scratch_bytes(int64_t n, int64_t V, int k);
