@@ -151,19 +151,35 @@ __device__ __forceinline__ float to_f32(E x) { return (float)x; }
 // max(a, b) that is NaN if either is (torch's amax); __builtin_fmaxf drops a NaN.
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Sum and maximum over aligned groups of `width` lanes (a power of two up to 64); every lane gets the result.  The order
-// of the additions is fixed.
-__device__ __forceinline__ float lanes_sum(float x, int width) {
-  for (int o = 1; o < width; o <<= 1) x = x + __shfl_xor(x, o, 64);
+// x of the partner lane at distance 1, 2, 4, 8 (within a row of 16 lanes, for values that are alike below that distance),
+// 16 and 32, moved within the vector unit (ds_bpermute, what a shuffle is, waits for LDS at each step).
+template <int CTRL>
+__device__ __forceinline__ float dpp_of(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+// op over aligned groups of `width` lanes (a power of two up to 64, the same in the whole wave); every lane gets the result.
+// op is commutative, so both partners compute the same bits; the order is fixed.
+template <class F>
+__device__ __forceinline__ float lanes_op(float x, int width, const F& op) {
+  if (width > 1) x = op(x, dpp_of<0xB1>(x));     // quad_perm 1, 0, 3, 2
+  if (width > 2) x = op(x, dpp_of<0x4E>(x));     // quad_perm 2, 3, 0, 1
+  if (width > 4) x = op(x, dpp_of<0x141>(x));    // row_half_mirror
+  if (width > 8) x = op(x, dpp_of<0x140>(x));    // row_mirror
+  if (width > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if (width > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
   return x;
 }
-__device__ __forceinline__ float lanes_max(float x, int width) {
-  for (int o = 1; o < width; o <<= 1) x = __builtin_fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
+__device__ __forceinline__ float lanes_sum(float x, int width) {
+  return lanes_op(x, width, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float lanes_max_nan(float x, int width) {
-  for (int o = 1; o < width; o <<= 1) x = max_nan(x, __shfl_xor(x, o, 64));
-  return x;
+  return lanes_op(x, width, [](float a, float b) { return max_nan(a, b); });
 }
 
 // Over the whole wave with data-parallel moves within it (no LDS), the same value in every lane; fixed order.

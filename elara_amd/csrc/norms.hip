@@ -9,9 +9,14 @@
 //
 // The norm is taken of the unrounded fp32 sum h; h itself is rounded once, when it is stored.  Sums are fp32.
 //
-// Layout.  A row lies in the registers of a team: 2^lg lanes of one wave (rows of up to 64 vectors of 16 bytes: several
-// rows a wave), a wave, or a block, NV vectors a lane; vector j * team + lane.  It is read once and written once.  Rows
-// too long for a block's registers (k_norm_long) are read again from the caches for the output.
+// Layout.  A row lies in the registers of a team: 2^lg lanes of one wave (rows of up to 64 vectors of 16 bytes: several rows
+// a wave), a wave, or a block, NV vectors a lane; vector j * team + lane.  It is read once and written once.  Rows too long
+// for a block's registers (k_norm_long) are read again from the caches for the output.
+//
+// Loads are non-temporal (read once), stores are not: 16,384 rows of 4,096 bf16 with a residual (537 MB) take 80 us (6.7
+// TB/s), with non-temporal stores 83, with plain loads too 91.  The backward of the same rows: 85 us and 5 for the sum of the
+// weight gradients (6.0 TB/s); 425,984 rows of 128 fp32: 107 us and 5 (5.9 TB/s).  fp8 of 8,192 rows of 2,048 with groups of
+// 128 (118 MB): 25 us (4.7 TB/s, of which a launch is 3 us).
 #include "elr_elem.h"
 
 namespace elr {
@@ -83,11 +88,36 @@ __device__ __forceinline__ void res_store(R* p, const Frag<E>& f, int64_t valid)
     Frag<R> b;
 #pragma unroll
     for (int j = 0; j < Elem<R>::VE; ++j) b.v[j] = f.v[q * Elem<R>::VE + j];
-    store_raw<R, true>(p + q * Elem<R>::VE, narrow<R>(b), valid - q * Elem<R>::VE);
+    store_raw<R, false>(p + q * Elem<R>::VE, narrow<R>(b), valid - q * Elem<R>::VE);
   }
 }
 
-// e4m3 of VE values already divided by their scale, at p.  The clamp takes the half ulp that a division may round up by.
+// The scale of values up to m, and what divides by it: a product with the reciprocal, or a division where that overflows
+// (scales below 2^-128).  (A division for each value took 32 us where this takes 27,
+// for 8,192 rows of 2,048.)
+struct Scale {
+  float s, inv;
+  bool exact;
+};
+__device__ __forceinline__ Scale scale_of(float m) {
+  Scale r;
+  r.s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
+  r.inv = 1.0f / r.s;
+  r.exact = !(r.inv < __builtin_inff());
+  return r;
+}
+template <class E>
+__device__ __forceinline__ void divide(Frag<E>& h, const Scale& k) {
+  if (k.exact) {
+#pragma unroll
+    for (int j = 0; j < Elem<E>::VE; ++j) h.v[j] = h.v[j] / k.s;
+  } else {
+#pragma unroll
+    for (int j = 0; j < Elem<E>::VE; ++j) h.v[j] = h.v[j] * k.inv;
+  }
+}
+
+// e4m3 of VE values already divided by their scale, at p.  The clamp takes what rounding may put above 448.
 template <class E>
 __device__ __forceinline__ void store_fp8(uint8_t* p, const Frag<E>& f, int64_t valid) {
   constexpr int VE = Elem<E>::VE;
@@ -141,11 +171,11 @@ __device__ __forceinline__ float team_max(float x, int lg, float* lds) {
 
 __device__ __forceinline__ float rstd_of(float sum, float D, float eps) { return 1.0f / sqrt_rn(sum / D + eps); }
 
-// T = 64: waves, each of 64 >> lg rows; T = 256: a block of 256 threads a row (lg = 6).
+// T = 64: blocks of four waves, each of 64 >> lg rows; else a block of T threads a row (lg = 6).
 template <class E, class R, bool FP8, int T, int NV>
-__global__ __launch_bounds__(256) void k_norm(NormArgs a, int lg) {
+__global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
-  __shared__ float lds[4];
+  __shared__ float lds[T > 64 ? T / 64 : 1];
   const int lane = threadIdx.x & 63;
   const int team = T > 64 ? T : 1 << lg;
   const int l = T > 64 ? (int)threadIdx.x : lane & (team - 1);
@@ -202,29 +232,27 @@ __global__ __launch_bounds__(256) void k_norm(NormArgs a, int lg) {
       if (a.group) {       // a group is an aligned run of lanes
         const int gl = a.group / VE;
         const float m = lanes_max_nan(amax, gl);
-        const float s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
+        const Scale k = scale_of(m);
         if (live && e < a.D) {
-          if ((lane & (gl - 1)) == 0) a.scale[row * (a.D / a.group) + e / a.group] = s;
-#pragma unroll
-          for (int j = 0; j < VE; ++j) h[i].v[j] = h[i].v[j] / s;
+          if ((lane & (gl - 1)) == 0) a.scale[row * (a.D / a.group) + e / a.group] = k.s;
+          divide<E>(h[i], k);
           store_fp8<E>((uint8_t*)a.y + row * a.D + e, h[i], a.D - e);
         }
         amax = 0.0f;
       }
     } else {
-      store_raw<E, true>((E*)a.y + at * a.D + e, narrow<E>(h[i]), live ? a.D - e : 0);
+      store_raw<E, false>((E*)a.y + at * a.D + e, narrow<E>(h[i]), live ? a.D - e : 0);
     }
   }
   if constexpr (FP8) {
     if (a.group) return;
     amax = team_max<T>(amax, lg, lds);
-    const float s = amax > 0.0f || amax != amax ? amax / kFp8Max : 1.0f;
-    if (l == 0 && live) a.scale[row] = s;
+    const Scale k = scale_of(amax);
+    if (l == 0 && live) a.scale[row] = k.s;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = (i * team + l) * VE;
-#pragma unroll
-      for (int j = 0; j < VE; ++j) h[i].v[j] = h[i].v[j] / s;
+      divide<E>(h[i], k);
       store_fp8<E>((uint8_t*)a.y + at * a.D + e, h[i], live ? a.D - e : 0);
     }
   }
@@ -235,7 +263,7 @@ __global__ __launch_bounds__(256) void k_norm(NormArgs a, int lg) {
 template <class E, class R, bool FP8>
 __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
   constexpr int VE = Elem<E>::VE, T = 256;
-  __shared__ float lds[4];
+  __shared__ float lds[T > 64 ? T / 64 : 1];
   const int64_t row = blockIdx.x;
   const E* x = (const E*)a.x + row * a.x_ld;
   const R* r = (const R*)a.r + row * a.r_ld;
@@ -268,7 +296,7 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
     for (int j = 0; j < VE; ++j) h.v[j] = h.v[j] * c * w.v[j];
     return h;
   };
-  float s = 1.0f;
+  Scale k{1.0f, 1.0f, false};
   if constexpr (FP8) {
     if (!a.group) {
       float m = 0.0f;
@@ -279,8 +307,8 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
           if (e + j < a.D) m = max_nan(m, __builtin_fabsf(h.v[j]));
       }
       m = team_max<T>(m, 6, lds);
-      s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
-      if (threadIdx.x == 0) a.scale[row] = s;
+      k = scale_of(m);
+      if (threadIdx.x == 0) a.scale[row] = k.s;
     }
   }
   const int64_t end = (a.D + T * VE - 1) / (T * VE) * (T * VE);    // whole blocks: the groups' shuffles
@@ -294,14 +322,13 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
         for (int j = 0; j < VE; ++j) m = max_nan(m, __builtin_fabsf(h.v[j]));
         const int gl = a.group / VE;
         m = lanes_max_nan(m, gl);
-        s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
-        if (e < a.D && (threadIdx.x & (gl - 1)) == 0) a.scale[row * (a.D / a.group) + e / a.group] = s;
+        k = scale_of(m);
+        if (e < a.D && (threadIdx.x & (gl - 1)) == 0) a.scale[row * (a.D / a.group) + e / a.group] = k.s;
       }
-#pragma unroll
-      for (int j = 0; j < VE; ++j) h.v[j] = h.v[j] / s;
+      divide<E>(h, k);
       store_fp8<E>((uint8_t*)a.y + row * a.D + e, h, valid);
     } else {
-      store_raw<E, true>((E*)a.y + row * a.D + e, narrow<E>(h), valid);
+      store_raw<E, false>((E*)a.y + row * a.D + e, narrow<E>(h), valid);
     }
     if (a.r) {
       const Frag<E> f = load(e < a.D ? e : 0);
@@ -321,13 +348,13 @@ struct NormBackArgs {
   float* part;                    // [gridDim.x][D] weight gradient of each block's rows, or NULL
 };
 
-// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks rows team, team + teams, ...; its weight
-// gradient stays in registers until the end, then the block's teams are added in a fixed order.
-template <class E, class R, int T, int NV>
-__global__ __launch_bounds__(256) void k_norm_back(NormBackArgs a, int lg) {
+// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time (U rows' loads in flight), `teams`
+// apart; its weight gradient stays in registers until the end, then the block's teams are added in a fixed order.
+template <class E, class R, int T, int NV, int U>
+__global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
   extern __shared__ float dwsum[];     // [D], only with a.part
-  __shared__ float lds[4];
+  __shared__ float lds[T > 64 ? T / 64 : 1];
   const int lane = threadIdx.x & 63;
   const int team = T > 64 ? T : 1 << lg;
   const int l = T > 64 ? (int)threadIdx.x : lane & (team - 1);
@@ -344,58 +371,59 @@ __global__ __launch_bounds__(256) void k_norm_back(NormBackArgs a, int lg) {
 #pragma unroll
     for (int j = 0; j < VE; ++j) dw[i].v[j] = 0.0f;
   }
-  for (int64_t b = base; b < a.n; b += teams) {
-    const int64_t row = b + (first - base);
-    const bool live = row < a.n;
-    const int64_t at = live ? row : 0;
-    const E* dy = (const E*)a.dy + at * a.dy_ld;
-    const R* h = (const R*)a.h + at * a.h_ld;
-    const R* dh = (const R*)a.dh + at * a.dh_ld;
-    u32x4 rdy[NV];
-    ResRaw<E, R> rh[NV], rd[NV];
+  for (int64_t b = base; b < a.n; b += teams * U) {
+    u32x4 rdy[U][NV];
+    ResRaw<E, R> rh[U][NV], rd[U][NV];
+    float c[U];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * team + l) * VE;
-      const int valid = live ? a.D - e : 0;
-      rdy[i] = load_raw<E, true>(dy + e, valid, 0.0f);
-      rh[i] = res_load<E, R>(h + e, valid);
-    }
-    if (a.dh) {
+    for (int q = 0; q < U; ++q) {
+      const int64_t row = b + (first - base) + q * teams;
+      const bool live = row < a.n;
+      const int64_t at = live ? row : 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e = (i * team + l) * VE;
-        rd[i] = res_load<E, R>(dh + e, live ? a.D - e : 0);
+        const int valid = live ? a.D - e : 0;
+        rdy[q][i] = load_raw<E, true>((const E*)a.dy + at * a.dy_ld + e, valid, 0.0f);
+        rh[q][i] = res_load<E, R>((const R*)a.h + at * a.h_ld + e, valid);
+        if (a.dh) rd[q][i] = res_load<E, R>((const R*)a.dh + at * a.dh_ld + e, valid);
       }
+      c[q] = live ? a.rstd[at] : 0.0f;
     }
-    const float c = live ? a.rstd[at] : 0.0f;
-    float dot = 0.0f;
-    Frag<E> u[NV], xh[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      u[i] = widen<E>(rdy[i]);
-      xh[i] = res_widen<E, R>(rh[i]);
+    for (int q = 0; q < U; ++q) {
+      const int64_t row = b + (first - base) + q * teams;
+      const bool live = row < a.n;
+      float dot = 0.0f;
+      Frag<E> u[NV], xh[NV];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        xh[i].v[j] = xh[i].v[j] * c;
-        dw[i].v[j] = __builtin_fmaf(u[i].v[j], xh[i].v[j], dw[i].v[j]);
-        u[i].v[j] = u[i].v[j] * w[i].v[j];
-        dot = __builtin_fmaf(u[i].v[j], xh[i].v[j], dot);
+      for (int i = 0; i < NV; ++i) {
+        u[i] = widen<E>(rdy[q][i]);
+        xh[i] = res_widen<E, R>(rh[q][i]);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          xh[i].v[j] = xh[i].v[j] * c[q];
+          dw[i].v[j] = __builtin_fmaf(u[i].v[j], xh[i].v[j], dw[i].v[j]);
+          u[i].v[j] = u[i].v[j] * w[i].v[j];
+          dot = __builtin_fmaf(u[i].v[j], xh[i].v[j], dot);
+        }
       }
-    }
-    dot = team_sum<T>(dot, lg, lds) * inv_d;
+      dot = team_sum<T>(dot, lg, lds) * inv_d;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * team + l) * VE;
-      Frag<E> f;
-      if (a.dh) {
-        f = res_widen<E, R>(rd[i]);
-      } else {
+      for (int i = 0; i < NV; ++i) {
+        const int e = (i * team + l) * VE;
+        Frag<E> f;
+        if (a.dh) {
+          f = res_widen<E, R>(rd[q][i]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) f.v[j] = 0.0f;
+          for (int j = 0; j < VE; ++j) f.v[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          f.v[j] = __builtin_fmaf(c[q], __builtin_fmaf(-xh[i].v[j], dot, u[i].v[j]), f.v[j]);
+        res_store<E, R>((R*)a.dx + (live ? row : 0) * a.D + e, f, live ? a.D - e : 0);
       }
-#pragma unroll
-      for (int j = 0; j < VE; ++j) f.v[j] = __builtin_fmaf(c, __builtin_fmaf(-xh[i].v[j], dot, u[i].v[j]), f.v[j]);
-      res_store<E, R>((R*)a.dx + at * a.D + e, f, live ? a.D - e : 0);
     }
   }
   if (!a.part) return;
@@ -435,7 +463,7 @@ __global__ __launch_bounds__(256) void k_norm_back(NormBackArgs a, int lg) {
 template <class E, class R>
 __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
   constexpr int VE = Elem<E>::VE, T = 256;
-  __shared__ float lds[4];
+  __shared__ float lds[T > 64 ? T / 64 : 1];
   const float inv_d = 1.0f / (float)a.D;
   float* part = a.part ? a.part + (int64_t)blockIdx.x * a.D : nullptr;
   bool fresh = true;
@@ -495,35 +523,40 @@ __global__ __launch_bounds__(1024) void k_norm_dw(const float* part, int rows, i
 
 // ---- host side
 
-// The team of a row of `nvec` vectors: 2^lg lanes of NV vectors (block: 256 threads).  NV = 0: the long kernels.
+// The team of a row of `nvec` vectors: 2^lg lanes (T = 64), or a block of T threads, of NV vectors each.  As many threads as
+// vectors as far as a block goes (rows of 4,096 bf16: 512 threads of one vector 84 us, 256 of two 88, a wave of eight 93; of
+// 2,048: 25 us against 28 for a wave of four).  NV = 0: the long kernels.
 struct Team {
-  int lg, NV;
-  bool block;
+  int lg, T, NV;
 };
-static Team team_of(int64_t nvec, int64_t n, int max_nv) {
+static Team team_of(int64_t nvec, int most_nv) {
   int lg = 0;
   while (lg < 6 && ((int64_t)1 << lg) < nvec) ++lg;
-  if (nvec <= 64) return {lg, 1, false};
-  if (nvec <= 128) return {6, 2, false};
-  if (nvec <= 256) return {6, 4, false};
-  if (nvec <= 512) return {6, 2, true};
-  if (nvec <= 1024) return {6, 4, true};
-  if (nvec <= 2048 && max_nv >= 8) return {6, 8, true};
-  return {6, 0, true};
+  if (nvec <= 64) return {lg, 64, 1};
+  if (nvec <= 128) return {6, 64, 2};
+  if (nvec <= 256) return {6, 256, 1};
+  if (nvec <= 512) return {6, 512, 1};
+  if (nvec <= 1024) return {6, 1024, 1};
+  if (nvec <= 2048) return {6, 1024, 2};
+  if (nvec <= 4096 && most_nv >= 4) return {6, 1024, 4};
+  return {6, 0, 0};
 }
 
 template <class E, class R, bool FP8>
 static void launch_norm(const NormArgs& a, hipStream_t st) {
-  const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, a.n, 8);
+  const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, 4);
   const unsigned rows = (unsigned)a.n;
   const unsigned waves = (unsigned)(((a.n + (64 >> t.lg) - 1) / (64 >> t.lg) + 3) / 4);
-  if (t.NV == 0) k_norm_long<E, R, FP8><<<rows, 256, 0, st>>>(a);
-  else if (t.block && t.NV == 2) k_norm<E, R, FP8, 256, 2><<<rows, 256, 0, st>>>(a, 6);
-  else if (t.block && t.NV == 4) k_norm<E, R, FP8, 256, 4><<<rows, 256, 0, st>>>(a, 6);
-  else if (t.block) k_norm<E, R, FP8, 256, 8><<<rows, 256, 0, st>>>(a, 6);
-  else if (t.NV == 1) k_norm<E, R, FP8, 64, 1><<<waves, 256, 0, st>>>(a, t.lg);
-  else if (t.NV == 2) k_norm<E, R, FP8, 64, 2><<<waves, 256, 0, st>>>(a, 6);
-  else k_norm<E, R, FP8, 64, 4><<<waves, 256, 0, st>>>(a, 6);
+  switch (t.T * 8 + t.NV) {
+    case 64 * 8 + 1: k_norm<E, R, FP8, 64, 1><<<waves, 256, 0, st>>>(a, t.lg); break;
+    case 64 * 8 + 2: k_norm<E, R, FP8, 64, 2><<<waves, 256, 0, st>>>(a, 6); break;
+    case 256 * 8 + 1: k_norm<E, R, FP8, 256, 1><<<rows, 256, 0, st>>>(a, 6); break;
+    case 512 * 8 + 1: k_norm<E, R, FP8, 512, 1><<<rows, 512, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 1: k_norm<E, R, FP8, 1024, 1><<<rows, 1024, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 2: k_norm<E, R, FP8, 1024, 2><<<rows, 1024, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 4: k_norm<E, R, FP8, 1024, 4><<<rows, 1024, 0, st>>>(a, 6); break;
+    default: k_norm_long<E, R, FP8><<<rows, 256, 0, st>>>(a); break;
+  }
 }
 
 constexpr int64_t kNormRowsPerLaunch = 1 << 22;
@@ -546,25 +579,35 @@ static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {
   }
 }
 
-// Blocks of the backward: enough to fill the chip, few enough that the partial weight gradients stay a small part.
-constexpr int64_t kBackBlocks = 512;
+// Blocks of the backward: enough to fill the chip, few enough that the partial weight gradients (written and read once, D
+// fp32 a block) stay a small part of a row's traffic.
+constexpr int64_t kBackBlocks = 512, kBackBlocksMost = 1024;
 static int64_t back_blocks(int64_t n, int64_t D, int type) {
-  const Team t = team_of((D + 16 / elem_size(type) - 1) / (16 / elem_size(type)), n, 4);
-  const int64_t per = t.block ? 1 : 4 << (6 - t.lg);
+  const Team t = team_of((D + 16 / elem_size(type) - 1) / (16 / elem_size(type)), 2);
+  const int64_t per = t.T == 64 ? 4 << (6 - t.lg) : 1;
+  const int64_t most = n / 64 < kBackBlocks ? kBackBlocks : n / 64 < kBackBlocksMost ? n / 64 : kBackBlocksMost;
   const int64_t b = (n + per - 1) / per;
-  return b < kBackBlocks ? b : kBackBlocks;
+  return b < most ? b : most;
 }
 
 template <class E, class R>
 static void launch_norm_back(const NormBackArgs& a, unsigned blocks, hipStream_t st) {
-  const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, a.n, 4);
+  const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, 2);
   const size_t lds = a.part ? (size_t)a.D * 4 : 0;
-  if (t.NV == 0) k_norm_back_long<E, R><<<blocks, 256, 0, st>>>(a);
-  else if (t.block && t.NV == 2) k_norm_back<E, R, 256, 2><<<blocks, 256, 0, st>>>(a, 6);
-  else if (t.block) k_norm_back<E, R, 256, 4><<<blocks, 256, 0, st>>>(a, 6);
-  else if (t.NV == 1) k_norm_back<E, R, 64, 1><<<blocks, 256, lds, st>>>(a, t.lg);
-  else if (t.NV == 2) k_norm_back<E, R, 64, 2><<<blocks, 256, lds, st>>>(a, 6);
-  else k_norm_back<E, R, 64, 4><<<blocks, 256, lds, st>>>(a, 6);
+  switch (t.T * 8 + t.NV) {
+    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 2><<<blocks, 256, lds, st>>>(a, t.lg); break;
+    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2><<<blocks, 256, lds, st>>>(a, 6); break;
+    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2><<<blocks, 256, 0, st>>>(a, 6); break;
+    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1><<<blocks, 512, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1><<<blocks, 1024, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 2:
+      if constexpr (sizeof(E) == sizeof(R)) {
+        k_norm_back<E, R, 1024, 2, 1><<<blocks, 1024, 0, st>>>(a, 6);
+        break;
+      }
+      [[fallthrough]];   // (its registers would spill)
+    default: k_norm_back_long<E, R><<<blocks, 256, 0, st>>>(a); break;
+  }
 }
 
 static int check_norm(int64_t n, int64_t D, int type, int res_type, int w_type) {
