@@ -374,8 +374,8 @@ static int run_grads(const elr_grad* g, int64_t n, bool scale, int write, float 
     else k_grad_sum_strided<P><<<b, kGradThreads, 0, st>>>(*s, part + at);
     at += b;
   });
-  // One launch of few blocks adds the partials up by itself; otherwise that is a launch, and a block has one chunk.
-  const bool own = scale && plan.launches == 1 && plan.chunks <= kOwnBlocks;
+  // Where the partials are few, every scaling block adds them up by itself; otherwise that is a launch.
+  const bool own = scale && plan.launches > 0 && plan.chunks <= kOwnBlocks;
   if (!own) k_grad_norm<P><<<1, kGradThreads, 0, st>>>(part, (int)at, norm);
   if (!scale) return launch_status();
   const Clip k{part, own ? (int)at : 0, max_norm, eps, norm, write};

@@ -32,10 +32,10 @@ constexpr int kChunks = 16;     // chunk maxima a thread keeps
 // Candidate lists, and vectors or chunks that hold candidates: of a block, and of a wave by itself (whose LDS bounds how many
 // run at once: 10.5 KB a wave was 4 waves a SIMD).
 template <int T>
-constexpr int kAbove = T > 64 ? 448 : 128;
+constexpr int kAbove = T > 128 ? 448 : T > 64 ? 192 : 128;
 constexpr int kTies = 64;
 template <int T>
-constexpr int kHits = T > 64 ? 256 : 80;
+constexpr int kHits = T > 128 ? 256 : T > 64 ? 128 : 80;
 constexpr uint32_t kFloorOrd = 0x007FFFFFu;   // order_of(-inf)
 constexpr int kMaxSplits = 64;
 
@@ -102,15 +102,17 @@ __device__ __forceinline__ void write_row(const LpArgs& a, int64_t row, const Su
 template <class E>
 constexpr uint32_t kBits = sizeof(E) == 4 ? ~0u : Elem<E>::kType == ELR_BF16 ? 0xFFFF0000u : 0xFFFFE000u;
 
-// The k-th largest of the 64 lanes' orders, bit by bit (its low bits 0 where kBits has none).
-template <class E>
-__device__ __forceinline__ uint32_t wave_kth(uint32_t o, int k) {
+// The k-th largest of the 64 lanes' N orders each, bit by bit (its low bits 0 where kBits has none).
+template <class E, int N>
+__device__ __forceinline__ uint32_t wave_kth(const uint32_t (&o)[N], int k) {
   uint32_t t = 0;
 #pragma unroll
-  for (int b = 31; (kBits<E> >> b & 1u) != 0 && b >= 0; --b) {
+  for (int b = 31; b >= __builtin_ctz(kBits<E>); --b) {
     const uint32_t c = t | 1u << b;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(o >= c)) >= k) t = c;
-    if (b == 0) break;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o[j] >= c));
+    if (n >= k) t = c;
   }
   return t;
 }
@@ -231,7 +233,8 @@ __device__ __forceinline__ uint32_t lower_bound(TopShared<T>& sh, float m, float
       }
     }
     if (T == 64 || threadIdx.x < 64) {
-      thr = wave_kth<E>(order_of(m), k);
+      const uint32_t o[1] = {order_of(m)};
+      thr = wave_kth<E, 1>(o, k);
       if (T > 64 && lane == 0) sh.thr = thr;
     }
   }
@@ -359,18 +362,18 @@ __device__ __forceinline__ RowPart<E, T> part_of(const LpArgs& a, int64_t row, i
   return r;
 }
 
-// The part's results: the row's if it is not split.
-template <class E, int T, bool TOP, class Fill>
+// The part's results: the row's if it is not split.  bound(thr): the bound to use, given the one from the threads' maxima.
+template <class E, int T, bool TOP, class Bound, class Fill>
 __device__ __forceinline__ void part_done(const LpArgs& a, int64_t row, int64_t unit, const RowPart<E, T>& r,
                                           TopShared<TOP ? T : 64>& sh, const Sums& q, bool has, float x_tok,
-                                          float mine, const Fill& fill) {
+                                          float mine, const Bound& bound, const Fill& fill) {
   if (a.splits == 1) {
     if (threadIdx.x == 0) write_row(a, row, q, has, x_tok);
   } else if (threadIdx.x == 0) {
     *(f32x4*)(a.part + unit * 4) = (f32x4){q.m, q.s, q.t, x_tok};
   }
   if constexpr (TOP) {
-    const uint32_t thr = lower_bound<E, T>(sh, mine, q.m, a.k);
+    const uint32_t thr = bound(lower_bound<E, T>(sh, mine, q.m, a.k));
     const float thr_f = thr <= kFloorOrd ? -0x1.fffffep+127f : value_of(thr);   // -inf: what is above it
     fill(thr, thr_f);
     if (a.splits == 1) {
@@ -454,7 +457,21 @@ __global__ __launch_bounds__(T) void k_lp_one(LpArgs a) {
       q.t = q.t + waves[w].t;
     }
   }
-  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, [&](uint32_t thr, float thr_f) {
+  const auto bound = [&](uint32_t thr) {
+    if constexpr (T == 64 && NV == 1 && TOP) {
+      // fewer vectors than k: that bound is -inf, so the k-th largest itself
+      if (thr > kFloorOrd || (r.len + r.shift) > a.k * VE) return thr;
+      uint32_t o[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        const int64_t e = e0 + j;
+        o[j] = e >= 0 && e < r.len ? order_of(x[0].v[j]) : 0;
+      }
+      return wave_kth<E, VE>(o, min(a.k, r.len));
+    }
+    return thr;
+  };
+  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, bound, [&](uint32_t thr, float thr_f) {
     if constexpr (TOP) {
       // the vectors that reach the bound to LDS, then a vector per thread
 #pragma unroll
@@ -473,6 +490,52 @@ __global__ __launch_bounds__(T) void k_lp_one(LpArgs a) {
         push_vec<E, T>(sh, widen<E>(sh.vecs[i]), thr, thr_f, r.first + (int32_t)sh.hits[i] * VE - r.shift);
     }
   });
+}
+
+// Short rows without alternatives: 2^lg lanes a row, kVecs vectors a lane, several rows a wave, so that a row's share of the
+// reductions is small (200,000 rows of 100 bf16: 74 us with a wave a row, 19 here; 60,000 of 1,000: 42 and 26).
+template <class E>
+__global__ __launch_bounds__(256) void k_lp_small(LpArgs a, int lg) {
+  constexpr int VE = Elem<E>::VE;
+  const int lane = threadIdx.x & 63, team = 1 << lg, l = lane & (team - 1);
+  const int64_t row = (((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - lg)) + (lane >> lg);
+  const bool live = row < a.n;            // (lanes past the last row take part in the reductions)
+  const E* p = (const E*)a.x + (live ? row : 0) * a.ld;
+  u32x4 raw[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int e = (u * team + l) * VE;
+    raw[u] = load_raw<E, true>(p + e, live ? a.V - e : 0, -__builtin_inff());
+  }
+  bool has = false;
+  float x_tok = 0.0f;
+  if (live && l == 0) {
+    const int64_t tok = token_at(a, row);
+    has = tok >= 0 && tok < a.V;
+    if (has) x_tok = to_f32(p[tok]);
+  }
+  Frag<E> x[kVecs];
+  Sums q{-__builtin_inff(), 0.0f, 0.0f};
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    x[u] = widen<E>(raw[u]);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) q.m = __builtin_fmaxf(q.m, x[u].v[j]);
+  }
+  q.m = lanes_op(q.m, team, [](float b, float c) { return __builtin_fmaxf(b, c); });
+  const float ref = exp_ref(q.m);
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float d = clamp_low(x[u].v[j] - ref);
+      const float e = exp_nat(d);
+      q.s = q.s + e;
+      q.t = __builtin_fmaf(e, d, q.t);
+    }
+  q.s = lanes_sum(q.s, team);
+  q.t = lanes_sum(q.t, team);
+  if (live && l == 0) write_row(a, row, q, has, x_tok);
 }
 
 // A longer part, T * kVecs vectors at a time.
@@ -538,7 +601,8 @@ __global__ __launch_bounds__(T) void k_lp_rows(LpArgs a) {
   }
   const float mine = q.m;
   q = block_join<T>(q, waves);
-  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, [&](uint32_t thr, float thr_f) {
+  const auto bound = [](uint32_t thr) { return thr; };
+  part_done<E, T, TOP>(a, row, unit, r, sh, q, has, x_tok, mine, bound, [&](uint32_t thr, float thr_f) {
     if constexpr (TOP) {
       // the chunks that reach the bound ...
       if (mine >= thr_f)
@@ -706,6 +770,7 @@ static void launch_part(const LpArgs& a, int64_t most, unsigned blocks, hipStrea
   else if (most <= 128 * VE) k_lp_one<E, 64, 2, TOP><<<blocks, 64, 0, st>>>(a);
   else if (most <= 256 * VE && a.splits == 1) k_lp_one<E, 64, 4, TOP><<<blocks, 64, 0, st>>>(a);
   else if (most <= kThreads * VE) k_lp_one<E, kThreads, 1, TOP><<<blocks, kThreads, 0, st>>>(a);
+  else if (most <= kThreads * 2 * VE && a.splits == 1) k_lp_one<E, 128, 4, TOP><<<blocks, 128, 0, st>>>(a);
   else if (most <= kThreads * 2 * VE) k_lp_one<E, kThreads, 2, TOP><<<blocks, kThreads, 0, st>>>(a);
   else if (most <= kThreads * 4 * VE) k_lp_one<E, kThreads, 4, TOP><<<blocks, kThreads, 0, st>>>(a);
   else k_lp_rows<E, kThreads, TOP><<<blocks, kThreads, 0, st>>>(a);
@@ -723,6 +788,12 @@ static void launch_rows(LpArgs a, hipStream_t st) {
   const int64_t steps = (most + kThreads * kVecs * VE - 1) / (kThreads * kVecs * VE);
   a.per_chunk = (int)((steps + kChunks - 1) / kChunks);
   const unsigned blocks = (unsigned)(a.n * a.splits);
+  if (a.k == 0 && a.V <= 64 * kVecs * VE) {      // never split
+    int lg = 0;
+    while ((VE * kVecs << lg) < a.V) ++lg;
+    k_lp_small<E><<<(unsigned)((((a.n - 1) >> (6 - lg)) >> 2) + 1), 256, 0, st>>>(a, lg);
+    return;
+  }
   if (a.k) launch_part<E, true>(a, most, blocks, st);
   else launch_part<E, false>(a, most, blocks, st);
   if (a.splits > 1) k_lp_join<<<(unsigned)a.n, kJoinThreads, 0, st>>>(a);
