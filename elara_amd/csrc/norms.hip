@@ -131,9 +131,12 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, const Frag<E>& f, int64_t 
     int b = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
     q[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], b, true);
   }
-  if (valid >= VE && ((uintptr_t)p & (VE - 1)) == 0) {
-    if constexpr (VE == 8) __builtin_nontemporal_store((u32x2){q[0], q[1]}, (u32x2*)p);
-    else __builtin_nontemporal_store(q[0], (uint32_t*)p);
+  // (rows of an odd number of bytes: the store takes any address)
+  typedef uint32_t u32x2_b __attribute__((ext_vector_type(2), aligned(1)));
+  typedef uint32_t u32_b __attribute__((aligned(1)));
+  if (valid >= VE) {
+    if constexpr (VE == 8) __builtin_nontemporal_store((u32x2_b){q[0], q[1]}, (u32x2_b*)p);
+    else *(u32_b*)p = q[0];
   } else {
 #pragma unroll
     for (int j = 0; j < VE; ++j)
@@ -581,12 +584,16 @@ static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {
 
 // Blocks of the backward: enough to fill the chip, few enough that the partial weight gradients (written and read once, D
 // fp32 a block) stay a small part of the rows' traffic; a block of 1,024 threads fills a CU (4,000 rows of 8,192 bf16: 43 us
-// with 256 blocks, 49 with 512).  Two rows a block where they are few (822 of 1,000 fp16: 11.6 us, 12.9 with one).
+// with 256 blocks, 49 with 512), four of 256 do (12,094 rows of 1,536: 31 us with 1,024 blocks, 40 with 512).  Two rows a
+// block where they are few (822 of 1,000 fp16: 11.6 us, 12.9 with one).
 constexpr int64_t kBackBlocks = 512, kBackBlocksMost = 1024, kBackFew = 32;
 static int64_t back_blocks(int64_t n, int64_t D, int type) {
   const Team t = team_of((D + 16 / elem_size(type) - 1) / (16 / elem_size(type)), 2);
   const int64_t per = t.T == 64 ? 4 << (6 - t.lg) : 1;
-  const int64_t most = t.T == 1024 ? 256 : n / 64 < kBackBlocks ? kBackBlocks : n / 64 < kBackBlocksMost ? n / 64 : kBackBlocksMost;
+  int64_t most = kBackBlocks;
+  if (t.T == 1024) most = 256;
+  else if (t.T == 256) most = kBackBlocksMost;
+  else if (t.T == 64) most = n / 64 < most ? most : n / 64 < kBackBlocksMost ? n / 64 : kBackBlocksMost;
   int64_t b = (n + per - 1) / per;
   if (b > kBackFew) b = (b + 1) / 2;
   return b < most ? b : most;

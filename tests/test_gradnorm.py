@@ -193,6 +193,25 @@ def test_streams_graph_and_repeats(dev):
 
 
 @pytest.mark.gpu
+def test_with_and_without_host_module(dev, monkeypatch):
+    """The native argument checks and the Python ones make the same call."""
+    gn = _gn()
+    grads = [_randn(dev, i, 300, 7 + i).to(TYPES[i % 3]) for i in range(5)] + [torch.zeros(0, device=dev)]
+
+    def run():
+        g = [t.clone() for t in grads]
+        outs = tuple(torch.empty_like(t, dtype=torch.float32) for t in grads)
+        return [gn.grad_norm(g, INF), gn.clip_grad_norm(g, 1.0, out=outs), *outs, gn.clip_grad_norm(g, 0.5, 1.0), *g]
+    want = run()
+    calls = []
+    monkeypatch.setattr(_lib, '_host', _lib._NoHost)
+    monkeypatch.setattr(_lib, 'check', lambda rc, what, f=_lib.check: (calls.append(what), f(rc, what)))
+    got = run()
+    assert len(calls) == 3 and all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        gn.clip_grad_norm([grads[0], grads[0]], 1.0)
+
+@pytest.mark.gpu
 def test_refusals(dev):
     gn = _gn()
     g = torch.zeros(6, 8, device=dev)

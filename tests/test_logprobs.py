@@ -310,6 +310,28 @@ def test_streams_and_graph(dev):
 
 
 @pytest.mark.gpu
+def test_with_and_without_host_module(dev, monkeypatch):
+    """The native argument checks and the Python ones make the same call."""
+    lp = _lp()
+    x = _randn(dev, 1, 2, 5, 3001).to(torch.bfloat16)
+    tok = torch.randint(0, 3001, (2, 5), generator=torch.Generator().manual_seed(1)).to(dev)
+    one = torch.ones(2, 5, device=dev)
+
+    def run():
+        r = lp.token_logprobs(x, tok, k=3)
+        none = lp.token_logprobs(x, tok.to(torch.int32))
+        assert none.top_id is None and none.top_logprob is None
+        out = torch.empty_like(x)
+        assert lp.token_logprobs_backward(x, tok, r.lse, None, one, out=out) is out
+        return [*r, none.logprob, out, lp.token_logprobs_backward(x, tok, r.lse, r.entropy, one, one, one)]
+    want = run()
+    calls = []
+    monkeypatch.setattr(_lib, '_host', _lib._NoHost)
+    monkeypatch.setattr(_lib, 'check', lambda rc, what, f=_lib.check: (calls.append(what), f(rc, what)))
+    got = run()
+    assert len(calls) == 4 and all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(got, want))
+
+@pytest.mark.gpu
 def test_refusals(dev):
     lp = _lp()
     x = torch.zeros(4, 50, device=dev)

@@ -246,6 +246,26 @@ def test_streams_graph_and_repeats(dev):
 
 
 @pytest.mark.gpu
+def test_with_and_without_host_module(dev, monkeypatch):
+    """The native argument checks and the Python ones make the same call."""
+    nm = _nm()
+    x, r = _randn(dev, 1, 2, 5, 256).to(torch.bfloat16), _randn(dev, 2, 2, 5, 256)
+    w = torch.full((256,), 1.5, dtype=torch.bfloat16, device=dev)
+
+    def run():
+        a, b = nm.rms_norm(x, w, residual=r), nm.rms_norm(x, None)
+        assert b.h is x
+        q, p = nm.rms_norm_fp8(x, w, residual=r, group=64), nm.rms_norm_fp8(x, w)
+        return [*a, b.y, b.rstd, q.y.view(torch.uint8), *q[1:], p.y.view(torch.uint8), p.scale,
+                *nm.rms_norm_backward(x, a.h, w, a.rstd, dh=r), nm.rms_norm_backward(x, x, None, b.rstd, need_dweight=False)[0]]
+    want = run()
+    calls = []
+    monkeypatch.setattr(_lib, '_host', _lib._NoHost)
+    monkeypatch.setattr(_lib, 'check', lambda rc, what, f=_lib.check: (calls.append(what), f(rc, what)))
+    got = run()
+    assert len(calls) == 6 and all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(got, want))
+
+@pytest.mark.gpu
 def test_refusals(dev):
     nm = _nm()
     x = torch.zeros(4, 96, dtype=torch.bfloat16, device=dev)
