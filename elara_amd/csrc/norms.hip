@@ -13,10 +13,10 @@
 // a wave), a wave, or a block, NV vectors a lane; vector j * team + lane.  It is read once and written once.  Rows too long
 // for a block's registers (k_norm_long) are read again from the caches for the output.
 //
-// Loads are non-temporal (read once), stores are not: 16,384 rows of 4,096 bf16 with a residual (537 MB) take 80 us (6.7
-// TB/s), with non-temporal stores 83, with plain loads too 91.  The backward of the same rows: 85 us and 5 for the sum of the
-// weight gradients (6.0 TB/s); 425,984 rows of 128 fp32: 107 us and 5 (5.9 TB/s).  fp8 of 8,192 rows of 2,048 with groups of
-// 128 (118 MB): 25 us (4.7 TB/s, of which a launch is 3 us).
+// Loads are non-temporal (read once; plain ones 3 to 14 % slower on 537 MB).  16,384 rows of 4,096 bf16 with a residual (537
+// MB) take 84 us (6.4 TB/s); their backward 85 us and 5 for the sum of the weight gradients (6.0 TB/s); that of 425,984 rows
+// of 128 fp32 (656 MB) 109 and 5 (5.8 TB/s).  fp8 of 8,192 rows of 2,048 with groups of 128 (118 MB): 24 us (4.9 TB/s, of
+// which a launch is 3 us).
 #include "elr_elem.h"
 
 namespace elr {
@@ -32,6 +32,7 @@ struct NormArgs {
   float eps;
   void *y, *h;                 // y: input's type, or e4m3 bytes; h: residual's type, NULL without a residual
   float *rstd, *scale;
+  int nt;                      // 16-byte stores past the caches
 };
 
 // Weight elements [e, e + VE) as fp32 (1 without a weight).
@@ -54,6 +55,16 @@ __device__ __forceinline__ Frag<E> weight_at(const void* w, int w_f32, int64_t e
     f = widen<E>(load_raw<E, false>((const E*)w + e, valid, 0.0f));
   }
   return f;
+}
+
+// Outputs that the last-level cache (256 MB) could not keep anyway are stored past it; smaller ones stay for what reads them
+// next.  16,384 rows of 4,096 bf16 with a residual (268 MB out): 84 us against 89; their backward (134 MB out): 94 past the
+// cache, 90 into it; 425,984 rows of 128 fp32, backward (218 MB out): 114 and 121.
+constexpr int64_t kKeepBytes = (int64_t)192 << 20;
+template <class E>
+__device__ __forceinline__ void store_out(E* p, u32x4 x, int64_t valid, int nt) {
+  if (nt) store_raw<E, true>(p, x, valid);
+  else store_raw<E, false>(p, x, valid);
 }
 
 // VE fp32 or 16-bit residual elements at the same places as an input vector of type E.
@@ -82,13 +93,13 @@ __device__ __forceinline__ Frag<E> res_widen(const ResRaw<E, R>& a) {
   return f;
 }
 template <class E, class R>
-__device__ __forceinline__ void res_store(R* p, const Frag<E>& f, int64_t valid) {
+__device__ __forceinline__ void res_store(R* p, const Frag<E>& f, int64_t valid, int nt) {
 #pragma unroll
   for (int q = 0; q < ResRaw<E, R>::N; ++q) {
     Frag<R> b;
 #pragma unroll
     for (int j = 0; j < Elem<R>::VE; ++j) b.v[j] = f.v[q * Elem<R>::VE + j];
-    store_raw<R, false>(p + q * Elem<R>::VE, narrow<R>(b), valid - q * Elem<R>::VE);
+    store_out<R>(p + q * Elem<R>::VE, narrow<R>(b), valid - q * Elem<R>::VE, nt);
   }
 }
 
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
 #pragma unroll
       for (int j = 0; j < VE; ++j) h[i].v[j] = h[i].v[j] + q.v[j];
       const int e = (i * team + l) * VE;
-      res_store<E, R>((R*)a.h + at * a.D + e, h[i], live ? a.D - e : 0);
+      res_store<E, R>((R*)a.h + at * a.D + e, h[i], live ? a.D - e : 0, a.nt);
     }
 #pragma unroll
     for (int j = 0; j < VE; ++j) ss = __builtin_fmaf(h[i].v[j], h[i].v[j], ss);
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
         amax = 0.0f;
       }
     } else {
-      store_raw<E, false>((E*)a.y + at * a.D + e, narrow<E>(h[i]), live ? a.D - e : 0);
+      store_out<E>((E*)a.y + at * a.D + e, narrow<E>(h[i]), live ? a.D - e : 0, a.nt);
     }
   }
   if constexpr (FP8) {
@@ -331,11 +342,11 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
       divide<E>(h, k);
       store_fp8<E>((uint8_t*)a.y + row * a.D + e, h, valid);
     } else {
-      store_raw<E, false>((E*)a.y + row * a.D + e, narrow<E>(h), valid);
+      store_out<E>((E*)a.y + row * a.D + e, narrow<E>(h), valid, a.nt);
     }
     if (a.r) {
       const Frag<E> f = load(e < a.D ? e : 0);
-      res_store<E, R>((R*)a.h + row * a.D + e, f, valid);
+      res_store<E, R>((R*)a.h + row * a.D + e, f, valid, a.nt);
     }
   }
 }
@@ -349,11 +360,12 @@ struct NormBackArgs {
   int w_f32;
   void* dx;                       // h's type, contiguous
   float* part;                    // [gridDim.x][D] weight gradient of each block's rows, or NULL
+  int nt;
 };
 
-// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time (U rows' loads in flight), `teams`
-// apart; its weight gradient stays in registers until the end, then the block's teams are added in a fixed order.
-template <class E, class R, int T, int NV, int U>
+// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time, `teams` apart; AHEAD: with
+// the next ones' loads in flight (a wave's rows: 121 us, 130 without; a block's: 95, and 91 without).  Its weight gradient stays in registers until the end, then the block's teams are added in a fixed order.
+template <class E, class R, int T, int NV, int U, bool AHEAD>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
   extern __shared__ float dwsum[];     // [D], only with a.part
@@ -374,10 +386,12 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
 #pragma unroll
     for (int j = 0; j < VE; ++j) dw[i].v[j] = 0.0f;
   }
-  for (int64_t b = base; b < a.n; b += teams * U) {
-    u32x4 rdy[U][NV];
-    ResRaw<E, R> rh[U][NV], rd[U][NV];
+  struct Rows {
+    u32x4 dy[U][NV];
+    ResRaw<E, R> h[U][NV], dh[U][NV];
     float c[U];
+  };
+  const auto load = [&](Rows& x, int64_t b) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int64_t row = b + (first - base) + q * teams;
@@ -387,12 +401,14 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
       for (int i = 0; i < NV; ++i) {
         const int e = (i * team + l) * VE;
         const int valid = live ? a.D - e : 0;
-        rdy[q][i] = load_raw<E, true>((const E*)a.dy + at * a.dy_ld + e, valid, 0.0f);
-        rh[q][i] = res_load<E, R>((const R*)a.h + at * a.h_ld + e, valid);
-        if (a.dh) rd[q][i] = res_load<E, R>((const R*)a.dh + at * a.dh_ld + e, valid);
+        x.dy[q][i] = load_raw<E, true>((const E*)a.dy + at * a.dy_ld + e, valid, 0.0f);
+        x.h[q][i] = res_load<E, R>((const R*)a.h + at * a.h_ld + e, valid);
+        if (a.dh) x.dh[q][i] = res_load<E, R>((const R*)a.dh + at * a.dh_ld + e, valid);
       }
-      c[q] = live ? a.rstd[at] : 0.0f;
+      x.c[q] = live ? a.rstd[at] : 0.0f;
     }
+  };
+  const auto compute = [&](const Rows& x, int64_t b) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int64_t row = b + (first - base) + q * teams;
@@ -401,11 +417,11 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
       Frag<E> u[NV], xh[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        u[i] = widen<E>(rdy[q][i]);
-        xh[i] = res_widen<E, R>(rh[q][i]);
+        u[i] = widen<E>(x.dy[q][i]);
+        xh[i] = res_widen<E, R>(x.h[q][i]);
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          xh[i].v[j] = xh[i].v[j] * c[q];
+          xh[i].v[j] = xh[i].v[j] * x.c[q];
           dw[i].v[j] = __builtin_fmaf(u[i].v[j], xh[i].v[j], dw[i].v[j]);
           u[i].v[j] = u[i].v[j] * w[i].v[j];
           dot = __builtin_fmaf(u[i].v[j], xh[i].v[j], dot);
@@ -417,16 +433,36 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
         const int e = (i * team + l) * VE;
         Frag<E> f;
         if (a.dh) {
-          f = res_widen<E, R>(rd[q][i]);
+          f = res_widen<E, R>(x.dh[q][i]);
         } else {
 #pragma unroll
           for (int j = 0; j < VE; ++j) f.v[j] = 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < VE; ++j)
-          f.v[j] = __builtin_fmaf(c[q], __builtin_fmaf(-xh[i].v[j], dot, u[i].v[j]), f.v[j]);
-        res_store<E, R>((R*)a.dx + (live ? row : 0) * a.D + e, f, live ? a.D - e : 0);
+          f.v[j] = __builtin_fmaf(x.c[q], __builtin_fmaf(-xh[i].v[j], dot, u[i].v[j]), f.v[j]);
+        res_store<E, R>((R*)a.dx + (live ? row : 0) * a.D + e, f, live ? a.D - e : 0, a.nt);
       }
+    }
+  };
+  if constexpr (AHEAD) {
+    Rows x, y;
+    int64_t b = base;
+    if (b < a.n) load(x, b);
+    while (b < a.n) {
+      load(y, b + teams * U);
+      compute(x, b);
+      b += teams * U;
+      if (b >= a.n) break;
+      load(x, b + teams * U);
+      compute(y, b);
+      b += teams * U;
+    }
+  } else {
+    for (int64_t b = base; b < a.n; b += teams * U) {
+      Rows x;
+      load(x, b);
+      compute(x, b);
     }
   }
   if (!a.part) return;
@@ -500,7 +536,7 @@ __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
         f.v[j] = __builtin_fmaf(c, __builtin_fmaf(-(q.v[j] * c), dot, y.v[j] * w.v[j]), f.v[j]);
-      res_store<E, R>((R*)a.dx + row * a.D + e, f, a.D - e);
+      res_store<E, R>((R*)a.dx + row * a.D + e, f, a.D - e, a.nt);
     }
   }
 }
@@ -604,14 +640,14 @@ static void launch_norm_back(const NormBackArgs& a, unsigned blocks, hipStream_t
   const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, 2);
   const size_t lds = a.part ? (size_t)a.D * 4 : 0;
   switch (t.T * 8 + t.NV) {
-    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 2><<<blocks, 256, lds, st>>>(a, t.lg); break;
-    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2><<<blocks, 256, lds, st>>>(a, 6); break;
-    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2><<<blocks, 256, 0, st>>>(a, 6); break;
-    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1><<<blocks, 512, 0, st>>>(a, 6); break;
-    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1><<<blocks, 1024, 0, st>>>(a, 6); break;
+    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 1, true><<<blocks, 256, lds, st>>>(a, t.lg); break;
+    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2, false><<<blocks, 256, lds, st>>>(a, 6); break;
+    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2, false><<<blocks, 256, 0, st>>>(a, 6); break;
+    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1, false><<<blocks, 512, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1, false><<<blocks, 1024, 0, st>>>(a, 6); break;
     case 1024 * 8 + 2:
       if constexpr (sizeof(E) == sizeof(R)) {
-        k_norm_back<E, R, 1024, 2, 1><<<blocks, 1024, 0, st>>>(a, 6);
+        k_norm_back<E, R, 1024, 2, 1, false><<<blocks, 1024, 0, st>>>(a, 6);
         break;
       }
       [[fallthrough]];   // (its registers would spill)
@@ -643,7 +679,8 @@ extern "C" int elr_rms_norm(const void* x, int type, int64_t n, int64_t D, int64
       !elem_aligned(weight, w_type) || (!fp8 && !elem_aligned(y, type)))
     return ELR_EINVAL;
   const NormArgs a{x, residual, weight, x_ld, res_ld, n, (int32_t)D, (int32_t)group, w_type == ELR_F32, eps,
-                   y, h, rstd, scale};
+                   y, h, rstd, scale,
+                   n * D * ((fp8 ? 1 : elem_size(type)) + (residual ? elem_size(res_type) : 0)) > kKeepBytes};
   hipStream_t st = (hipStream_t)stream;
   const bool q = fp8 != 0, wide = residual && res_type == ELR_F32;
   switch (type) {
@@ -677,7 +714,7 @@ extern "C" int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_
   const int64_t blocks = back_blocks(n, D, type);
   if (dweight && n > 0 && (!scratch || scratch_bytes < blocks * D * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const NormBackArgs a{dy, h, dh, weight, dy_ld, h_ld, dh_ld, rstd, n, (int32_t)D, w_type == ELR_F32, dx,
-                       dweight ? (float*)scratch : nullptr};
+                       dweight ? (float*)scratch : nullptr, n * D * elem_size(h_type) > kKeepBytes};
   if (n > 0) {
     const bool wide = h_type == ELR_F32;
     switch (type) {
