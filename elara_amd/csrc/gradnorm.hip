@@ -390,7 +390,7 @@ static int run_grads(const elr_grad* g, int64_t n, bool scale, int write, float 
 static int grads_by_norm(const elr_grad* g, int64_t n, int p, bool scale, int write, float max_norm, float eps,
                          float* norm, void* scratch, int64_t bytes, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  if (!norm) return ELR_EINVAL;
+  if (!norm || !(max_norm >= 0.0f) || !(eps >= 0.0f)) return ELR_EINVAL;
   if (int rc = check_grads(g, n, scale)) return rc;
   switch (p) {
     case 0: return run_grads<0>(g, n, scale, write, max_norm, eps, norm, scratch, bytes, st);

@@ -43,9 +43,11 @@ def _describe(grads, out):
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise RuntimeError(f'out must hold {len(grads)} tensors, got {len(outs)}')
-    dev = grads[0].device
+    dev = getattr(grads[0], 'device', None)
     arr = (_lib.Grad * len(grads))()
     for i, (t, o) in enumerate(zip(grads, outs)):
+        if not (isinstance(t, torch.Tensor) and isinstance(o, torch.Tensor)):
+            raise RuntimeError(f'gradient {i} and its output must be tensors, got {type(t).__name__}, {type(o).__name__}')
         if not (t.is_cuda and t.device == dev and t.dtype in _lib.ETYPE and t.layout == torch.strided):
             raise RuntimeError(f'gradient {i} must be a cuda float32, float16 or bfloat16 tensor on {dev}, got {t.dtype} '
                                f'{t.device}')
@@ -114,6 +116,6 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None):
     straight into the float32 rows that gpu_adam reads).  In place a norm of at most max_norm costs no write.  A NaN makes
     the norm and every gradient NaN; an infinite norm scales by 0."""
     max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise RuntimeError(f'max_norm must be at least 0, got {max_norm}')
+    if not (max_norm >= 0.0 and eps >= 0.0):
+        raise RuntimeError(f'max_norm and eps must be at least 0, got {max_norm} and {eps}')
     return _run(grads, out, _kind(norm_type), (max_norm, float(eps)))

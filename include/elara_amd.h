@@ -801,7 +801,7 @@ typedef struct elr_grad {
 } elr_grad;
 
 /* grads: a host array, read during the call.  norm: device fp32 [1].  scratch: elr_grad_norm_scratch_bytes(grads, n)
- * bytes, 8-byte aligned (-1: bad argument).  Outputs must not overlap one another or other tensors' data. */
+ * bytes, 8-byte aligned (-1: bad argument); max_norm and eps at least 0.  Outputs must not overlap one another or other tensors' data. */
 int64_t elr_grad_norm_scratch_bytes(const elr_grad* grads, int64_t n);
 int elr_grad_norm(const elr_grad* grads, int64_t n, int p, float* norm, void* scratch, int64_t scratch_bytes,
                   void* stream);

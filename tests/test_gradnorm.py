@@ -218,6 +218,7 @@ def test_refusals(dev):
     for bad in (lambda: gn.grad_norm([]), lambda: gn.grad_norm([g.cpu()]), lambda: gn.grad_norm([g.double()]),
                 lambda: gn.grad_norm([g, g.cpu()]), lambda: gn.grad_norm([g], 3.0), lambda: gn.grad_norm([g], 'x'),
                 lambda: gn.clip_grad_norm([g], -1.0), lambda: gn.clip_grad_norm([g], float('nan')),
+                lambda: gn.clip_grad_norm([g], 1.0, eps=-1.0), lambda: gn.grad_norm([g, None]), lambda: gn.grad_norm([None]),
                 lambda: gn.clip_grad_norm([g, g], 1.0), lambda: gn.clip_grad_norm([g[:1].expand(6, 8)], 1.0),
                 lambda: gn.clip_grad_norm([g], 1.0, out=[]), lambda: gn.clip_grad_norm([g], 1.0, out=[g.half()]),
                 lambda: gn.clip_grad_norm([g], 1.0, out=[g[:5]]),
@@ -243,6 +244,8 @@ def test_cabi_refusals():
               arr(out=1026), arr(rows=1 << 40, cols=1 << 40), arr(type=2, out=p)):
         assert clip(a, sb=1 << 20) == -1
     assert clip(arr(), n=-1) == -1 and clip(None) == -1 and clip(arr(), norm=None, sb=1 << 20) == -1
+    for m, eps in ((-1.0, 0.0), (float('nan'), 0.0), (1.0, -1.0), (1.0, float('nan'))):
+        assert L.elr_clip_grad_norm(arr(), 1, 2, m, eps, ctypes.c_void_p(256), ctypes.c_void_p(256), 1 << 20, None) == -1
     assert clip(arr(out_type=2), sb=1 << 20) == -2 and clip(arr(), kind=3, sb=1 << 20) == -2
     assert clip(arr(), sb=7) == -3 and clip(arr(), s=None, sb=1 << 20) == -3
     assert clip(arr(), s=ctypes.c_void_p(260), sb=1 << 20) == -3
