@@ -155,12 +155,12 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, const Frag<E>& f, int64_t 
   }
 }
 
-// Sum (or NaN-keeping maximum) over a team: 2^lg lanes, or (T > 64) the whole block through LDS.
+// Sum (or NaN-keeping maximum) over a team: 2^lg lanes, or (T > 64) the whole block through LDS, T / 64 floats that no
+// thread may still be reading from an earlier call.
 template <int T>
 __device__ __forceinline__ float team_sum(float x, int lg, float* lds) {
   x = lanes_sum(x, 1 << lg);
   if constexpr (T > 64) {
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
     x = lds[0];
@@ -173,7 +173,6 @@ template <int T>
 __device__ __forceinline__ float team_max(float x, int lg, float* lds) {
   x = lanes_max_nan(x, 1 << lg);
   if constexpr (T > 64) {
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
     x = lds[0];
@@ -189,7 +188,7 @@ __device__ __forceinline__ float rstd_of(float sum, float D, float eps) { return
 template <class E, class R, bool FP8, int T, int NV>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
-  __shared__ float lds[T > 64 ? T / 64 : 1];
+  __shared__ float lds[2][T > 64 ? T / 64 : 1];
   const int lane = threadIdx.x & 63;
   const int team = T > 64 ? T : 1 << lg;
   const int l = T > 64 ? (int)threadIdx.x : lane & (team - 1);
@@ -214,6 +213,12 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
       res[i] = res_load<E, R>(r + e, live ? a.D - e : 0);
     }
   }
+  Frag<E> w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (i * team + l) * VE;
+    w[i] = weight_at<E>(a.w, a.w_f32, e, a.D - e);
+  }
   Frag<E> h[NV];
   float ss = 0.0f;
 #pragma unroll
@@ -229,17 +234,16 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
 #pragma unroll
     for (int j = 0; j < VE; ++j) ss = __builtin_fmaf(h[i].v[j], h[i].v[j], ss);
   }
-  ss = team_sum<T>(ss, lg, lds);
+  ss = team_sum<T>(ss, lg, lds[0]);
   const float c = rstd_of(ss, (float)a.D, a.eps);
   if (l == 0 && live) a.rstd[row] = c;
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = (i * team + l) * VE;
-    const Frag<E> w = weight_at<E>(a.w, a.w_f32, e, a.D - e);
 #pragma unroll
     for (int j = 0; j < VE; ++j) {
-      h[i].v[j] = h[i].v[j] * c * w.v[j];
+      h[i].v[j] = h[i].v[j] * c * w[i].v[j];
       if (FP8 && e + j < a.D) amax = max_nan(amax, __builtin_fabsf(h[i].v[j]));
     }
     if constexpr (FP8) {
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
   }
   if constexpr (FP8) {
     if (a.group) return;
-    amax = team_max<T>(amax, lg, lds);
+    amax = team_max<T>(amax, lg, lds[1]);
     const Scale k = scale_of(amax);
     if (l == 0 && live) a.scale[row] = k.s;
 #pragma unroll
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
 template <class E, class R, bool FP8>
 __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
   constexpr int VE = Elem<E>::VE, T = 256;
-  __shared__ float lds[T > 64 ? T / 64 : 1];
+  __shared__ float lds[2][T > 64 ? T / 64 : 1];
   const int64_t row = blockIdx.x;
   const E* x = (const E*)a.x + row * a.x_ld;
   const R* r = (const R*)a.r + row * a.r_ld;
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < VE; ++j) ss = __builtin_fmaf(h.v[j], h.v[j], ss);
   }
-  ss = team_sum<T>(ss, 6, lds);
+  ss = team_sum<T>(ss, 6, lds[0]);
   const float c = rstd_of(ss, (float)a.D, a.eps);
   if (threadIdx.x == 0) a.rstd[row] = c;
   auto norm = [&](int64_t e) {
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(256) void k_norm_long(NormArgs a) {
         for (int j = 0; j < VE; ++j)
           if (e + j < a.D) m = max_nan(m, __builtin_fabsf(h.v[j]));
       }
-      m = team_max<T>(m, 6, lds);
+      m = team_max<T>(m, 6, lds[1]);
       k = scale_of(m);
       if (threadIdx.x == 0) a.scale[row] = k.s;
     }
@@ -369,7 +373,7 @@ template <class E, class R, int T, int NV, int U, bool AHEAD>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
   extern __shared__ float dwsum[];     // [D], only with a.part
-  __shared__ float lds[T > 64 ? T / 64 : 1];
+  __shared__ float lds[2][T > 64 ? T / 64 : 1];
   const int lane = threadIdx.x & 63;
   const int team = T > 64 ? T : 1 << lg;
   const int l = T > 64 ? (int)threadIdx.x : lane & (team - 1);
@@ -408,6 +412,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
       x.c[q] = live ? a.rstd[at] : 0.0f;
     }
   };
+  int turn = 0;       // rows alternate between two places in LDS: one barrier a row
   const auto compute = [&](const Rows& x, int64_t b) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
@@ -427,7 +432,8 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
           dot = __builtin_fmaf(u[i].v[j], xh[i].v[j], dot);
         }
       }
-      dot = team_sum<T>(dot, lg, lds) * inv_d;
+      dot = team_sum<T>(dot, lg, lds[turn]) * inv_d;
+      turn ^= 1;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e = (i * team + l) * VE;
@@ -502,10 +508,11 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
 template <class E, class R>
 __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
   constexpr int VE = Elem<E>::VE, T = 256;
-  __shared__ float lds[T > 64 ? T / 64 : 1];
+  __shared__ float lds[2][T > 64 ? T / 64 : 1];
   const float inv_d = 1.0f / (float)a.D;
   float* part = a.part ? a.part + (int64_t)blockIdx.x * a.D : nullptr;
   bool fresh = true;
+  int turn = 0;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const E* dy = (const E*)a.dy + row * a.dy_ld;
     const R* h = (const R*)a.h + row * a.h_ld;
@@ -524,7 +531,8 @@ __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
       }
     }
     fresh = false;
-    dot = team_sum<T>(dot, 6, lds) * inv_d;
+    dot = team_sum<T>(dot, 6, lds[turn]) * inv_d;
+    turn ^= 1;
     for (int64_t e = threadIdx.x * VE; e < a.D; e += T * VE) {
       const Frag<E> y = widen<E>(load_raw<E, false>(dy + e, a.D - e, 0.0f));
       const Frag<E> q = res_widen<E, R>(res_load<E, R>(h + e, a.D - e));
