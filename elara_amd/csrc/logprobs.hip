@@ -15,13 +15,15 @@
 // anyway) the k-th largest is a lower bound of the row's k-th largest element; about 64 ln(64 / (64 - k)) elements of a
 // random row reach it.  A part that fits the block's registers is searched there.  A longer one keeps the maximum of each
 // thread's chunks in LDS, and only chunks whose maximum reaches the bound are read again, a vector per lane.  The elements
-// found are ranked.  Rows with more of them than the lists hold (many equal values, few unmasked ones) take the radix
-// selection below: four counting passes, then the ties in index order.
+// found are ranked.  Where the bound's own value is too frequent for its list (equal values, masked ones) its first places
+// are taken in index order; where too many elements lie above it (the large ones all with a few threads) four counting
+// passes over the row find the k-th largest itself.
 // Order: larger first, ties by the lower id; -0 equals +0; a NaN ranks as -inf.
 //
 // Measured (bf16 but where said): 4,096 rows of 32,768 47 us (5.7 TB/s), with k = 5 52; 1,024 of 131,072 46 (5.8 TB/s);
-// 1,024 of 100,003 fp32 63 (6.5 TB/s); one row of 131,072 in 64 splits 4.6, with k = 20 11.  An element costs ten
-// instructions and an exponential, about 42 cycles of a SIMD for 64 of them: three quarters of the time that memory takes.
+// 1,024 of 100,003 fp32 63 (6.5 TB/s); one row of 131,072 in 64 splits 4.4, with k = 20 10.  An element costs ten
+// instructions, one of them an exponential, about 42 cycles of a SIMD for 64 of them: 36 of the 47 us above.  (The exponent
+// as one fma, with another path for rows at a type's lowest value, gained nothing: 45.5 and 52.)
 // Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 345 us (6.2 TB/s), 301 of 50,021 fp32 22 us (5.5 TB/s).
 #include "elr_elem.h"
 
@@ -148,7 +150,7 @@ struct RowPart {
   int32_t shift;        // elements between the start of p's memory line and p: vectors are laid from there
 };
 
-// The elements of the part that satisfy `pred(order)`, counted over the whole block into *count, in no order.
+// f(order, id) for every element of the part, in no order.
 template <class E, int T, class F>
 __device__ __forceinline__ void each_elem(const RowPart<E, T>& r, const F& f) {
   constexpr int VE = Elem<E>::VE;
@@ -295,10 +297,9 @@ __device__ __forceinline__ void rank_cands(int nc, int k, const At& at, const Ou
   }
 }
 
-// The k likeliest of a part from the lists, in order, through out(rank, packed); thr: the bound they were filled by.  With a
-// bound of -inf they hold what lies above it only.  More hits or ties than the lists hold: the bound is one value, so the
-// elements above it are collected again, if need be above a bound that at most k of them reach, and its ties follow in
-// index order.
+// The k likeliest of a part from the lists, in order, through out(rank, packed); thr: the bound they were filled by (of -inf:
+// with what lies above it).  Too many hits: the elements above the bound are collected from the whole part.  Too many of
+// those: above the k-th largest itself, which fewer than k are.  The rest are ties of that one value, in index order.
 template <class E, int T, class Out>
 __device__ __forceinline__ void finish_top(int k, const RowPart<E, T>& r, TopShared<T>& sh, uint32_t thr, const Out& out) {
   __syncthreads();

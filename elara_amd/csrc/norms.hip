@@ -213,12 +213,6 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
       res[i] = res_load<E, R>(r + e, live ? a.D - e : 0);
     }
   }
-  Frag<E> w[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (i * team + l) * VE;
-    w[i] = weight_at<E>(a.w, a.w_f32, e, a.D - e);
-  }
   Frag<E> h[NV];
   float ss = 0.0f;
 #pragma unroll
@@ -241,9 +235,11 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm(NormArgs a, int lg) 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = (i * team + l) * VE;
+    // (loaded with the row the weight costs 2 % more: 86 us for 84)
+    const Frag<E> w = weight_at<E>(a.w, a.w_f32, e, a.D - e);
 #pragma unroll
     for (int j = 0; j < VE; ++j) {
-      h[i].v[j] = h[i].v[j] * c * w[i].v[j];
+      h[i].v[j] = h[i].v[j] * c * w.v[j];
       if (FP8 && e + j < a.D) amax = max_nan(amax, __builtin_fabsf(h[i].v[j]));
     }
     if constexpr (FP8) {
