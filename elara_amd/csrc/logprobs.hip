@@ -819,7 +819,7 @@ static void launch_back(const LpBackArgs& a0, hipStream_t st) {
   const bool one = most <= 64 * VE;
   const int64_t per = 64 * VE * (one ? 1 : kBackVecs);
   a.chunks = (int32_t)((most + per - 1) / per);
-  const int64_t rows = (int64_t)1 << 28;          // waves of a launch
+  const int64_t rows = (int64_t)1 << 25;          // waves of a launch (a grid has less than 2^32 threads)
   const int64_t step = rows / a.chunks < 1 ? 1 : rows / a.chunks;
   for (int64_t r = 0; r < a.n; r += step) {
     const int64_t m = a.n - r < step ? a.n - r : step;

@@ -602,7 +602,7 @@ static void launch_norm(const NormArgs& a, hipStream_t st) {
   }
 }
 
-constexpr int64_t kNormRowsPerLaunch = 1 << 22;
+constexpr int64_t kNormRowsPerLaunch = 1 << 21;   // (a grid has less than 2^32 threads)
 
 template <class E, class R>
 static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {

@@ -35,7 +35,7 @@ def _autograd(model, ids, targets, eps):
     ent = -(logp.exp() * logp).sum(-1)
     loss = -((own + model.beta * ent) * has).sum() / has.sum()
     loss.backward()
-    return loss, table.grad, [w.grad for pair in blocks for w in pair] + [head.grad] + [g.grad for g in gains]
+    return loss.detach(), table.grad, [w.grad for pair in blocks for w in pair] + [head.grad] + [g.grad for g in gains]
 
 
 @pytest.mark.gpu

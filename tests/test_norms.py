@@ -217,6 +217,20 @@ def test_offsets_beyond_32_bits(dev):
 
 
 @pytest.mark.gpu
+def test_more_rows_than_a_launch(dev):
+    nm = _nm()
+    n = (1 << 21) + 9
+    x = _randn(dev, 1, 1 << 12, 64).to(torch.bfloat16).repeat((1 << 9) + 1, 1)[:n]
+    r = torch.ones_like(x)
+    out, q = nm.rms_norm(x, None, residual=r), nm.rms_norm_fp8(x, None, residual=r, group=32)
+    for a in (0, (1 << 21) - 3, n - 7):
+        s = slice(a, a + 7)
+        want = nm.rms_norm(x[s].clone(), None, residual=r[s].clone())
+        wq = nm.rms_norm_fp8(x[s].clone(), None, residual=r[s].clone(), group=32)
+        assert all(torch.equal(p[s], w) for p, w in zip(out, want))
+        assert torch.equal(q.y[s].view(torch.uint8), wq.y.view(torch.uint8)) and torch.equal(q.scale[s], wq.scale)
+
+@pytest.mark.gpu
 def test_streams_graph_and_repeats(dev):
     """A side stream and every replay of a graph give the eager bits; so do repeated calls (the weight gradient's order)."""
     nm = _nm()
