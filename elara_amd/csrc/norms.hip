@@ -625,8 +625,9 @@ static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {
 // Blocks of the backward: enough to fill the chip, few enough that the partial weight gradients (written and read once, D
 // fp32 a block) stay a small part of the rows' traffic; a block of 1,024 threads fills a CU (4,000 rows of 8,192 bf16: 43 us
 // with 256 blocks, 49 with 512), four of 256 do (12,094 rows of 1,536: 31 us with 1,024 blocks, 40 with 512).  Two rows a
-// block where they are few (822 of 1,000 fp16: 11.6 us, 12.9 with one).
-constexpr int64_t kBackBlocks = 512, kBackBlocksMost = 1024, kBackFew = 32;
+// block where they are few (822 of 1,000 fp16: 11.6 us, 12.9 with one), and one block, which needs no addition of partial
+// sums, for what up to three would do (30 rows of 64 fp32: 4.4 us, 5.9 with two blocks).
+constexpr int64_t kBackBlocks = 512, kBackBlocksMost = 1024, kBackFew = 32, kBackOne = 3;
 static int64_t back_blocks(int64_t n, int64_t D, int type) {
   const Team t = team_of((D + 16 / elem_size(type) - 1) / (16 / elem_size(type)), 2);
   const int64_t per = t.T == 64 ? 4 << (6 - t.lg) : 1;
@@ -636,6 +637,7 @@ static int64_t back_blocks(int64_t n, int64_t D, int type) {
   else if (t.T == 64) most = n / 64 < most ? most : n / 64 < kBackBlocksMost ? n / 64 : kBackBlocksMost;
   int64_t b = (n + per - 1) / per;
   if (b > kBackFew) b = (b + 1) / 2;
+  if (b <= kBackOne) b = 1;
   return b < most ? b : most;
 }
 
@@ -718,7 +720,7 @@ extern "C" int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_
   const int64_t blocks = back_blocks(n, D, type);
   if (dweight && n > 0 && (!scratch || scratch_bytes < blocks * D * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const NormBackArgs a{dy, h, dh, weight, dy_ld, h_ld, dh_ld, rstd, n, (int32_t)D, w_type == ELR_F32, dx,
-                       dweight ? (float*)scratch : nullptr, n * D * elem_size(h_type) > kKeepBytes};
+                       !dweight ? nullptr : blocks == 1 ? dweight : (float*)scratch, n * D * elem_size(h_type) > kKeepBytes};
   if (n > 0) {
     const bool wide = h_type == ELR_F32;
     switch (type) {
@@ -733,7 +735,7 @@ extern "C" int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_
         break;
     }
   }
-  if (dweight)   // no rows: zeros
+  if (dweight && (n == 0 || blocks > 1))   // no rows: zeros
     k_norm_dw<<<(unsigned)((D + 31) / 32), 1024, 0, st>>>((const float*)scratch, n > 0 ? (int)blocks : 0, (int32_t)D,
                                                          dweight);
   return launch_status();
