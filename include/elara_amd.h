@@ -768,7 +768,7 @@ int elr_token_logprobs_backward(const void* logits, int type, int64_t n, int64_t
  * 128 or 256 columns that divides D (scale fp32 [n, D / group]).
  *   x of `type`, residual (or NULL) and h of res_type = type or ELR_F32, weight (or NULL: ones) of w_type = type or
  *   ELR_F32; rows of x and residual x_ld and res_ld elements apart; y, h, rstd [n] contiguous.  h is written only with a
- *   residual and must not overlap x or the residual.
+ *   residual.  y and h must not overlap x, the residual or one another (long rows are read a second time).
  * ------------------------------------------------------------------------------------------------------- */
 int elr_rms_norm(const void* x, int type, int64_t n, int64_t D, int64_t x_ld, const void* residual, int res_type,
                  int64_t res_ld, const void* weight, int w_type, float eps, void* y, int fp8, int64_t group,
@@ -801,7 +801,8 @@ typedef struct elr_grad {
 } elr_grad;
 
 /* grads: a host array, read during the call.  norm: device fp32 [1].  scratch: elr_grad_norm_scratch_bytes(grads, n)
- * bytes, 8-byte aligned (-1: bad argument); max_norm and eps at least 0.  Outputs must not overlap one another or other tensors' data. */
+ * bytes, 8-byte aligned (-1: bad argument); max_norm and eps at least 0.  Outputs must not overlap one another or other
+ * tensors' data. */
 int64_t elr_grad_norm_scratch_bytes(const elr_grad* grads, int64_t n);
 int elr_grad_norm(const elr_grad* grads, int64_t n, int p, float* norm, void* scratch, int64_t scratch_bytes,
                   void* stream);
