@@ -103,18 +103,21 @@ __device__ __forceinline__ void res_store(R* p, const Frag<E>& f, int64_t valid,
   }
 }
 
-// The scale of values up to m, and what divides by it: a product with the reciprocal, or a division where that overflows
-// (scales below 2^-128).  (A division for each value took 32 us where this takes 27,
-// for 8,192 rows of 2,048.)
+// The scale of values up to m, and what divides by it.  The quotient is the correctly rounded one: q = y RN(1 / s) is within
+// two ulps, its residual q s - y is exact in one fma, and a second fma takes it off (Markstein's theorem, for a correctly
+// rounded reciprocal).  A product with the reciprocal alone takes values at e4m3's ties to the wrong side.  8,192 rows of 2,048
+// take 24 us either way; a division for each value cost 5 us more.  A scale below 2^-80, whose residuals could underflow, and
+// one that is infinite or NaN, divides.
 struct Scale {
   float s, inv;
   bool exact;
 };
+constexpr float kLeastScale = 0x1.0p-80f;
 __device__ __forceinline__ Scale scale_of(float m) {
   Scale r;
   r.s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
   r.inv = 1.0f / r.s;
-  r.exact = !(r.inv < __builtin_inff());
+  r.exact = !(r.s >= kLeastScale && r.s < __builtin_inff());
   return r;
 }
 template <class E>
@@ -124,7 +127,10 @@ __device__ __forceinline__ void divide(Frag<E>& h, const Scale& k) {
     for (int j = 0; j < Elem<E>::VE; ++j) h.v[j] = h.v[j] / k.s;
   } else {
 #pragma unroll
-    for (int j = 0; j < Elem<E>::VE; ++j) h.v[j] = h.v[j] * k.inv;
+    for (int j = 0; j < Elem<E>::VE; ++j) {
+      const float q = h.v[j] * k.inv;
+      h.v[j] = __builtin_fmaf(-__builtin_fmaf(q, k.s, -h.v[j]), k.inv, q);   // (the signs keep -0)
+    }
   }
 }
 

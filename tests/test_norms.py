@@ -160,6 +160,38 @@ def test_special_values(dev):
         check(x[3:], None, None, fp8=0)
 
 
+def quotients(x, w, r, rstd, group):
+    """(e4m3 bytes, scales) of rstd's row sums by the definition, each fp32 operation rounded once (IEEE, on the CPU)."""
+    x, rstd = x.cpu().float(), rstd.cpu()
+    h = x + r.cpu().float() if r is not None else x
+    y = (h * rstd[:, None]) * (w.cpu().float() if w is not None else 1.0)
+    grp = y.view(y.shape[0], -1, group or y.shape[1])
+    amax = grp.abs().amax(-1, keepdim=True)
+    scale = amax / torch.full_like(amax, 448.0)
+    scale = torch.where(scale == 0, 1.0, scale)
+    return (grp / scale).clamp(-448.0, 448.0).view_as(y).to(torch.float8_e4m3fn), scale[..., 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D,group', [(64, 0), (64, 32), (1000, 0), (2048, 128), (4096, 0), (4096, 256), (20_480, 0), (20_480, 64)])
+def test_fp8_is_the_rounded_quotient(dev, D, group, dtype):
+    """Every byte is y / scale rounded, and every scale max|y| / 448, also where quotients lie on e4m3's ties: whole numbers
+    up to a largest of 448, of which rstd cancels.  A large and a tiny row, whose scales divide otherwise, are among them."""
+    n = 400
+    x = torch.randint(-447, 448, (n, D), generator=torch.Generator().manual_seed(D + group)).float()
+    x[:, ::group or D] = 448.0
+    x[0] *= 2.0 ** -120 if dtype != torch.float16 else 1.0
+    x[1] = -0.0
+    x = x.to(dtype).to(dev)
+    w = torch.where(torch.arange(D) % 3 == 0, -1.0, 1.0).to(dev)
+    for weight, eps in ((None, EPS), (w, 1.0)):
+        q = _nm().rms_norm_fp8(x, weight, eps, group=group)
+        y, scale = quotients(x, weight, None, q.rstd, group)
+        assert torch.equal(q.scale.cpu(), scale)
+        assert torch.equal(q.y.cpu().view(torch.uint8), y.view(torch.uint8))
+
+
 @pytest.mark.gpu
 def test_layouts(dev):
     """Row strides, broadcast and transposed rows, unaligned bases, leading dimensions, no rows; in place over dh."""
