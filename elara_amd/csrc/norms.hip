@@ -2,7 +2,7 @@
 // backward (HBM-bound).  No counterpart in the reference.
 //
 // A row of D elements:  h = x + r;  c = 1 / sqrt(sum h^2 / D + eps);  y = h c w.
-// fp8: over the row, or over each group of columns, scale = max|y| / 448 (1 where that is 0) and q = e4m3(y / scale), round
+// fp8: over the row, or over each group of columns, scale = max|y| / 448 (1 where that rounds to 0) and q = e4m3(y / scale), round
 // to nearest even; 448 is the largest finite e4m3 value.
 // Backward, of y's gradient dy and the gradient dh that arrives on the residual stream, with u = w dy and xh = h c:
 //   dx = c (u - xh sum(u xh) / D) + dh  (x's and r's alike);   dw = sum over the rows of dy xh.
@@ -115,7 +115,8 @@ struct Scale {
 constexpr float kLeastScale = 0x1.0p-80f;
 __device__ __forceinline__ Scale scale_of(float m) {
   Scale r;
-  r.s = m > 0.0f || m != m ? m / kFp8Max : 1.0f;
+  r.s = m / kFp8Max;
+  if (r.s == 0.0f) r.s = 1.0f;     // nothing but zeros, or values whose scale rounds to 0 (up to 3.1e-43)
   r.inv = 1.0f / r.s;
   r.exact = !(r.s >= kLeastScale && r.s < __builtin_inff());
   return r;

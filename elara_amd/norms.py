@@ -91,8 +91,8 @@ def rms_norm(x, weight, eps=1e-6, residual=None):
 
 
 def rms_norm_fp8(x, weight, eps=1e-6, residual=None, group=0):
-    """rms_norm with y in float8_e4m3fn: y / scale, rounded to nearest even, scale = max|y| / 448 (1 where that is 0) over
-    each row (group=0) or each group of 32, 64, 128 or 256 columns."""
+    """rms_norm with y in float8_e4m3fn: y / scale, rounded to nearest even, scale = max|y| / 448 (1 where that
+    rounds to 0) over each row (group=0) or each group of 32, 64, 128 or 256 columns."""
     group = int(group)
     if group and (group not in GROUPS or x.dim() < 1 or x.shape[-1] % group):
         raise RuntimeError(f'group must be 0 or one of {GROUPS} that divides D, got {group}')

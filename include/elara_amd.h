@@ -764,8 +764,8 @@ int elr_token_logprobs_backward(const void* logits, int type, int64_t n, int64_t
  * Root-mean-square norm with the residual's addition (no counterpart in the reference).  For each of n rows of D:
  *   h = x + residual (h = x without one);  rstd = 1 / sqrt(mean h^2 + eps);  y = h rstd weight,
  * sums in fp32, the norm of the unrounded h.  fp8 = 0: y has x's type.  fp8 = 1: y holds e4m3 bytes of y / scale, with
- * scale = max|y| / 448 (1 where that is 0) over each row (group = 0; scale fp32 [n]) or over each `group` of 32, 64,
- * 128 or 256 columns that divides D (scale fp32 [n, D / group]).
+ * scale = max|y| / 448 (1 where that rounds to 0) over each row (group = 0; scale fp32 [n]) or over each `group` of 32,
+ * 64, 128 or 256 columns that divides D (scale fp32 [n, D / group]).
  *   x of `type`, residual (or NULL) and h of res_type = type or ELR_F32, weight (or NULL: ones) of w_type = type or
  *   ELR_F32; rows of x and residual x_ld and res_ld elements apart; y, h, rstd [n] contiguous.  h is written only with a
  *   residual.  y and h must not overlap x, the residual or one another (long rows are read a second time).

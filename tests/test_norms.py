@@ -193,6 +193,31 @@ def test_fp8_is_the_rounded_quotient(dev, D, group, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('D,group', [(64, 32), (256, 64), (2048, 128), (20_480, 32), (64, 0), (500, 0), (4096, 0), (20_480, 0)])
+def test_fp8_of_values_below_any_scale(dev, D, group, dtype):
+    """Groups (or rows) of zeros and one value so small that max|y| / 448 rounds to 0: scale 1, no NaN; beside it the
+    values whose scale is a subnormal."""
+    x = torch.zeros(6, D)
+    if group:
+        x[:, group:] = torch.randn(6, D - group, generator=torch.Generator().manual_seed(D))
+    x[:, 3] = torch.tensor([1.0, -1.0, 0.0, 1.0, 1.0, 2.0])
+    x = x.to(dtype).to(dev)
+    w = torch.ones(D, device=dev)
+    w[3] = 2.0 ** -136
+    q = _nm().rms_norm_fp8(x, w, 1e4, group=group)              # rstd about 1/100: |y| 82 or 164 times 2^-149
+    y, scale = quotients(x, w, None, q.rstd, group)
+    assert bool((q.scale[:, 0] == 1).all()) and not q.y[:, :group or D].float().any()
+    w[3] = 2.0 ** -133
+    p = _nm().rms_norm_fp8(x, w, 1.0, group=group)
+    z, tiny = quotients(x, w, None, p.rstd, group)
+    assert bool((tiny[[0, 1, 3, 4, 5], 0] < 2.0 ** -130).all()) and tiny[2, 0] == 1 and bool((p.scale[:2, 0] > 0).all())
+    for a, b, s, t in ((q.y, y, q.scale, scale), (p.y, z, p.scale, tiny)):
+        assert torch.isfinite(a.float()).all() and torch.equal(s.cpu(), t)
+        assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
 def test_layouts(dev):
     """Row strides, broadcast and transposed rows, unaligned bases, leading dimensions, no rows; in place over dh."""
     nm = _nm()
