@@ -24,7 +24,7 @@
 // 1,024 of 100,003 fp32 63 (6.5 TB/s); one row of 131,072 in 64 splits 4.4, with k = 20 10.  An element costs ten
 // instructions, one of them an exponential, about 42 cycles of a SIMD for 64 of them: 36 of the 47 us above.  (The exponent
 // as one fma, with another path for rows at a type's lowest value, gained nothing: 45.5 and 52.)
-// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 345 us (6.2 TB/s), 301 of 50,021 fp32 22 us (5.5 TB/s).
+// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 338 us (6.3 TB/s), 301 of 50,021 fp32 21 us (5.6 TB/s).
 #include "elr_elem.h"
 
 namespace elr {
@@ -700,9 +700,83 @@ constexpr int kBackVecs = 4;
 // for log V and e^(x - lse) would be 1 for each of the V.  Such a row gets no gradient.
 constexpr float kEmptyLse = -0x1.0p+100f;
 
-// A wave's vectors of a row, from element e0 of lane 0 on; ALL: every one lies within the row.
+// From here on half an ulp of lse (2^-17 and more) is what p = e^(x - lse) would err by, and at a common offset of 10^9 lse has
+// no digit of log V left.  The maximum and the sum of such a wide row are taken again.
+constexpr float kWideLse = 256.0f;
+
+// What a row's gradient needs; logp = (x - ref) - sub.
+struct RowGrad {
+  int64_t tok;
+  float g, h, c0, ref, sub;
+  bool has, empty, wide;
+};
+__device__ __forceinline__ RowGrad row_grad(const LpBackArgs& a, int64_t row) {
+  RowGrad r;          // (no load waits for the token: 200,000 rows of 100 in 80 us, 84 where that of g did)
+  r.ref = a.lse[row];
+  const float g = a.d_logprob ? a.d_logprob[row] : 0.0f;
+  r.h = a.d_entropy ? a.d_entropy[row] : 0.0f;
+  const float z = a.d_lse ? a.d_lse[row] : 0.0f;
+  const float ent = a.d_entropy ? a.entropy[row] : 0.0f;
+  r.tok = a.idx64 ? ((const int64_t*)a.tokens)[row] : (int64_t)((const int32_t*)a.tokens)[row];
+  r.has = r.tok >= 0 && r.tok < a.V;
+  r.g = r.has ? g : 0.0f;
+  r.c0 = (z - r.g) - r.h * ent;
+  r.sub = 0.0f;
+  r.empty = r.ref < kEmptyLse;
+  const float size = __builtin_fabsf(r.ref);
+  r.wide = size >= kWideLse && size < __builtin_inff() && !r.empty;
+  return r;
+}
+// A wide row's gradient by its own maximum m and sum s: p = e^((x - m) - log s), in which nothing cancels.  An lse that is not
+// m + log s to its last bits (it may be of more logits than these) is used as it is.
+__device__ __forceinline__ void use_own(RowGrad& r, float m, float s) {
+  const float logs = __builtin_logf(s), rest = (m - r.ref) + logs;
+  if (__builtin_fabsf(rest) <= __builtin_fabsf(r.ref) * 0x1.0p-22f) {
+    r.ref = m;
+    r.sub = logs;
+  }
+}
+// The gradients of the vector at element e of the row.  SUB: r.sub may be other than 0.
+template <class E, bool SUB>
+__device__ __forceinline__ u32x4 grad_vec(const RowGrad& r, u32x4 raw, int64_t e) {
+  constexpr int VE = Elem<E>::VE;
+  Frag<E> y = widen<E>(raw);
+  const int at = r.has && r.tok >= e && r.tok < e + VE ? (int)(r.tok - e) : -1;
+#pragma unroll
+  for (int j = 0; j < VE; ++j) {
+    const float d0 = y.v[j] - r.ref;
+    const float logp = clamp_low(SUB ? d0 - r.sub : d0);
+    const float d = exp_nat(logp) * __builtin_fmaf(-r.h, logp, r.c0);
+    y.v[j] = r.empty ? 0.0f : j == at ? d + r.g : d;
+  }
+  return narrow<E>(y);
+}
+
+// A wave's running maximum and sum, each lane's its own, with U more vectors.
+template <class E, int U>
+__device__ __forceinline__ void add_vecs(Sums& q, const u32x4 (&raw)[U]) {
+  constexpr int VE = Elem<E>::VE;
+  Frag<E> y[U];
+  float m = q.m;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    y[u] = widen<E>(raw[u]);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) m = __builtin_fmaxf(m, y[u].v[j]);
+  }
+  const float ref = exp_ref(m);
+  q.s = q.s * exp_nat(clamp_low(q.m - ref));
+  q.m = m;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) q.s = q.s + exp_nat(clamp_low(y[u].v[j] - ref));
+}
+
+// A wave's vectors of a row, from element e0 of lane 0 on; ALL: every one lies within the row.  False: a wide row of more than
+// this chunk, of which nothing is written.
 template <class E, int U, bool ALL>
-__device__ __forceinline__ void back_vecs(const LpBackArgs& a, int64_t row, const E* x, E* out, int64_t s0) {
+__device__ __forceinline__ bool back_vecs(const LpBackArgs& a, int64_t row, const E* x, E* out, int64_t s0) {
   constexpr int VE = Elem<E>::VE;
   const int lane = threadIdx.x & 63;
   const int64_t e0 = s0 + lane * VE;
@@ -712,31 +786,60 @@ __device__ __forceinline__ void back_vecs(const LpBackArgs& a, int64_t row, cons
     if constexpr (ALL) raw[u] = load_raw<E, true>(x + e0 + u * 64 * VE, VE, 0.0f);
     else raw[u] = load_part<E, true>(x, e0 + u * 64 * VE, a.V, -__builtin_inff());
   }
-  const int64_t tok = a.idx64 ? ((const int64_t*)a.tokens)[row] : (int64_t)((const int32_t*)a.tokens)[row];
-  const bool has = tok >= 0 && tok < a.V;
-  const float g = has && a.d_logprob ? a.d_logprob[row] : 0.0f;
-  const float h = a.d_entropy ? a.d_entropy[row] : 0.0f;
-  const float z = a.d_lse ? a.d_lse[row] : 0.0f;
-  const float lse = a.lse[row];
-  const float c0 = (z - g) - (a.d_entropy ? h * a.entropy[row] : 0.0f);
-  const bool empty = lse < kEmptyLse;
+  RowGrad r = row_grad(a, row);
+  if (r.wide) {
+    if constexpr (U > 1) return false;
+    Sums q{-__builtin_inff(), 0.0f, 0.0f};      // (the row is this chunk)
+    add_vecs<E>(q, raw);
+    q = wave_join(q);
+    use_own(r, q.m, q.s);
+    store_part<E, true>(out, e0, a.V, grad_vec<E, true>(r, raw[0], e0));
+    return true;
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t e = e0 + u * 64 * VE;
-    Frag<E> y = widen<E>(raw[u]);
-    const int at = has && tok >= e && tok < e + VE ? (int)(tok - e) : -1;
+    const u32x4 y = grad_vec<E, false>(r, raw[u], e);
+    if constexpr (ALL) store_raw<E, true>(out + e, y, VE);
+    else store_part<E, true>(out, e, a.V, y);
+  }
+  return true;
+}
+
+// A whole wide row by one wave.  In place no other wave may write before the sum is taken, so the row's other waves leave it
+// alone.  4,096 rows of 131,072 bf16, all wide, take 1,133 us (338 where none is), one such row
+// alone 130.
+template <class E>
+__device__ __forceinline__ void back_wide(const LpBackArgs& a, int64_t row, const E* x, E* out) {
+  constexpr int VE = Elem<E>::VE, U = 16 / VE;      // (more vectors a step would cost the other rows' waves registers)
+  constexpr int64_t kStep = 64 * U * VE;
+  const int lane = threadIdx.x & 63;
+  const int64_t first = -(int64_t)line_shift<E>(out, 128);
+  const auto load = [&](u32x4 (&raw)[U], int64_t e0) {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float logp = clamp_low(y.v[j] - lse);
-      const float d = exp_nat(logp) * __builtin_fmaf(-h, logp, c0);
-      y.v[j] = empty ? 0.0f : j == at ? d + g : d;
+    for (int u = 0; u < U; ++u) raw[u] = load_part<E, false>(x, e0 + u * 64 * VE, a.V, -__builtin_inff());
+  };
+  Sums q{-__builtin_inff(), 0.0f, 0.0f};
+  for (int64_t s0 = first; s0 < a.V; s0 += kStep) {
+    u32x4 raw[U];
+    load(raw, s0 + lane * VE);
+    add_vecs<E>(q, raw);
+  }
+  q = wave_join(q);
+  RowGrad r = row_grad(a, row);
+  use_own(r, q.m, q.s);
+  for (int64_t s0 = first; s0 < a.V; s0 += kStep) {
+    u32x4 raw[U];
+    load(raw, s0 + lane * VE);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t e = s0 + lane * VE + u * 64 * VE;
+      store_part<E, true>(out, e, a.V, grad_vec<E, true>(r, raw[u], e));
     }
-    if constexpr (ALL) store_raw<E, true>(out + e, narrow<E>(y), VE);
-    else store_part<E, true>(out, e, a.V, narrow<E>(y));
   }
 }
 
-// Chunks of 64 * U vectors, one wave each, laid from the memory line in which the output's row starts.
+// Chunks of 64 * U vectors, one wave each, laid from the memory line in which the output's row starts.  U = 1: a row is one.
 template <class E, int U>
 __global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
   constexpr int VE = Elem<E>::VE;
@@ -747,9 +850,13 @@ __global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
   if (row >= a.n) return;
   const E* x = (const E*)a.x + row * a.ld;
   E* out = (E*)a.out + row * a.out_ld;
-  const int64_t s0 = (int64_t)(wave - in * (uint32_t)a.chunks) * kChunk - line_shift<E>(out, 128);
-  if (s0 >= 0 && s0 + kChunk <= a.V) back_vecs<E, U, true>(a, row, x, out, s0);
-  else back_vecs<E, U, false>(a, row, x, out, s0);
+  const uint32_t chunk = wave - in * (uint32_t)a.chunks;
+  const int64_t s0 = (int64_t)chunk * kChunk - line_shift<E>(out, 128);
+  const bool done = s0 >= 0 && s0 + kChunk <= a.V ? back_vecs<E, U, true>(a, row, x, out, s0)
+                                                  : back_vecs<E, U, false>(a, row, x, out, s0);
+  if constexpr (U > 1) {          // (blocks of four waves: another of the chip's parts for each wide row)
+    if (!done && chunk == in * 4u % (uint32_t)a.chunks) back_wide<E>(a, row, x, out);
+  }
 }
 
 // ---- host side

@@ -97,8 +97,8 @@ def token_logprobs_backward(logits, tokens, lse, entropy, d_logprob, d_entropy=N
     """The gradient to the logits of sum(d_logprob * logprob + d_entropy * entropy + d_lse * lse), in the logits' type and
     shape.  lse and entropy are token_logprobs' (entropy may be None without d_entropy); d_* are float32 of tokens' shape,
     None for zero.  Rows without a token get nothing from d_logprob; rows of nothing but -inf, or nothing but
-    float32's or bfloat16's lowest value, get 0.  out: where to write
-    it, a tensor of the logits' shape and type whose rows lie apart by a fixed stride; the logits themselves are allowed,
+    float32's or bfloat16's lowest value, get 0.  Where |lse| is 256 or more (a large offset common to the row) lse's last
+    digits no longer tell p, and the row's sum is taken again (a slower pass over it).  out: where to write it, a tensor of the logits' shape and type whose rows lie apart by a fixed stride; the logits themselves are allowed,
     and are then overwritten."""
     r = (_lib._host or _lib.host()).logprobs_back(logits, tokens, lse, entropy, d_logprob, d_entropy, d_lse, out)
     if r != _lib.NOT_TAKEN:

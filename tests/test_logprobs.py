@@ -177,6 +177,73 @@ def test_masked_rows(dev, V, dtype):
     assert not d[1].any() and torch.isfinite(d).all()
 
 
+def check_offset_backward(x, tok, g, h, z, out=None):
+    """check_backward with lse's own rounding taken no further than |lse| = 256: a row's common offset costs nothing."""
+    n, V = x.shape
+    f = _lp().token_logprobs(x, tok)
+    xs, ts = x.double().cpu().numpy(), tok.cpu().numpy().astype(np.int64)
+    gs, hs, zs = (t.double().cpu().numpy() for t in (g, h, z))
+    ref, p, logp, lse, ent = ref_backward(xs, ts, gs, hs, zs)
+    d = _lp().token_logprobs_backward(x, tok, f.lse, f.entropy, g, h, z, out=out)
+    a = d.double().cpu().numpy()
+    lp0, l0 = np.where(p == 0, 0.0, np.abs(logp)), np.minimum(np.abs(lse), 256.0)[:, None]
+    e = (V / 64 + 2 * math.log(V) + 64) * U
+    mag = p * (np.abs(gs) + np.abs(zs) + np.abs(hs) * ent)[:, None] + p * np.abs(hs)[:, None] * lp0
+    bound = mag * (e + (2 * lp0 + 2 * l0 + 16) * U) + p * np.abs(hs)[:, None] * e * (3 + ent[:, None])
+    bound = bound + HALF_ULP[x.dtype] * (np.abs(ref) + bound) + 4 * U * np.abs(ref) + TINY[x.dtype] + 1e-37
+    assert np.all(np.abs(a - ref) <= bound), (np.abs(a - ref) - bound).max(1)
+    return d
+
+
+OFFSETS = {torch.float32: (-1e30, -1e9, -65_504.0, -255.0, 300.0, 1e6, 1e20), torch.bfloat16: (-1e30, -1e9, -3e4, 255.0, 300.0, 1e6),
+           torch.float16: (-65_504.0, -65_000.0, -300.0, 260.0, 2e4, 65_504.0)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('V', [1, 2, 63, 300, 513, 1025, 4000, 9001, 40_003])
+def test_backward_of_rows_with_an_offset(dev, V, dtype):
+    """Rows of a large common offset, of which lse keeps few digits of log V or none: rows that a mask of -1e9 or the like left
+    nothing of (alike in every place), and spread ones; with and without a token, in place, unaligned and over row strides."""
+    low, rows = torch.finfo(dtype).min, []
+    for i, c in enumerate(OFFSETS[dtype]):
+        flat = torch.full((V,), c)
+        near = (c + torch.randn(V, generator=torch.Generator().manual_seed(V + i)) * 2.5).clamp(low, -low)
+        some = torch.where(torch.arange(V) % 3 == 0, near, torch.tensor(low))      # two of three masked
+        rows += [flat, flat, near, near, some]
+    x = torch.stack(rows).to(dtype).to(dev)
+    n = x.shape[0]
+    tok = (torch.arange(n) * 7 % V).to(dev)
+    tok[::5] = -1                                                                  # one of each flat pair is ignored
+    g, h, z = (_randn(dev, j, n, scale=1.0) for j in range(3))
+    want = check_offset_backward(x, tok, g, h, z)
+    y = x.clone()
+    assert torch.equal(check_offset_backward(y, tok, g, h, z, out=y), want)
+    buf = torch.zeros(n, V + 13, dtype=dtype, device=dev)
+    buf[:, 5:5 + V] = x
+    want = check_offset_backward(buf[:, 5:5 + V], tok, g, h, z, out=torch.empty_like(buf)[:, 5:5 + V])
+    got = check_offset_backward(buf[:, 5:5 + V], tok, g, h, z, out=buf[:, 5:5 + V])      # (the order of sums goes by alignment)
+    assert torch.equal(got, want) and not buf[:, :5].any() and not buf[:, 5 + V:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('offset', [0.0, 1000.0])
+def test_backward_with_the_lse_of_more_logits(dev, offset):
+    """An lse over a wider row than these logits (here twice as many) is used as it is; it errs by its rounding, at most
+    1013 * 2^-24 of p, beside the forward's and the exponential's bounds."""
+    lp = _lp()
+    V = 5000
+    x = _randn(dev, 1, 6, 2 * V) + offset
+    tok = torch.full((6,), -1, device=dev)
+    f = lp.token_logprobs(x, tok)
+    z = torch.ones(6, device=dev)
+    d = torch.cat([lp.token_logprobs_backward(x[:, :V], tok, f.lse, None, None, d_lse=z),
+                   lp.token_logprobs_backward(x[:, V:], tok, f.lse, None, None, d_lse=z)], 1).double()
+    ref = torch.softmax(x.double(), -1)
+    e = (2 * V / 64 + 2 * math.log(2 * V) + 64) * U
+    assert bool(((d - ref).abs() <= ref * (e + (2 * 30 + 2 * 1013 + 16) * U) + 1e-37).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('V', [100, 3000, 50_000])
