@@ -6,11 +6,13 @@ to the HIP runtime torch already loaded (same soname), and torch's streams are v
 """
 import contextlib
 import ctypes
+import math
 import os
 import threading
 import warnings
 from pathlib import Path
 
+import numpy as np
 import torch
 
 # ELARA_AMD_LIB may name another build of the same library (e.g. a tuning variant); default: the in-tree build.
@@ -351,6 +353,68 @@ def split_empty(dev, dtype, sizes):
     """Uninitialised 1-D tensors of the given sizes, views of one allocation: one allocator call and one split for a
     launch's outputs of one dtype (fewer Python-level tensor constructions than an allocation each)."""
     return torch.empty(sum(sizes), dtype=dtype, device=dev).split(list(sizes))
+
+
+def _spans(t):
+    """t's memory as spans of `width` bytes at its address plus every sum of multiples below `count` of the (count, stride in
+    bytes) of `steps`, largest stride first; neighbouring dimensions merged."""
+    dims = sorted(((st * t.element_size(), n) for n, st in zip(t.shape, t.stride()) if n > 1), reverse=True)
+    if dims and dims[-1][0] == 0:
+        dims = [d for d in dims if d[0]]
+    steps, width = [], t.element_size()
+    while dims and dims[-1][0] == width:
+        width *= dims.pop()[1]
+    for st, n in dims:
+        if steps and steps[-1][1] == st * n:
+            steps[-1] = (steps[-1][0] * n, st)
+        else:
+            steps.append((n, st))
+    return t.data_ptr(), width, steps
+
+
+def _starts(address, steps):
+    a = np.array([address], dtype=np.int64)
+    for n, st in steps:
+        a = (a[:, None] + st * np.arange(n, dtype=np.int64)).ravel()
+    a.sort()
+    return a
+
+
+def _end(address, width, steps):
+    return address + width + sum((n - 1) * st for n, st in steps)
+
+
+def overlaps_itself(t):
+    """Whether two elements of t share memory."""
+    if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())) and t.numel():
+        return True
+    if t.numel() < 2 or t.is_contiguous():
+        return False
+    a, width, steps = _spans(t)
+    extent = width
+    for n, st in reversed(steps):      # each stride beyond all that lies within: no overlap
+        if st < extent:
+            return bool((np.diff(_starts(a, steps)) < width).any())
+        extent += (n - 1) * st
+    return False
+
+
+def overlap(t, u):
+    """Whether t and u share memory.  Views whose ranges meet (columns of one matrix, say) are told apart by their addresses
+    modulo the common divisor of their strides; what that leaves open by listing their runs."""
+    if not t.numel() or not u.numel():
+        return False
+    a, wa, sa = _spans(t)
+    b, wb, sb = _spans(u)
+    if _end(a, wa, sa) <= b or _end(b, wb, sb) <= a:
+        return False
+    g = math.gcd(*(st for _, st in sa + sb))
+    d = (b - a) % g if g else 0
+    if g and d >= wa and d + wb <= g:
+        return False
+    x, y = _starts(a, sa), _starts(b, sb)
+    i = np.searchsorted(x, y + wb) - 1     # the last run of t that begins before the end of each of u's
+    return bool(((i >= 0) & (x[i] + wa > y)).any())
 
 
 ESIZE = {torch.int8: 1, torch.bool: 1, torch.uint8: 1, torch.int32: 4, torch.int64: 8, torch.float32: 4}

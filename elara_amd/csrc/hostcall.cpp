@@ -437,6 +437,28 @@ PyObject* norm_back(PyObject*, PyObject* const* a, Py_ssize_t na) {
   }
 }
 
+// A tensor's bytes.
+struct Range {
+  uintptr_t begin, end;
+  bool out;
+};
+Range range_of(const at::Tensor& t, bool out) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + static_cast<uintptr_t>(t.numel() * t.element_size()), out};
+}
+// Whether an output meets another range (inputs may meet one another).
+bool meet(std::vector<Range>& r) {
+  const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+  uintptr_t out_end = 0, end = 0;
+  for (const Range& x : r) {
+    if (x.begin < (x.out ? end : out_end)) return true;
+    end = std::max(end, x.end);
+    if (x.out) out_end = std::max(out_end, x.end);
+  }
+  return false;
+}
+
 // clip(grads, out or None, kind, max_norm or None, eps) -> (return code, norm), or NOT_TAKEN; max_norm None: the norm alone
 PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (na != 5 || !f_clip) return not_taken();
@@ -452,8 +474,8 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (n == 0 || (outs && PySequence_Fast_GET_SIZE(a[1]) != n)) return not_taken();
   try {
     std::vector<elr_grad> list(static_cast<size_t>(n));
-    std::vector<const void*> written;
-    written.reserve(static_cast<size_t>(n));
+    std::vector<Range> ranges;      // of what a call that scales reads and writes; in place: once
+    if (scale) ranges.reserve(static_cast<size_t>(outs ? 2 * n : n));
     const at::Tensor* first = nullptr;
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* to = PySequence_Fast_GET_ITEM(a[0], i);
@@ -467,10 +489,11 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
         return not_taken();
       const int64_t m = t->numel();
       list[static_cast<size_t>(i)] = elr_grad{t->data_ptr(), o->data_ptr(), 1, m, m, 1, m, 1, type, ot};
-      if (m) written.push_back(o->data_ptr());
+      if (!scale || m == 0) continue;
+      ranges.push_back(range_of(*o, true));
+      if (o->data_ptr() != t->data_ptr() || ot != type) ranges.push_back(range_of(*t, false));
     }
-    std::sort(written.begin(), written.end());
-    if (scale && std::adjacent_find(written.begin(), written.end()) != written.end()) return not_taken();
+    if (meet(ranges)) return not_taken();
     at::Tensor norm;
     int rc = kNotTaken;
     {

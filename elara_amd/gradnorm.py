@@ -77,12 +77,7 @@ def _run(grads, out, kind, clip):
         return r[1]
     grads, outs, dev, arr = _describe(grads, out)
     if clip:
-        seen = set()
-        for i, o in enumerate(outs):
-            if o.numel() and (o.data_ptr() in seen or _self_overlap(o)):
-                raise RuntimeError(f'output {i} overlaps itself or another: each element is scaled once')
-            if o.numel():
-                seen.add(o.data_ptr())
+        _check_outputs(grads, outs)
     L = _lib.lib()
     n = len(arr)
     nbytes = L.elr_grad_norm_scratch_bytes(arr, n)
@@ -98,9 +93,34 @@ def _run(grads, out, kind, clip):
     return norm
 
 
-def _self_overlap(t):
-    """Whether some dimension of more than one element has stride 0 (an expanded tensor)."""
-    return any(s == 0 and d > 1 for s, d in zip(t.stride(), t.shape))
+def _same_places(t, o):
+    """Whether o is t's memory, element by element."""
+    return t.data_ptr() == o.data_ptr() and t.dtype == o.dtype and all(
+        a == b for n, a, b in zip(t.shape, t.stride(), o.stride()) if n > 1)
+
+
+def _check_outputs(grads, outs):
+    """Each element is read and scaled once: an output may be its own gradient, and shares no memory with anything else."""
+    spans = []                                     # (first byte, end, is an output, number, tensor)
+    for i, (t, o) in enumerate(zip(grads, outs)):
+        if not t.numel():
+            continue
+        if _lib.overlaps_itself(o):
+            raise RuntimeError(f'output {i} overlaps itself or another: each element is scaled once')
+        for x, out in ((o, True),) if o is t or _same_places(t, o) else ((o, True), (t, False)):
+            end = x.data_ptr() + x.element_size() * (1 + sum((n - 1) * st for n, st in zip(x.shape, x.stride())))
+            spans.append((x.data_ptr(), end, out, i, x))
+    spans.sort(key=lambda s: s[:2])
+    open_ = []                                     # those that reach to where the next begins
+    for s in spans:
+        open_ = [q for q in open_ if q[1] > s[0]]
+        for q in open_:
+            if (q[2] or s[2]) and _lib.overlap(q[4], s[4]):
+                if q[2] and s[2]:
+                    raise RuntimeError(f'output {q[3]} overlaps itself or another: each element is scaled once')
+                o, t = (q, s) if q[2] else (s, q)
+                raise RuntimeError(f'output {o[3]} overlaps gradient {t[3]}, in another place or order than its own')
+        open_.append(s)
 
 
 def grad_norm(grads, norm_type=2.0):
@@ -113,8 +133,9 @@ def grad_norm(grads, norm_type=2.0):
 def clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None):
     """Scales grads so that their global norm is at most max_norm, and returns the norm before that (grad_norm's).
     In place, or into out: a list of tensors of grads' shapes, each of its gradient's type or float32 (16-bit gradients
-    straight into the float32 rows that gpu_adam reads).  In place a norm of at most max_norm costs no write.  A NaN makes
-    the norm and every gradient NaN; an infinite norm scales by 0."""
+    straight into the float32 rows that gpu_adam reads).  An output may be its own gradient, and shares no memory with another
+    output or gradient.  In place a norm of at most max_norm costs no write.  A NaN makes the norm and every gradient NaN; an
+    infinite norm scales by 0."""
     max_norm = float(max_norm)
     if not (max_norm >= 0.0 and eps >= 0.0):
         raise RuntimeError(f'max_norm and eps must be at least 0, got {max_norm} and {eps}')

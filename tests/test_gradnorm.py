@@ -6,6 +6,7 @@ two roundings and the product one, so an output is within 8 u before its own rou
 """
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -261,3 +262,77 @@ def test_python_refuses_host_tensors():
         gn.grad_norm([torch.zeros(3)])
     with pytest.raises(RuntimeError, match='must be a cuda'):
         gn.clip_grad_norm([torch.zeros(3)], 1.0)
+
+
+def _bytes_of(t):
+    idx = torch.zeros(t.shape, dtype=torch.int64)
+    for d, (n, s) in enumerate(zip(t.shape, t.stride())):
+        idx = idx + (torch.arange(n) * s).view([-1 if e == d else 1 for e in range(t.dim())])
+    return [t.data_ptr() + int(i) * t.element_size() + b for i in idx.reshape(-1) for b in range(t.element_size())]
+
+
+def test_overlap_is_exact():
+    """_lib.overlap and overlaps_itself against the sets of bytes, on random views of one buffer."""
+    rng = random.Random(3)
+    buf = torch.zeros(700)
+    found = [0, 0, 0, 0]
+    for _ in range(1500):
+        views = []
+        for _ in range(2):
+            dt = rng.choice((torch.float32, torch.bfloat16))
+            base = buf.view(dt)
+            shape = [rng.randint(1, 4) for _ in range(rng.randint(0, 3))]
+            stride = [rng.choice((0, 1, 2, 3, 4, 6, 8, 12, 24, 25)) for _ in shape]
+            views.append(base.as_strided(shape, stride, rng.randint(0, 60)))
+        sets = [_bytes_of(v) for v in views]
+        assert _lib.overlap(*views) == _lib.overlap(*views[::-1]) == bool(set(sets[0]) & set(sets[1]))
+        own = len(set(sets[0])) < len(sets[0])
+        assert _lib.overlaps_itself(views[0]) == own
+        found[bool(set(sets[0]) & set(sets[1]))] += 1
+        found[2 + own] += 1
+    assert min(found) > 100
+    rows = torch.zeros(1 << 20, 96)                                     # told apart without a list of their rows
+    assert not _lib.overlap(rows[:, :32], rows[:, 32:]) and not _lib.overlap(rows[:, ::2], rows[:, 1::2])
+    assert _lib.overlap(rows[:, :33], rows[:, 32:])
+
+
+def test_outputs_that_overlap():
+    gn = _gn()
+    flat = torch.zeros(300)
+    a, b = flat[:100], flat[100:200]
+    m = flat[:240].view(20, 12)
+    for grads, outs in (([a, b], [b, a]),                               # swapped
+                        ([flat[:200], flat[64:264]], None),             # at an offset
+                        ([a], [flat[1:101]]), ([a, flat[50:60]], [torch.zeros(100), a[:10]]),
+                        ([m], [flat[:240].view(12, 20).t()]),           # in place in another order
+                        ([m[:, :7], m[:, 6:]], None), ([m, m[3]], None), ([flat.as_strided((5, 5), (2, 1))], None),
+                        ([torch.zeros(100), b], [b, a])):
+        with pytest.raises(RuntimeError, match='overlaps'):
+            gn._check_outputs(grads, grads if outs is None else outs)
+    for grads, outs in (([a, b], None), ([a, a], [b, flat[200:]]), ([m[:, :7], m[:, 7:]], None), ([m[::2], m[1::2]], None),
+                        ([m[:, ::3].t(), m[:, 1::3], m[:, 2::3]], None), ([a, b], [a, flat[200:]]), ([a], [a.view(100)]),
+                        ([a.bfloat16()[:50], a], [a[:50].clone(), b]),
+                        ([flat[:0], flat[:0]], None), ([m.t(), m], [m.clone().t(), torch.zeros(20, 12)])):
+        gn._check_outputs(grads, grads if outs is None else outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('native', [True, False])
+def test_overlapping_outputs_are_refused(dev, monkeypatch, native):
+    """Both host paths refuse outputs that share memory, and run nothing."""
+    gn = _gn()
+    if not native:
+        monkeypatch.setattr(_lib, '_host', _lib._NoHost)
+    flat = _randn(dev, 1, 300)
+    keep = flat.clone()
+    a, b, half = flat[:100], flat[100:200], flat[:100].view(torch.bfloat16)[:100]
+    for grads, outs in (([a, b], [b, a]), ([flat, flat[64:]], None), ([flat[64:], flat], None), ([a], [flat[1:101]]),
+                        ([a, b], [b, torch.zeros_like(b)]), ([half], [a]), ([a, flat[40:60]], [a, torch.zeros(20, device=dev)])):
+        with pytest.raises(RuntimeError, match='overlaps'):
+            gn.clip_grad_norm(grads, 1.0, out=outs)
+        assert torch.equal(flat, keep)
+    m = flat[:240].view(20, 12)
+    check([m[:, :7], m[:, 7:]], 2.0, 1.0)
+    check([a.clone(), b], 2.0, 1.0, [torch.empty_like(a), b])
+    x = flat[:100].clone()
+    check([x, x], 2.0, 1.0, [torch.empty_like(x), torch.empty_like(x)])
