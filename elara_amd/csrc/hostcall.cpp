@@ -437,6 +437,14 @@ PyObject* norm_back(PyObject*, PyObject* const* a, Py_ssize_t na) {
   }
 }
 
+// A reference given back at the end of its block, with the GIL.
+struct Held {
+  PyObject* o;
+  explicit Held(PyObject* p) : o(p) {}
+  Held(const Held&) = delete;
+  ~Held() { Py_XDECREF(o); }
+};
+
 // A tensor's bytes.
 struct Range {
   uintptr_t begin, end;
@@ -469,17 +477,24 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
   double max_norm = 0, eps = 0;
   const bool scale = a[3] != Py_None;
   if (!integer(a[2], kind) || (scale && (!real(a[3], max_norm) || !real(a[4], eps)))) return not_taken();
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(a[0]);
+  // Tuples of its own: another thread may change the caller's lists while this one launches without the GIL, and the tensors
+  // have to outlive that.
   const bool outs = a[1] != Py_None;
-  if (n == 0 || (outs && PySequence_Fast_GET_SIZE(a[1]) != n)) return not_taken();
+  const Held ins(PySequence_Tuple(a[0])), to_outs(outs ? PySequence_Tuple(a[1]) : nullptr);
+  if (!ins.o || (outs && !to_outs.o)) {
+    PyErr_Clear();
+    return not_taken();
+  }
+  const Py_ssize_t n = PyTuple_GET_SIZE(ins.o);
+  if (n == 0 || (outs && PyTuple_GET_SIZE(to_outs.o) != n)) return not_taken();
   try {
     std::vector<elr_grad> list(static_cast<size_t>(n));
     std::vector<Range> ranges;      // of what a call that scales reads and writes; in place: once
     if (scale) ranges.reserve(static_cast<size_t>(outs ? 2 * n : n));
     const at::Tensor* first = nullptr;
     for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* to = PySequence_Fast_GET_ITEM(a[0], i);
-      PyObject* oo = outs ? PySequence_Fast_GET_ITEM(a[1], i) : to;
+      PyObject* to = PyTuple_GET_ITEM(ins.o, i);
+      PyObject* oo = outs ? PyTuple_GET_ITEM(to_outs.o, i) : to;
       const at::Tensor *t = plain(to), *o = oo == to ? t : plain(oo);
       if (!t || !o) return not_taken();
       if (!first) first = t;

@@ -7,6 +7,7 @@ two roundings and the product one, so an output is within 8 u before its own rou
 import ctypes
 import math
 import random
+import threading
 
 import pytest
 import torch
@@ -336,3 +337,27 @@ def test_overlapping_outputs_are_refused(dev, monkeypatch, native):
     check([a.clone(), b], 2.0, 1.0, [torch.empty_like(a), b])
     x = flat[:100].clone()
     check([x, x], 2.0, 1.0, [torch.empty_like(x), torch.empty_like(x)])
+
+
+@pytest.mark.gpu
+def test_a_list_changed_by_another_thread(dev):
+    """A call works on the tensors that its list held when it began, and keeps them: their norm is that of one whole list."""
+    gn = _gn()
+    lists = [[torch.full((5000 + i,), v, device=dev) for i in range(40)] for v in (1.0, 2.0)]
+    norms = {float(gn.grad_norm(x)) for x in lists}
+    torch.cuda.synchronize()
+    shared, stop = list(lists[0]), threading.Event()
+
+    def change():
+        v = 0
+        while not stop.is_set():
+            v = 1 - v
+            shared[:] = [t.clone() for t in lists[v]]
+    worker = threading.Thread(target=change)
+    worker.start()
+    try:
+        got = [gn.grad_norm(shared) for _ in range(200)]
+    finally:
+        stop.set()
+        worker.join()
+    assert {float(x) for x in got} <= norms and len(norms) == 2
