@@ -260,6 +260,28 @@ PyObject* wrap_or_none(const at::Tensor& t) {
   Py_RETURN_NONE;
 }
 
+// A tensor's bytes.
+struct Range {
+  uintptr_t begin, end;
+  bool out;
+};
+Range range_of(const at::Tensor& t, bool out) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + static_cast<uintptr_t>(t.numel() * t.element_size()), out};
+}
+// Whether an output meets another range (inputs may meet one another).
+bool meet(std::vector<Range>& r) {
+  const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+  uintptr_t out_end = 0, end = 0;
+  for (const Range& x : r) {
+    if (x.begin < (x.out ? end : out_end)) return true;
+    end = std::max(end, x.end);
+    if (x.out) out_end = std::max(out_end, x.end);
+  }
+  return false;
+}
+
 // logprobs(logits, tokens, k) -> (return code, logprob, lse, entropy, top_logprob, top_id), or NOT_TAKEN
 PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (na != 3 || !f_lp) return not_taken();
@@ -320,6 +342,10 @@ PyObject* logprobs_back(PyObject*, PyObject* const* a, Py_ssize_t na) {
       return not_taken();
   if (out && (out->scalar_type() != x->scalar_type() || out->device() != x->device() || out->sizes() != x->sizes()))
     return not_taken();
+  if (out && out->data_ptr() != x->data_ptr()) {
+    std::vector<Range> ranges{range_of(*x, false), range_of(*out, true)};
+    if (meet(ranges)) return not_taken();
+  }
   try {
     at::Tensor made;
     int rc = kNotTaken;
@@ -444,28 +470,6 @@ struct Held {
   Held(const Held&) = delete;
   ~Held() { Py_XDECREF(o); }
 };
-
-// A tensor's bytes.
-struct Range {
-  uintptr_t begin, end;
-  bool out;
-};
-Range range_of(const at::Tensor& t, bool out) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return {p, p + static_cast<uintptr_t>(t.numel() * t.element_size()), out};
-}
-// Whether an output meets another range (inputs may meet one another).
-bool meet(std::vector<Range>& r) {
-  const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
-  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
-  uintptr_t out_end = 0, end = 0;
-  for (const Range& x : r) {
-    if (x.begin < (x.out ? end : out_end)) return true;
-    end = std::max(end, x.end);
-    if (x.out) out_end = std::max(out_end, x.end);
-  }
-  return false;
-}
 
 // clip(grads, out or None, kind, max_norm or None, eps) -> (return code, norm), or NOT_TAKEN; max_norm None: the norm alone
 PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {

@@ -98,8 +98,9 @@ def token_logprobs_backward(logits, tokens, lse, entropy, d_logprob, d_entropy=N
     shape.  lse and entropy are token_logprobs' (entropy may be None without d_entropy); d_* are float32 of tokens' shape,
     None for zero.  Rows without a token get nothing from d_logprob; rows of nothing but -inf, or nothing but
     float32's or bfloat16's lowest value, get 0.  Where |lse| is 256 or more (a large offset common to the row) lse's last
-    digits no longer tell p, and the row's sum is taken again (a slower pass over it).  out: where to write it, a tensor of the logits' shape and type whose rows lie apart by a fixed stride; the logits themselves are allowed,
-    and are then overwritten."""
+    digits no longer tell p, and the row's sum is taken again (a slower pass over it).  out: where to write it, a
+    tensor of the logits' shape and type whose rows lie apart by a fixed stride; the logits themselves are allowed, and are
+    then overwritten, but no other memory of theirs."""
     r = (_lib._host or _lib.host()).logprobs_back(logits, tokens, lse, entropy, d_logprob, d_entropy, d_lse, out)
     if r != _lib.NOT_TAKEN:
         _lib.check(r[0], 'elr_token_logprobs_backward')
@@ -125,6 +126,8 @@ def token_logprobs_backward(logits, tokens, lse, entropy, d_logprob, d_entropy=N
     o = out if out.dim() == 2 else out.view(n, V)      # (view raises where no fixed row stride exists)
     if (V > 1 and o.stride(1) != 1) or (n > 1 and o.stride(0) < V):
         raise RuntimeError('out must have contiguous rows that do not overlap')
+    if (o.data_ptr(), _ld(o)) != (x.data_ptr(), _ld(x)) and _lib.overlap(o, x):
+        raise RuntimeError('out must be the logits themselves or share no memory with them')
     with _lib.on_device(dev):
         rc = _lib.lib().elr_token_logprobs_backward(
             x.data_ptr(), _lib.ETYPE[x.dtype], n, V, _ld(x), tok.data_ptr(), int(tok.dtype == torch.int64), _lib.ptr(lse),

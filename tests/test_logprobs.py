@@ -440,6 +440,36 @@ def test_refusals(dev):
     lp.token_logprobs(x, tok - 100, check=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('native', [True, False])
+def test_out_that_overlaps_the_logits(dev, monkeypatch, native):
+    """Refused unless it is the logits themselves; other columns of the same rows, or the memory of logits that were copied
+    for their strides, are taken."""
+    lp = _lp()
+    if not native:
+        monkeypatch.setattr(_lib, '_host', _lib._NoHost)
+    flat = _randn(dev, 1, 1100)
+    keep = flat.clone()
+    x, tok = flat[:1000].view(10, 100), torch.arange(10, device=dev)
+    r = lp.token_logprobs(x, tok)
+    one = torch.ones(10, device=dev)
+    wide = flat[:1080].view(10, 108)
+    for logits, out in ((x, flat[4:1004].view(10, 100)), (x, flat[100:].view(10, 100)), (wide[:, :100], wide[:, 8:]),
+                        (wide[:, :100], wide[:, 1:101]), (x[:1].expand(10, 100), x), (x, flat[:1080].view(10, 108)[:, :100])):
+        with pytest.raises(RuntimeError, match='out must be'):
+            lp.token_logprobs_backward(logits, tok, r.lse, None, one, out=out)
+        assert torch.equal(flat, keep)
+    half = flat[:1000].view(5, 200)
+    f = lp.token_logprobs(half[:, :100], tok[:5])
+    want = lp.token_logprobs_backward(half[:, :100].contiguous(), tok[:5], f.lse, None, one[:5])
+    got = lp.token_logprobs_backward(half[:, :100], tok[:5], f.lse, None, one[:5], out=half[:, 100:])
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-7) and torch.equal(half[:, :100], keep[:1000].view(5, 200)[:, :100])
+    sq = flat[:900].view(30, 30)
+    f = lp.token_logprobs(sq.t(), tok[0].expand(30))
+    want = lp.token_logprobs_backward(sq.t().contiguous(), tok[0].expand(30), f.lse, None, one[0].expand(30))
+    assert torch.equal(lp.token_logprobs_backward(sq.t(), tok[0].expand(30), f.lse, None, one[0].expand(30), out=sq), want)
+
+
 def test_cabi_refusals():
     """Arguments that the library refuses on the host (none of these calls reaches the GPU)."""
     L = _lib.lib()
