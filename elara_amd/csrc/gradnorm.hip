@@ -11,7 +11,7 @@
 //
 // Sums are fp64: no overflow or underflow of squares, and the norm is exact to its one rounding to fp32.  It costs nothing
 // (fp32 sums: 131 us against 133 for 717 MB).  A NaN gives a NaN norm; a norm of +inf gives c = 0 (so inf * 0 = NaN where a
-// gradient was inf), as dividing by it does.
+// gradient was inf), as dividing by it does, unless max_norm is +inf too; no gradient and eps = 0 gives c = 1.
 //
 // The tensors travel in the kernel arguments, kList of them a launch: nothing is copied to the device ahead, and a captured
 // graph holds its own list.  Each is cut into chunks of 16 KB.
@@ -211,7 +211,9 @@ __device__ __forceinline__ float coef_of(const Clip& k, Acc<P>* lds) {
   } else {
     x = *k.norm;
   }
-  const float c = k.max_norm / (x + k.eps);
+  const float d = x + k.eps;
+  if (d == 0.0f || (d == __builtin_inff() && k.max_norm == d)) return 1.0f;   // nothing to scale, or no bound: not 0/0, inf/inf
+  const float c = k.max_norm / d;
   return c > 1.0f ? 1.0f : c;    // NaN stays
 }
 

@@ -135,7 +135,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None):
     In place, or into out: a list of tensors of grads' shapes, each of its gradient's type or float32 (16-bit gradients
     straight into the float32 rows that gpu_adam reads).  An output may be its own gradient, and shares no memory with another
     output or gradient.  In place a norm of at most max_norm costs no write.  A NaN makes the norm and every gradient NaN; an
-    infinite norm scales by 0."""
+    infinite norm scales by 0, unless max_norm is infinite too, which never scales; gradients of nothing but 0 stay."""
     max_norm = float(max_norm)
     if not (max_norm >= 0.0 and eps >= 0.0):
         raise RuntimeError(f'max_norm and eps must be at least 0, got {max_norm} and {eps}')

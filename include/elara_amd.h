@@ -790,7 +790,8 @@ int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_t D, int64_
  * The global norm of many gradients, and clipping by it (no counterpart in the reference).
  *   norm = (sum |g|^p)^(1/p) over all elements of all n tensors, p = 1, 2, or 0 for the largest |g| (summed in fp64);
  *   clip: out = g min(1, max_norm / (norm + eps)) for each tensor.
- * A NaN makes the norm NaN, and then the outputs; an infinite norm scales by 0.
+ * A NaN makes the norm NaN, and then the outputs; an infinite norm scales by 0, or by 1 if max_norm is infinite too;
+ * norm = eps = 0 scales by 1.
  * ------------------------------------------------------------------------------------------------------- */
 typedef struct elr_grad {
   const void* data;

@@ -361,3 +361,26 @@ def test_a_list_changed_by_another_thread(dev):
         stop.set()
         worker.join()
     assert {float(x) for x in got} <= norms and len(norms) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [10, 5_000_000])
+@pytest.mark.parametrize('out', [False, True])
+def test_nothing_to_scale(dev, dtype, n, out):
+    """0 / 0 and inf / inf: gradients of nothing but zeros with max_norm = eps = 0, and an infinite norm without a bound."""
+    gn = _gn()
+    for max_norm, eps in ((0.0, 0.0), (1.0, 0.0), (INF, 0.0)):
+        g = torch.zeros(n, dtype=dtype, device=dev)
+        o = torch.full((n,), 7.0, device=dev)
+        assert float(gn.clip_grad_norm([g], max_norm, eps=eps, out=[o] if out else None)) == 0
+        assert not (o if out else g).any()
+    for p in (1.0, 2.0, INF):
+        g = torch.ones(n, dtype=dtype, device=dev)
+        g[-1] = -INF
+        o = torch.zeros(n, device=dev)
+        assert float(gn.clip_grad_norm([g], INF, p, out=[o] if out else None)) == INF
+        assert torch.equal((o if out else g).float(), torch.cat([torch.ones(n - 1, device=dev), g.new_full((1,), -INF).float()]))
+        g[0] = float('nan')
+        gn.clip_grad_norm([g], INF, p, out=[o] if out else None)
+        assert torch.isnan(o if out else g).all()
