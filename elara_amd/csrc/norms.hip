@@ -552,18 +552,19 @@ __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
   }
 }
 
-// dw[e] = sum over the blocks' partial rows, in a fixed order: 32 columns a block, 32 threads a column, each every 32nd row.
-__global__ __launch_bounds__(1024) void k_norm_dw(const float* part, int rows, int32_t D, float* dw) {
+// dw[e] = sum over the blocks' partial rows, D apart, in a fixed order: 32 columns a block, 32 threads a column, each every 32nd
+// row.
+__global__ __launch_bounds__(1024) void k_norm_dw(const float* part, int rows, int32_t D, int32_t cols, float* dw) {
   __shared__ float s[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + c;
   float x = 0.0f;
-  if (e < D)
+  if (e < cols)
 #pragma unroll 8
     for (int r = g; r < rows; r += 32) x = x + part[(int64_t)r * D + e];
   s[g][c] = x;
   __syncthreads();
-  if (g == 0 && e < D) {
+  if (g == 0 && e < cols) {
     float t = s[0][c];
 #pragma unroll
     for (int i = 1; i < 32; ++i) t = t + s[i][c];
@@ -610,6 +611,7 @@ static void launch_norm(const NormArgs& a, hipStream_t st) {
 }
 
 constexpr int64_t kNormRowsPerLaunch = 1 << 21;   // (a grid has less than 2^32 threads)
+constexpr int64_t kDwColumns = 1 << 26;
 
 template <class E, class R>
 static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {
@@ -742,8 +744,12 @@ extern "C" int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_
         break;
     }
   }
-  if (dweight && (n == 0 || blocks > 1))   // no rows: zeros
-    k_norm_dw<<<(unsigned)((D + 31) / 32), 1024, 0, st>>>((const float*)scratch, n > 0 ? (int)blocks : 0, (int32_t)D,
-                                                         dweight);
+  if (dweight && (n == 0 || blocks > 1)) {   // no rows: zeros
+    for (int64_t e = 0; e < D; e += kDwColumns) {
+      const int64_t m = D - e < kDwColumns ? D - e : kDwColumns;
+      k_norm_dw<<<(unsigned)((m + 31) / 32), 1024, 0, st>>>(n > 0 ? (const float*)scratch + e : nullptr,
+                                                           n > 0 ? (int)blocks : 0, (int32_t)D, (int32_t)m, dweight + e);
+    }
+  }
   return launch_status();
 }

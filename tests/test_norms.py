@@ -288,6 +288,24 @@ def test_more_rows_than_a_launch(dev):
         assert torch.equal(q.y[s].view(torch.uint8), wq.y.view(torch.uint8)) and torch.equal(q.scale[s], wq.scale)
 
 @pytest.mark.gpu
+def test_weight_gradient_of_more_columns_than_a_launch(dev):
+    """Rows of 2^27 + 33: the sum of the blocks' weight gradients takes several launches; without rows it is 0."""
+    nm = _nm()
+    n, D = 4, (1 << 27) + 33
+    empty = torch.zeros(0, D, dtype=torch.bfloat16, device=dev)
+    dw = nm.rms_norm_backward(empty, empty, None, torch.zeros(0, device=dev))[1]
+    assert dw.shape == (D,) and not dw.any()
+    i = torch.arange(D, device=dev)
+    h = torch.stack([((i + 3 * r) % 251 - 125).to(torch.bfloat16) for r in range(n)])
+    dy = torch.stack([((i + r) % 7 - 3).to(torch.bfloat16) for r in range(n)])
+    rstd = torch.tensor([0.5, 0.25, 1.0, 2.0], device=dev)               # whole numbers and powers of two: sums are exact
+    dw = nm.rms_norm_backward(dy, h, None, rstd)[1]
+    for a in range(0, D, 1 << 25):
+        s = slice(a, min(D, a + (1 << 25)))
+        assert torch.equal(dw[s], (dy[:, s].float() * h[:, s].float() * rstd[:, None]).sum(0))
+
+
+@pytest.mark.gpu
 def test_streams_graph_and_repeats(dev):
     """A side stream and every replay of a graph give the eager bits; so do repeated calls (the weight gradient's order)."""
     nm = _nm()
