@@ -20,7 +20,7 @@ _KINDS = {1.0: 1, 2.0: 2, math.inf: 0}
 def _two_strides(t, o):
     """(rows, cols, ld, cs, out_ld, out_cs) of t's elements and o's in the same order, neighbouring dimensions merged."""
     dims = []
-    for d in sorted(range(t.dim()), key=lambda i: (-t.stride(i), -t.shape[i])):
+    for d in sorted(range(t.dim()), key=lambda i: (-t.stride(i), -o.stride(i), -t.shape[i])):
         if t.shape[d] == 1:
             continue
         ts, os = t.stride(d), o.stride(d)

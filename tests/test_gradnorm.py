@@ -384,3 +384,25 @@ def test_nothing_to_scale(dev, dtype, n, out):
         g[0] = float('nan')
         gn.clip_grad_norm([g], INF, p, out=[o] if out else None)
         assert torch.isnan(o if out else g).all()
+
+
+def test_two_strides_of_broadcast_gradients():
+    """A gradient broadcast over three dimensions or more (a sum's) into a dense output is one run of the output's memory."""
+    gn = _gn()
+    for shape in ((2, 3, 4), (4, 3, 2), (3, 3, 3), (5, 1, 4, 2)):
+        t, o = torch.zeros(1).expand(shape), torch.zeros(shape)
+        rows, cols, ld, cs, old, ocs = gn._two_strides(t, o)
+        assert rows * cols == o.numel() and (ld, cs) == (0, 0)
+        assert sorted(i * old + j * ocs for i in range(rows) for j in range(cols)) == list(range(o.numel()))
+        p = o.permute(*reversed(range(o.dim())))
+        rows, cols, ld, cs, old, ocs = gn._two_strides(t.permute(*reversed(range(o.dim()))), p)
+        assert rows * cols == o.numel() and sorted(i * old + j * ocs for i in range(rows) for j in range(cols)) == list(range(o.numel()))
+
+
+@pytest.mark.gpu
+def test_broadcast_gradients(dev):
+    for shape in ((2, 3, 4), (4, 3, 2), (7, 5, 6, 3), (30, 40, 50)):
+        g = torch.full((1,), 0.5, device=dev)
+        check([g.expand(shape)], 2.0, 1.0, [torch.empty(shape, device=dev)])
+        check([g.to(torch.bfloat16).expand(shape), _randn(dev, 1, *shape)], 1.0, 1.0,
+              [torch.empty(shape, device=dev), torch.empty(shape, device=dev)])
