@@ -331,6 +331,35 @@ def test_gradient_against_differences(dev, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('V', [40, 3000])
+@pytest.mark.parametrize('part', ['logprob', 'entropy', 'lse'])
+def test_each_gradient_along_its_own_sign(dev, V, part):
+    """One output at a time, along the signs of its reference gradient: the derivative is that gradient's 1-norm, more than ten
+    times what the difference may err by, so a term that is missing, halved or turned round fails.  With |v| <= 1 the third
+    derivatives are sums of cumulants of v and x: at most 8 for logprob and lse, 2 * 8 + 32 E|x - E x| < 80 for the entropy.
+    The forward's error is e (2 + entropy) + 4 u |f| (|f| < 13) at each end, the ends' rounding 4.5 u of each logit."""
+    lp = _lp()
+    n, s = 6, 2.0 ** -6
+    x = _randn(dev, V, n, V, scale=1.0)
+    tok = torch.arange(n, device=dev) * 5
+    ones, none = torch.ones(n, device=dev), np.zeros(n)
+    which = [part == p for p in ('logprob', 'entropy', 'lse')]
+    ref = ref_backward(x.double().cpu().numpy(), tok.cpu().numpy(), *(none + w for w in which))[0]
+    v = torch.from_numpy(np.sign(ref)).float().to(dev)
+    r = lp.token_logprobs(x, tok)
+    d = lp.token_logprobs_backward(x, tok, r.lse, r.entropy, *(ones if w else None for w in which))
+
+    def f(y):
+        return getattr(lp.token_logprobs(y, tok), part).double()
+    dot = (d.double() * v.double()).sum(1)
+    diff = (f(x + s * v) - f(x - s * v)) / (2 * s)
+    e = (V / 64 + 2 * math.log(V) + 64) * U
+    err = (e * (2 + math.log(V)) + 4 * 13 * U + 2 * 4.5 * U) / s + 80 * s * s / 6
+    assert float((dot - diff).abs().max()) < err
+    assert float(diff.abs().min()) > 10 * err
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(dev):
     """The last rows of 2.2 * 10^9 logits: element offsets past 2^31, byte offsets past 2^32."""
     lp = _lp()

@@ -262,6 +262,44 @@ def test_gradient_against_differences(dev, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('D', [48, 4096])
+def test_gradients_along_their_own_signs(dev, D):
+    """Central differences along the signs of the reference gradients, and along x's, where only the term with the row's mean
+    keeps the derivative small (dy has a part along x): each is checked against more than ten times what the difference may
+    err by.  For |v| <= 1, q = mean h^2 + eps and c = q^(-1/2): |q'| <= 2 (sqrt(q) + s), |q''| <= 2, and the third derivative of
+    a row's y is at most (|x| + s) times c's third, plus 3 times its second, of each weight."""
+    nm = _nm()
+    n, s = 4, 2.0 ** -7
+    x, w = _randn(dev, 1, n, D), 1 + 0.1 * _randn(dev, 2, D)
+    dy = _randn(dev, 5, n, D) + x
+    X, W, G = x.double(), w.double(), dy.double()
+    _, c, y = _ref(x, w, None)
+    c = c[:, None]
+    mean = (G * W * X * c).mean(-1, keepdim=True)
+    dx_ref, dw_ref = c * (G * W - X * c * mean), (G * X * c).sum(0)
+
+    def f(a, b):
+        return float((nm.rms_norm(a, b).y.double() * G).sum())
+    out = nm.rms_norm(x, w)
+    dx, dw = (t.double() for t in nm.rms_norm_backward(dy, out.h, w, out.rstd))
+    q = (X * X).mean(-1, keepdim=True) + EPS
+    low, q1 = (q.sqrt() - s) ** 2, 2 * (q.sqrt() + s)
+    c2 = 0.75 * low ** -2.5 * q1 ** 2 + low ** -1.5
+    c3 = 15 / 8 * low ** -3.5 * q1 ** 3 + 9 / 2 * low ** -2.5 * q1
+    third = float(((G * W).abs() * ((X.abs() + s) * c3 + 3 * c2)).sum())
+    err_w = 1.1 * float((G * y).abs().sum()) * (_adds(D) + 12 * U) / s
+    err = err_w + third * s * s / 6
+    for v in (dx_ref.sign(), X.sign()):
+        t = (s * v).float()
+        diff = (f(x + t, w) - f(x - t, w)) / (2 * s)
+        assert abs(float((dx * v).sum()) - diff) < err
+    assert float(dx_ref.abs().sum()) > 10 * err and abs(float((X.sign() * X * c * c * mean).sum())) > 10 * err
+    t = (s * dw_ref.sign()).float()
+    diff = (f(x, w + t) - f(x, w - t)) / (2 * s)
+    assert abs(float((dw * dw_ref.sign()).sum()) - diff) < err_w and diff > 10 * err_w
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(dev):
     nm = _nm()
     n, D = 1_050_000, 2048                                  # 2.15 * 10^9 elements
