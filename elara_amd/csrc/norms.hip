@@ -16,7 +16,9 @@
 // Loads are non-temporal (read once; plain ones 3 to 14 % slower on 537 MB).  16,384 rows of 4,096 bf16 with a residual (537
 // MB) take 84 us (6.4 TB/s); their backward 85 us and 5 for the sum of the weight gradients (6.0 TB/s); that of 425,984 rows
 // of 128 fp32 (656 MB) 109 and 5 (5.8 TB/s).  fp8 of 8,192 rows of 2,048 with groups of 128 (118 MB): 24 us (4.9 TB/s, of
-// which a launch is 3 us).
+// which a launch is 3 us); of 16,384 rows of 4,096 with a scale a row (470 MB) 82 us (5.8 TB/s).  An fp32 residual stream
+// under bf16: 16,384 of 1,024 40 us forward (5.0 TB/s) and 51 backward (4.6), of 4,096 206 (3.9) and 243 (3.9).  2,048 rows of
+// 20,480, which are read more than once: 66 us (5.1 TB/s), backward 245 (1.4).
 #include "elr_elem.h"
 
 namespace elr {
@@ -106,8 +108,8 @@ __device__ __forceinline__ void res_store(R* p, const Frag<E>& f, int64_t valid,
 // The scale of values up to m, and what divides by it.  The quotient is the correctly rounded one: q = y RN(1 / s) is within
 // two ulps, its residual q s - y is exact in one fma, and a second fma takes it off (Markstein's theorem, for a correctly
 // rounded reciprocal).  A product with the reciprocal alone takes values at e4m3's ties to the wrong side.  8,192 rows of 2,048
-// take 24 us either way; a division for each value cost 5 us more.  A scale below 2^-80, whose residuals could underflow, and
-// one that is infinite or NaN, divides.
+// take 24 us either way, and 27 with a division for each value.  A scale below 2^-80, whose residuals could underflow, and one
+// that is infinite or NaN, divides.
 struct Scale {
   float s, inv;
   bool exact;
@@ -370,9 +372,10 @@ struct NormBackArgs {
   int nt;
 };
 
-// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time, `teams` apart; AHEAD: with
-// the next ones' loads in flight (a wave's rows: 121 us, 130 without; a block's: 95, and 91 without).  Its weight gradient stays in registers until the end, then the block's teams are added in a fixed order.
-template <class E, class R, int T, int NV, int U, bool AHEAD>
+// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time, `teams` apart.  (With the next rows'
+// loads in flight: 425,984 rows of 128 fp32 114 us either way, 16,384 of 4,096 bf16 95 us against 89.)  Its weight gradient
+// stays in registers until the end, then the block's teams are added in a fixed order.
+template <class E, class R, int T, int NV, int U>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
   extern __shared__ float dwsum[];     // [D], only with a.part
@@ -454,25 +457,10 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
       }
     }
   };
-  if constexpr (AHEAD) {
-    Rows x, y;
-    int64_t b = base;
-    if (b < a.n) load(x, b);
-    while (b < a.n) {
-      load(y, b + teams * U);
-      compute(x, b);
-      b += teams * U;
-      if (b >= a.n) break;
-      load(x, b + teams * U);
-      compute(y, b);
-      b += teams * U;
-    }
-  } else {
-    for (int64_t b = base; b < a.n; b += teams * U) {
-      Rows x;
-      load(x, b);
-      compute(x, b);
-    }
+  for (int64_t b = base; b < a.n; b += teams * U) {
+    Rows x;
+    load(x, b);
+    compute(x, b);
   }
   if (!a.part) return;
   if constexpr (T == 64) {
@@ -632,10 +620,12 @@ static void norm_rows(NormArgs a, bool fp8, hipStream_t st) {
 }
 
 // Blocks of the backward: enough to fill the chip, few enough that the partial weight gradients (written and read once, D
-// fp32 a block) stay a small part of the rows' traffic; a block of 1,024 threads fills a CU (4,000 rows of 8,192 bf16: 43 us
-// with 256 blocks, 49 with 512), four of 256 do (12,094 rows of 1,536: 31 us with 1,024 blocks, 40 with 512).  Two rows a
-// block where they are few (822 of 1,000 fp16: 11.6 us, 12.9 with one), and one block, which needs no addition of partial
-// sums, for what up to three would do (30 rows of 64 fp32: 4.4 us, 5.9 with two blocks).
+// fp32 a block) stay a small part of the rows' traffic.  bf16 but where said: a block of 1,024 threads fills a CU (4,000 rows
+// of 8,192: 53 us with 256 blocks, 59 with 512; 8,192 of 5,120 69 and 75; 4,000 of 4,096 fp32 47 either way).  Blocks of 256,
+// four a CU: 12,094 of 1,536 38 us with 1,024 blocks, 46 with 512, though 16,384 of 2,048 take 54 and 52, 5,000 of 1,024 fp32
+// 21 and 20.  Two rows a block where they are few (822 of 1,000 fp16 12.5 us, 14.0 with one; 200 of 4,096 9.2 and 10.3), and
+// one block, which needs no addition of partial sums, for what up to three would do (30 of 64 fp32 6.0 us, 8.2 with two; 3 of
+// 4,096 6.1 and 8.5).
 constexpr int64_t kBackBlocks = 512, kBackBlocksMost = 1024, kBackFew = 32, kBackOne = 3;
 static int64_t back_blocks(int64_t n, int64_t D, int type) {
   const Team t = team_of((D + 16 / elem_size(type) - 1) / (16 / elem_size(type)), 2);
@@ -655,14 +645,14 @@ static void launch_norm_back(const NormBackArgs& a, unsigned blocks, hipStream_t
   const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, 2);
   const size_t lds = a.part ? (size_t)a.D * 4 : 0;
   switch (t.T * 8 + t.NV) {
-    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 1, true><<<blocks, 256, lds, st>>>(a, t.lg); break;
-    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2, false><<<blocks, 256, lds, st>>>(a, 6); break;
-    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2, false><<<blocks, 256, 0, st>>>(a, 6); break;
-    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1, false><<<blocks, 512, 0, st>>>(a, 6); break;
-    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1, false><<<blocks, 1024, 0, st>>>(a, 6); break;
+    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 1><<<blocks, 256, lds, st>>>(a, t.lg); break;
+    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2><<<blocks, 256, lds, st>>>(a, 6); break;
+    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2><<<blocks, 256, 0, st>>>(a, 6); break;
+    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1><<<blocks, 512, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1><<<blocks, 1024, 0, st>>>(a, 6); break;
     case 1024 * 8 + 2:
       if constexpr (sizeof(E) == sizeof(R)) {
-        k_norm_back<E, R, 1024, 2, 1, false><<<blocks, 1024, 0, st>>>(a, 6);
+        k_norm_back<E, R, 1024, 2, 1><<<blocks, 1024, 0, st>>>(a, 6);
         break;
       }
       [[fallthrough]];   // (its registers would spill)
