@@ -260,8 +260,9 @@ _host = None
 
 
 def host():
-    """The native argument checks of the row ops and of the operators (csrc/hostcall.cpp), bound to the loaded library.  Without the module,
-    or with one built for another torch or Python, a warning says so once and the Python path takes every call."""
+    """The native argument checks of the row ops and of the operators (csrc/hostcall.cpp), bound to the loaded library.
+    Without the module, or with one built for another torch or Python, a warning says so once and the Python path takes
+    every call."""
     global _host
     if _host is None:
         L = lib()

@@ -14,7 +14,9 @@
 // gradient was inf), as dividing by it does, unless max_norm is +inf too; no gradient and eps = 0 gives c = 1.
 //
 // The tensors travel in the kernel arguments, kList of them a launch: nothing is copied to the device ahead, and a captured
-// graph holds its own list.  Each is cut into chunks of 16 KB.
+// graph holds its own list.  Each is cut into chunks of 16 KB.  A tensor that is not one run of memory has launches of its own,
+// a thread an element with a 64-bit division for its place: 8,192 x 8,192 in rows 8,256 apart fp32 105 us for the norm and 234
+// with the scaling (48 and 130 as one run), bf16 102 and 206 (28 and 74).
 //
 // Measured: 641 MB of bf16 gradients packed next to one another and 77 MB of fp32 rows, into fp32 (240 tensors): sum 125 us
 // (5.7 TB/s), scaling 322 us (6.4 TB/s; the sum's last reads are still in the last-level cache when the scaling, which goes

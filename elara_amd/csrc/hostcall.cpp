@@ -1,7 +1,7 @@
 // Host side of the row ops' Python entry points: the argument checks and the C-ABI call of ops.gpu_adam,
 // gpu_ops.init_rows and gpu_ops.replay_rows in one native call, and of the operators in logprobs, norms and gradnorm, for
-// the arguments a training loop passes (plain contiguous GPU tensors of the expected types on the current device).  Everything else -- other types, strides or
-// devices, arenas in host memory, wrapped tensors, errors -- is answered with NOT_TAKEN, and the Python path then
+// the arguments a training loop passes (plain contiguous GPU tensors of the expected types on the current device).
+// Everything else -- other types, strides or devices, arenas in host memory, wrapped tensors, errors -- is answered with NOT_TAKEN, and the Python path then
 // converts, raises or runs as it always has, so the two accept and refuse the same calls.
 //
 // Why: at a few hundred rows a call is host time.  The Python checks and ctypes conversions of gpu_adam took 3.7 of its

@@ -11,7 +11,7 @@
 // fp32), so that e * (x - m) is 0 there too and not 0 * inf.  A row of nothing but -inf has s = 0: lse and logprob are
 // -inf, entropy 0, and no gradient.  A NaN (or +inf) anywhere gives NaN, as the formula does: the clamp keeps a NaN.
 //
-// The k likeliest (k <= 32) need no second pass over the row.  Among the maxima of 64 disjoint parts of it (the lanes', taken
+// The k likeliest (k <= 32) need no second pass over the row, but for a few of its places.  Among the maxima of 64 disjoint parts of it (the lanes', taken
 // anyway) the k-th largest is a lower bound of the row's k-th largest element; about 64 ln(64 / (64 - k)) elements of a
 // random row reach it.  A part that fits the block's registers is searched there.  A longer one keeps the maximum of each
 // thread's chunks in LDS, and only chunks whose maximum reaches the bound are read again, a vector per lane.  The elements
@@ -23,8 +23,11 @@
 // Measured (bf16 but where said): 4,096 rows of 32,768 47 us (5.7 TB/s), with k = 5 52; 1,024 of 131,072 46 (5.8 TB/s);
 // 1,024 of 100,003 fp32 63 (6.5 TB/s); one row of 131,072 in 64 splits 4.4, with k = 20 10.  An element costs ten
 // instructions, one of them an exponential, about 42 cycles of a SIMD for 64 of them: 36 of the 47 us above.  (The exponent
-// as one fma, with another path for rows at a type's lowest value, gained nothing: 45.5 and 52.)
-// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 338 us (6.3 TB/s), 301 of 50,021 fp32 21 us (5.6 TB/s).
+// as one fma, with another path for rows at a type's lowest value, gained nothing: 45.5 and 52.)  Many shorter rows pay more for
+// the k likeliest, which one wave or block of each row selects and ranks while its lanes are idle: 16,384 of 4,096 24 us without,
+// 41, 44 and 48 with k = 5, 20 and 32; 60,000 of 1,000 25, and 86 with 20; 200,000 of 100 19, and 158, 281 and 296.
+// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 338 us (6.3 TB/s), 301 of 50,021 fp32 21 us (5.6 TB/s); a wave a row at least:
+// 60,000 of 1,000 66 us (3.7 TB/s), 200,000 of 100 78 (1.1).
 #include "elr_elem.h"
 
 namespace elr {
@@ -807,8 +810,7 @@ __device__ __forceinline__ bool back_vecs(const LpBackArgs& a, int64_t row, cons
 }
 
 // A whole wide row by one wave.  In place no other wave may write before the sum is taken, so the row's other waves leave it
-// alone.  4,096 rows of 131,072 bf16, all wide, take 1,133 us (338 where none is), one such row
-// alone 130.
+// alone.  4,096 rows of 131,072 bf16, all wide, take 1,133 us (338 where none is), one such row alone 130.
 template <class E>
 __device__ __forceinline__ void back_wide(const LpBackArgs& a, int64_t row, const E* x, E* out) {
   constexpr int VE = Elem<E>::VE, U = 16 / VE;      // (more vectors a step would cost the other rows' waves registers)

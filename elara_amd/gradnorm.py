@@ -5,8 +5,11 @@ reference, whose step updates unclipped.
     clip_grad_norm(grads, max_norm, norm_type=2.0, eps=1e-6, out=None) -> norm   grads scaled by min(1, max_norm / (norm + eps))
 
 They run the HIP kernels behind elr_grad_norm and elr_clip_grad_norm (elara_amd/csrc/gradnorm.hip) on torch's current
-stream: two launches for up to 136 tensors, and no host synchronisation.  A batch's summed row gradients
-(dedup.embedding_dense_backward, dedup.segment_sum_plan) are one of the tensors.
+stream, without a host synchronisation: two launches for up to 136 tensors that are each one run of memory, of up to 16 MB
+together, a third beyond that, two more for each further 136 and for each tensor that is not one run (an element a thread
+there: 2 to 4 times the time).  A batch's summed row gradients (dedup.embedding_dense_backward, dedup.segment_sum_plan) are one
+of the tensors; the sums that ElaraStep takes within its native step are not reachable, so only a loop over the row ops (or the
+host-planned step's plan and update) can clip.  Gradients are written without bumping their version.
 """
 import math
 
@@ -126,7 +129,7 @@ def _check_outputs(grads, outs):
 def grad_norm(grads, norm_type=2.0):
     """(sum |g|^p)^(1/p) over every element of every tensor of grads (p = norm_type: 1, 2 or inf), as a float32 scalar on
     the GPU.  grads: cuda float32, float16 or bfloat16 tensors of one device, of any shapes and of strides that reduce to
-    two.  Summed in float64; the order of the additions depends on the sizes alone."""
+    two.  Summed in float64; the order of the additions depends on the sizes, strides and alignments alone."""
     return _run(grads, None, _kind(norm_type), None)
 
 

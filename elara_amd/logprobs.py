@@ -8,7 +8,8 @@ sigmoid, srm2/models.py).
                                                              the gradient to the logits
 
 Both run the HIP kernels behind elr_token_logprobs and elr_token_logprobs_backward (elara_amd/csrc/logprobs.hip) on torch's
-current stream, without a host synchronisation.  The row is read once, whatever k.
+current stream, without a host synchronisation.  The row is read once, and with k a few of its places again (all of it where the
+large logits crowd).  Neither registers with autograd: results are detached, and what is written into `out` bumps no version.
 """
 from typing import NamedTuple, Optional
 

@@ -6,7 +6,8 @@ counterpart in the reference.
     rms_norm_backward(dy, h, weight, rstd, dh=None) -> (dx, dweight)
 
 They run the HIP kernels behind elr_rms_norm and elr_rms_norm_backward (elara_amd/csrc/norms.hip) on torch's current
-stream: one launch forward (each row is read and written once), two backward.
+stream: one launch forward (each row is read and written once; rows of more than 4,096 16-byte vectors are read again), two
+backward (one where the rows are few).  Neither registers with autograd: results are detached.
 """
 from typing import NamedTuple
 

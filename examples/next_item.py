@@ -117,7 +117,8 @@ class NextItem:
         return loss, norm
 
     def likeliest(self, ids, k=5):
-        """The k likeliest next items of each id and their log probabilities, the output product's input in fp8."""
+        """The k likeliest next items of each id and their log probabilities, the output product's input in fp8.  (This library
+        has no fp8 product, so the bytes are widened for torch's; a program with one passes q.y and q.scale to it.)"""
         add, h, _ = self.forward(ids)
         q = norms.rms_norm_fp8(add, self._gain(-1), EPS, residual=h)
         logits = (q.y.to(self.dtype) @ self._weight(self.head).t()) * q.scale.to(self.dtype)
