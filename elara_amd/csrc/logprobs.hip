@@ -11,9 +11,9 @@
 // fp32), so that e * (x - m) is 0 there too and not 0 * inf.  A row of nothing but -inf has s = 0: lse and logprob are
 // -inf, entropy 0, and no gradient.  A NaN (or +inf) anywhere gives NaN, as the formula does: the clamp keeps a NaN.
 //
-// The k likeliest (k <= 32) need no second pass over the row, but for a few of its places.  Among the maxima of 64 disjoint parts of it (the lanes', taken
-// anyway) the k-th largest is a lower bound of the row's k-th largest element; about 64 ln(64 / (64 - k)) elements of a
-// random row reach it.  A part that fits the block's registers is searched there.  A longer one keeps the maximum of each
+// The k likeliest (k <= 32) need no second pass over the row, but for a few of its places.  Among the maxima of 64 disjoint
+// parts of it (the lanes', taken anyway) the k-th largest is a lower bound of the row's k-th largest element; about
+// 64 ln(64 / (64 - k)) elements of a random row reach it.  A part that fits the block's registers is searched there.  A longer one keeps the maximum of each
 // thread's chunks in LDS, and only chunks whose maximum reaches the bound are read again, a vector per lane.  The elements
 // found are ranked.  Where the bound's own value is too frequent for its list (equal values, masked ones) its first places
 // are taken in index order; where too many elements lie above it (the large ones all with a few threads) four counting
@@ -26,8 +26,8 @@
 // as one fma, with another path for rows at a type's lowest value, gained nothing: 45.5 and 52.)  Many shorter rows pay more for
 // the k likeliest, which one wave or block of each row selects and ranks while its lanes are idle: 16,384 of 4,096 24 us without,
 // 41, 44 and 48 with k = 5, 20 and 32; 60,000 of 1,000 25, and 86 with 20; 200,000 of 100 19, and 158, 281 and 296.
-// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 338 us (6.3 TB/s), 301 of 50,021 fp32 21 us (5.6 TB/s); a wave a row at least:
-// 60,000 of 1,000 66 us (3.7 TB/s), 200,000 of 100 78 (1.1).
+// Backward: 4,096 of 131,072 (1 GB in, 1 GB out) 338 to 344 us (6.3 TB/s), 301 of 50,021 fp32 21 us (5.6 TB/s); a wave a row
+// at least: 60,000 of 1,000 66 us (3.7 TB/s), 200,000 of 100 78 (1.1).
 #include "elr_elem.h"
 
 namespace elr {

@@ -17,8 +17,9 @@
 // MB) take 84 us (6.4 TB/s); their backward 85 us and 5 for the sum of the weight gradients (6.0 TB/s); that of 425,984 rows
 // of 128 fp32 (656 MB) 109 and 5 (5.8 TB/s).  fp8 of 8,192 rows of 2,048 with groups of 128 (118 MB): 24 us (4.9 TB/s, of
 // which a launch is 3 us); of 16,384 rows of 4,096 with a scale a row (470 MB) 82 us (5.8 TB/s).  An fp32 residual stream
-// under bf16: 16,384 of 1,024 40 us forward (5.0 TB/s) and 51 backward (4.6), of 4,096 206 (3.9) and 243 (3.9).  2,048 rows of
-// 20,480, which are read more than once: 66 us (5.1 TB/s), backward 245 (1.4).
+// under bf16: 16,384 of 1,024 40 us forward (5.0 TB/s) and 51 backward (4.6), of 4,096 206 (3.9) and 243 (3.9).  bf16 rows of
+// 20,480 (2,048 of them) 66 us (5.1 TB/s), and 245 backward (1.4), which reads such rows twice; of 100,000 (1,024), read twice
+// either way, 256 (3.2) and 630 (1.3).
 #include "elr_elem.h"
 
 namespace elr {
