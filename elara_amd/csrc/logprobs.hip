@@ -704,7 +704,7 @@ constexpr int kBackVecs = 4;
 constexpr float kEmptyLse = -0x1.0p+100f;
 
 // From here on half an ulp of lse (2^-17 and more) is what p = e^(x - lse) would err by, and at a common offset of 10^9 lse has
-// no digit of log V left.  The maximum and the sum of such a wide row are taken again.
+// no digit of log V left.  The sum of such a wide row's e^(x - lse), which should be 1, is taken then.
 constexpr float kWideLse = 256.0f;
 
 // What a row's gradient needs; logp = (x - ref) - sub.
@@ -730,14 +730,12 @@ __device__ __forceinline__ RowGrad row_grad(const LpBackArgs& a, int64_t row) {
   r.wide = size >= kWideLse && size < __builtin_inff() && !r.empty;
   return r;
 }
-// A wide row's gradient by its own maximum m and sum s: p = e^((x - m) - log s), in which nothing cancels.  An lse that is not
-// m + log s to its last bits (it may be of more logits than these) is used as it is.
-__device__ __forceinline__ void use_own(RowGrad& r, float m, float s) {
-  const float logs = __builtin_logf(s), rest = (m - r.ref) + logs;
-  if (__builtin_fabsf(rest) <= __builtin_fabsf(r.ref) * 0x1.0p-22f) {
-    r.ref = m;
-    r.sub = logs;
-  }
+// A wide row's gradient by its own sum, s = sum e^(x - lse): p = e^((x - lse) - log s).  lse is no less than any x, and x - lse
+// has all the digits that x has.  An lse from which the row's own is further than its rounding (it may be of more logits than
+// these) is used as it is.
+__device__ __forceinline__ void use_sum(RowGrad& r, float s) {
+  const float rest = __builtin_logf(s);
+  if (__builtin_fabsf(rest) <= __builtin_fabsf(r.ref) * 0x1.0p-22f) r.sub = rest;
 }
 // The gradients of the vector at element e of the row.  SUB: r.sub may be other than 0.
 template <class E, bool SUB>
@@ -755,25 +753,13 @@ __device__ __forceinline__ u32x4 grad_vec(const RowGrad& r, u32x4 raw, int64_t e
   return narrow<E>(y);
 }
 
-// A wave's running maximum and sum, each lane's its own, with U more vectors.
-template <class E, int U>
-__device__ __forceinline__ void add_vecs(Sums& q, const u32x4 (&raw)[U]) {
-  constexpr int VE = Elem<E>::VE;
-  Frag<E> y[U];
-  float m = q.m;
+// s with e^(x - ref) of a vector's elements (those outside the row are -inf: nothing).
+template <class E>
+__device__ __forceinline__ float add_vec(float s, u32x4 raw, float ref) {
+  const Frag<E> y = widen<E>(raw);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    y[u] = widen<E>(raw[u]);
-#pragma unroll
-    for (int j = 0; j < VE; ++j) m = __builtin_fmaxf(m, y[u].v[j]);
-  }
-  const float ref = exp_ref(m);
-  q.s = q.s * exp_nat(clamp_low(q.m - ref));
-  q.m = m;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int j = 0; j < VE; ++j) q.s = q.s + exp_nat(clamp_low(y[u].v[j] - ref));
+  for (int j = 0; j < Elem<E>::VE; ++j) s = s + exp_nat(clamp_low(y.v[j] - ref));
+  return s;
 }
 
 // A wave's vectors of a row, from element e0 of lane 0 on; ALL: every one lies within the row.  False: a wide row of more than
@@ -792,10 +778,7 @@ __device__ __forceinline__ bool back_vecs(const LpBackArgs& a, int64_t row, cons
   RowGrad r = row_grad(a, row);
   if (r.wide) {
     if constexpr (U > 1) return false;
-    Sums q{-__builtin_inff(), 0.0f, 0.0f};      // (the row is this chunk)
-    add_vecs<E>(q, raw);
-    q = wave_join(q);
-    use_own(r, q.m, q.s);
+    use_sum(r, wave_sum(add_vec<E>(0.0f, raw[0], r.ref)));     // (the row is this chunk)
     store_part<E, true>(out, e0, a.V, grad_vec<E, true>(r, raw[0], e0));
     return true;
   }
@@ -809,28 +792,35 @@ __device__ __forceinline__ bool back_vecs(const LpBackArgs& a, int64_t row, cons
   return true;
 }
 
-// A whole wide row by one wave.  In place no other wave may write before the sum is taken, so the row's other waves leave it
-// alone.  4,096 rows of 131,072 bf16, all wide, take 1,133 us (338 where none is), one such row alone 130.
+// A whole wide row by one wave, or by the `waves` of a block of which all are the row's.  In place none may write before the sum
+// is taken, so the row's other waves leave it alone.  4,096 rows of 131,072 bf16, all wide, take 752 us (344 where none is), one
+// such row alone 36 (a wave a row: 1,133 and 130); 200,000 of 100, each in its wave's registers, 95 (78).
 template <class E>
-__device__ __forceinline__ void back_wide(const LpBackArgs& a, int64_t row, const E* x, E* out) {
+__device__ __forceinline__ void back_wide(const LpBackArgs& a, int64_t row, const E* x, E* out, int waves, float* sums) {
   constexpr int VE = Elem<E>::VE, U = 16 / VE;      // (more vectors a step would cost the other rows' waves registers)
   constexpr int64_t kStep = 64 * U * VE;
-  const int lane = threadIdx.x & 63;
-  const int64_t first = -(int64_t)line_shift<E>(out, 128);
+  const int lane = threadIdx.x & 63, w = waves > 1 ? (int)(threadIdx.x >> 6) : 0;
+  const int64_t first = w * kStep - line_shift<E>(out, 128);
   const auto load = [&](u32x4 (&raw)[U], int64_t e0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = load_part<E, false>(x, e0 + u * 64 * VE, a.V, -__builtin_inff());
   };
-  Sums q{-__builtin_inff(), 0.0f, 0.0f};
-  for (int64_t s0 = first; s0 < a.V; s0 += kStep) {
+  RowGrad r = row_grad(a, row);
+  float s = 0.0f;
+  for (int64_t s0 = first; s0 < a.V; s0 += waves * kStep) {
     u32x4 raw[U];
     load(raw, s0 + lane * VE);
-    add_vecs<E>(q, raw);
+#pragma unroll
+    for (int u = 0; u < U; ++u) s = add_vec<E>(s, raw[u], r.ref);
   }
-  q = wave_join(q);
-  RowGrad r = row_grad(a, row);
-  use_own(r, q.m, q.s);
-  for (int64_t s0 = first; s0 < a.V; s0 += kStep) {
+  s = wave_sum(s);
+  if (waves > 1) {
+    if (lane == 0) sums[w] = s;
+    __syncthreads();
+    s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+  use_sum(r, s);
+  for (int64_t s0 = first; s0 < a.V; s0 += waves * kStep) {
     u32x4 raw[U];
     load(raw, s0 + lane * VE);
 #pragma unroll
@@ -856,8 +846,16 @@ __global__ __launch_bounds__(256) void k_lp_back(LpBackArgs a, int64_t row0) {
   const int64_t s0 = (int64_t)chunk * kChunk - line_shift<E>(out, 128);
   const bool done = s0 >= 0 && s0 + kChunk <= a.V ? back_vecs<E, U, true>(a, row, x, out, s0)
                                                   : back_vecs<E, U, false>(a, row, x, out, s0);
-  if constexpr (U > 1) {          // (blocks of four waves: another of the chip's parts for each wide row)
-    if (!done && chunk == in * 4u % (uint32_t)a.chunks) back_wide<E>(a, row, x, out);
+  if constexpr (U > 1) {
+    // (another chunk for each row: with the first one always, all of them fell to one of the chip's eight parts)
+    __shared__ float sums[4];
+    const uint32_t chunks = (uint32_t)a.chunks;
+    if (done) return;
+    if (chunks % 4 == 0) {                           // every block is one row's: all four waves come here
+      if (chunk / 4 == in % (chunks / 4)) back_wide<E>(a, row, x, out, 4, sums);
+    } else if (chunk == in * 4u % chunks) {
+      back_wide<E>(a, row, x, out, 1, sums);
+    }
   }
 }
 
@@ -928,6 +926,7 @@ static void launch_back(const LpBackArgs& a0, hipStream_t st) {
   const bool one = most <= 64 * VE;
   const int64_t per = 64 * VE * (one ? 1 : kBackVecs);
   a.chunks = (int32_t)((most + per - 1) / per);
+  if (a.chunks > 16) a.chunks = (a.chunks + 3) / 4 * 4;     // whole blocks, which can share a wide row
   const int64_t rows = (int64_t)1 << 25;          // waves of a launch (a grid has less than 2^32 threads)
   const int64_t step = rows / a.chunks < 1 ? 1 : rows / a.chunks;
   for (int64_t r = 0; r < a.n; r += step) {

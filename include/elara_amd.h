@@ -753,8 +753,8 @@ int elr_token_logprobs(const void* logits, int type, int64_t n, int64_t V, int64
 /* Its gradient to the logits: d_logits[v] = [v = token] g + p_v (z - g - h (log p_v + entropy)), with g, h, z the
  * gradients of logprob, entropy and lse (each fp32 [n] or NULL: zero), lse and entropy from the forward (entropy may be
  * NULL without d_entropy).  A row without a token has g = 0, a row with lse below -2^100 (nothing
- * but -inf, or nothing but fp32's or bf16's lowest value) no gradient.  Where |lse| is 256 or more, p is taken from the
- * row's own maximum and sum (if lse is theirs), of which lse holds too few digits.  d_logits has
+ * but -inf, or nothing but fp32's or bf16's lowest value) no gradient.  Where |lse| is 256 or more, of which fp32 then
+ * holds too few digits, p is divided by the row's sum of e^(x - lse) (if lse is the row's own).  d_logits has
  * `type` and the row stride out_ld >= V; it may be the logits themselves (same stride). */
 int elr_token_logprobs_backward(const void* logits, int type, int64_t n, int64_t V, int64_t ld, const void* tokens,
                                 int idx64, const float* lse, const float* entropy, const float* d_logprob,
