@@ -106,6 +106,18 @@ SIGNATURES = {
     'elr_rms_norm_backward_scratch_bytes': (c_i64, [c_i64, c_i64, ctypes.c_int]),
     'elr_rms_norm_backward': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, ctypes.c_int, c_i64, c_vp,
                                              c_i64, c_vp, ctypes.c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'elr_quantize_int8': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_vp, c_vp, c_vp]),
+    'elr_dequantize_int8': (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, ctypes.c_int, c_vp]),
+    'elr_int8_linear_scratch_bytes': (c_i64, [c_i64, c_i64, c_i64]),
+    'elr_int8_linear': (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, ctypes.c_int, c_vp,
+                                       c_i64, c_vp]),
+    'elr_int8_weight_grad_scratch_bytes': (c_i64, [c_i64, c_i64, c_i64, ctypes.c_int]),
+    'elr_int8_weight_grad': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp,
+                                            ctypes.c_int, c_vp, c_i64, c_vp]),
+    'elr_rms_norm_backward_int8': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp,
+                                                  ctypes.c_int, c_i64, c_vp, ctypes.c_int] + [c_vp] * 4 + [c_i64, c_vp]),
+    'elr_sample_tokens': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, c_f64, c_vp, c_i64, c_vp, ctypes.c_int,
+                                         c_f64, c_vp, c_f64, c_vp, c_vp, c_vp, c_vp]),
     'elr_grad_norm_scratch_bytes': (c_i64, [c_vp, c_i64]),
     'elr_grad_norm': (ctypes.c_int, [c_vp, c_i64, ctypes.c_int, c_vp, c_vp, c_i64, c_vp]),
     'elr_clip_grad_norm': (ctypes.c_int, [c_vp, c_i64, ctypes.c_int, c_f32, c_f32, c_vp, c_vp, c_i64, c_vp]),
@@ -254,6 +266,7 @@ NOT_TAKEN = -1000   # _hostcall's answer for arguments the Python path has to lo
 class _NoHost:
     """Stands in for _hostcall where it is not built for this interpreter's torch: the Python path takes every call."""
     adam = init = replay = logprobs = logprobs_back = norm = norm_back = clip = staticmethod(lambda *a: NOT_TAKEN)
+    quantize = dequantize = linear = weight_grad = norm_back_int8 = sample = adam
 
 
 _host = None
@@ -276,6 +289,9 @@ def host():
                 'token_logprobs_scratch_bytes', 'token_logprobs', 'token_logprobs_backward', 'rms_norm',
                 'rms_norm_backward_scratch_bytes', 'rms_norm_backward', 'grad_norm_scratch_bytes', 'grad_norm',
                 'clip_grad_norm')))
+            h.bind_int8(*(ctypes.cast(getattr(L, 'elr_' + f), c_vp).value for f in (
+                'quantize_int8', 'dequantize_int8', 'int8_linear_scratch_bytes', 'int8_linear', 'int8_weight_grad_scratch_bytes',
+                'int8_weight_grad', 'rms_norm_backward_int8', 'sample_tokens')))
         except ImportError as e:
             warnings.warn(f'elara_amd._hostcall is not used (small row-op calls take several microseconds longer): {e}',
                           stacklevel=3)

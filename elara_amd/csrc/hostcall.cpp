@@ -1,5 +1,5 @@
 // Host side of the row ops' Python entry points: the argument checks and the C-ABI call of ops.gpu_adam,
-// gpu_ops.init_rows and gpu_ops.replay_rows in one native call, and of the operators in logprobs, norms and gradnorm, for
+// gpu_ops.init_rows and gpu_ops.replay_rows in one native call, and of the operators in logprobs, norms, gradnorm, int8 and sampling, for
 // the arguments a training loop passes (plain contiguous GPU tensors of the expected types on the current device).
 // Everything else -- other types, strides or devices, arenas in host memory, wrapped tensors, errors -- is answered with NOT_TAKEN, and the Python path then
 // converts, raises or runs as it always has, so the two accept and refuse the same calls.
@@ -535,6 +535,263 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
   }
 }
 
+// ---- int8, sampling
+
+decltype(&elr_quantize_int8) f_quantize = nullptr;
+decltype(&elr_dequantize_int8) f_dequantize = nullptr;
+decltype(&elr_int8_linear_scratch_bytes) f_linear_bytes = nullptr;
+decltype(&elr_int8_linear) f_linear = nullptr;
+decltype(&elr_int8_weight_grad_scratch_bytes) f_wgrad_bytes = nullptr;
+decltype(&elr_int8_weight_grad) f_wgrad = nullptr;
+decltype(&elr_rms_norm_backward_int8) f_norm_back8 = nullptr;
+decltype(&elr_sample_tokens) f_sample = nullptr;
+
+PyObject* bind_int8(PyObject*, PyObject* args) {
+  unsigned long long a[8];
+  if (!PyArg_ParseTuple(args, "KKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7)) return nullptr;
+  set_address(f_quantize, a[0]), set_address(f_dequantize, a[1]);
+  set_address(f_linear_bytes, a[2]), set_address(f_linear, a[3]);
+  set_address(f_wgrad_bytes, a[4]), set_address(f_wgrad, a[5]);
+  set_address(f_norm_back8, a[6]), set_address(f_sample, a[7]);
+  Py_RETURN_NONE;
+}
+
+bool group_ok(int64_t g) { return g == 0 || g == 32 || g == 64 || g == 128 || g == 256; }
+int64_t groups_of(int64_t D, int64_t g) { return g ? (D + g - 1) / g : 1; }
+
+// The three parts of an Int8Rows (q, scale, group), with a scale for each of a row's groups.
+struct Rows8 {
+  const at::Tensor *q = nullptr, *scale = nullptr;
+  int64_t group = 0, n = 0, D = 0;
+  bool take(PyObject* qo, PyObject* so, PyObject* go) {
+    if (!(q = plain(qo)) || !(scale = plain(so)) || !integer(go, group) || !group_ok(group) || q->scalar_type() != at::kChar ||
+        q->dim() < 1 || q->numel() == 0 || scale->scalar_type() != at::kFloat || scale->device() != q->device() ||
+        scale->dim() != q->dim())
+      return false;
+    const int64_t d = q->dim() - 1;
+    D = q->size(d), n = q->numel() / D;
+    return scale->size(d) == groups_of(D, group) && scale->sizes().slice(0, d) == q->sizes().slice(0, d);
+  }
+  const int8_t* data() const { return static_cast<const int8_t*>(q->data_ptr()); }
+};
+
+at::ScalarType scalar_type_of(int64_t elem) {
+  return elem == ELR_F32 ? at::kFloat : elem == ELR_F16 ? at::kHalf : at::kBFloat16;
+}
+
+// quantize(x, group, pow2) -> (return code, q, scale), or NOT_TAKEN
+PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 3 || !f_quantize) return not_taken();
+  const at::Tensor* x = plain(a[0]);
+  int64_t group, pow2;
+  if (!x || !integer(a[1], group) || !integer(a[2], pow2) || x->dim() < 1 || x->numel() == 0 || !group_ok(group))
+    return not_taken();
+  const int type = elem_type(*x);
+  const int64_t D = x->size(-1), n = x->numel() / D;
+  if (type < 0) return not_taken();
+  try {
+    at::Tensor q, scale;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x, st)) {
+        std::vector<int64_t> shape(x->sizes().begin(), x->sizes().end());
+        q = empty_on(*x, shape, at::kChar);
+        shape.back() = groups_of(D, group);
+        scale = empty_on(*x, shape, at::kFloat);
+        rc = f_quantize(x->data_ptr(), type, n, D, D, group, pow2 != 0, static_cast<int8_t*>(q.data_ptr()),
+                        static_cast<float*>(scale.data_ptr()), st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(q), THPVariable_Wrap(scale));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// dequantize(q, scale, group, type) -> (return code, x), or NOT_TAKEN
+PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 4 || !f_dequantize) return not_taken();
+  Rows8 r;
+  int64_t type;
+  if (!r.take(a[0], a[1], a[2]) || !integer(a[3], type) || type < 0) return not_taken();
+  try {
+    at::Tensor x;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*r.q, st)) {
+        x = empty_on(*r.q, r.q->sizes(), scalar_type_of(type));
+        rc = f_dequantize(r.data(), r.n, r.D, r.D, r.group, floats(r.scale), x.data_ptr(), static_cast<int>(type), st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(x));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// linear(x.q, x.scale, x.group, w.q, w.scale, w.group, type) -> (return code, y), or NOT_TAKEN
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 7 || !f_linear) return not_taken();
+  Rows8 x, w;
+  int64_t type;
+  if (!x.take(a[0], a[1], a[2]) || !w.take(a[3], a[4], a[5]) || !integer(a[6], type) || type < 0 || x.group || w.group ||
+      w.q->dim() != 2 || w.D != x.D || w.q->device() != x.q->device() || x.D >= int64_t(1) << 17)
+    return not_taken();
+  try {
+    at::Tensor y;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x.q, st)) {
+        std::vector<int64_t> shape(x.q->sizes().begin(), x.q->sizes().end());
+        shape.back() = w.n;
+        y = empty_on(*x.q, shape, scalar_type_of(type));
+        const int64_t bytes = f_linear_bytes(x.n, w.n, x.D);
+        const at::Tensor scratch = scratch_on(*x.q, bytes);
+        rc = f_linear(x.data(), x.n, x.D, x.D, floats(x.scale), w.data(), w.n, w.D, floats(w.scale), y.data_ptr(),
+                      static_cast<int>(type), data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(y));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// weight_grad(dy, x.q, x.scale, x.group, transposed) -> (return code, dw), or NOT_TAKEN
+PyObject* weight_grad(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 5 || !f_wgrad) return not_taken();
+  const at::Tensor* dy = plain(a[0]);
+  Rows8 x;
+  int64_t transposed;
+  if (!dy || !x.take(a[1], a[2], a[3]) || !integer(a[4], transposed) || dy->dim() != x.q->dim() || dy->numel() == 0 ||
+      dy->device() != x.q->device())
+    return not_taken();
+  const int64_t d = dy->dim() - 1, N = dy->size(d);
+  const int type = elem_type(*dy);
+  if (type < 0 || dy->sizes().slice(0, d) != x.q->sizes().slice(0, d)) return not_taken();
+  try {
+    at::Tensor dw;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*dy, st)) {
+        dw = empty_on(*dy, transposed ? at::IntArrayRef{x.D, N} : at::IntArrayRef{N, x.D}, at::kFloat);
+        const int64_t bytes = f_wgrad_bytes(x.n, N, x.D, type);
+        const at::Tensor scratch = scratch_on(*dy, bytes);
+        rc = f_wgrad(dy->data_ptr(), type, x.n, N, N, x.data(), x.D, x.D, x.group, floats(x.scale),
+                     static_cast<float*>(dw.data_ptr()), transposed != 0, data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(dw));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// norm_back_int8(dy, h.q, h.scale, h.group, weight, rstd, dh, need_dweight) -> (return code, dx, dweight), or NOT_TAKEN
+PyObject* norm_back_int8(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 8 || !f_norm_back8) return not_taken();
+  const at::Tensor *dy = plain(a[0]), *w, *rstd = plain(a[5]), *dh;
+  Rows8 h;
+  int64_t need;
+  if (!dy || !h.take(a[1], a[2], a[3]) || !maybe(a[4], w) || !rstd || !maybe(a[6], dh) || !integer(a[7], need) ||
+      dy->sizes() != h.q->sizes() || dy->device() != h.q->device())
+    return not_taken();
+  const int type = elem_type(*dy);
+  int wt, xt = type;
+  if (type < 0 || !weight_ok(w, *dy, h.D, wt) || rstd->scalar_type() != at::kFloat || rstd->device() != dy->device() ||
+      rstd->sizes() != dy->sizes().slice(0, dy->dim() - 1))
+    return not_taken();
+  if (dh) {
+    xt = elem_type(*dh);
+    if (dh->sizes() != dy->sizes() || dh->device() != dy->device() || (xt != type && xt != ELR_F32)) return not_taken();
+  }
+  try {
+    at::Tensor dx, dw;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*dy, st)) {
+        dx = empty_on(*dy, dy->sizes(), scalar_type_of(xt));
+        at::Tensor scratch;
+        int64_t bytes = 0;
+        if (need) {
+          dw = empty_on(*dy, {h.D}, at::kFloat);
+          bytes = f_norm_bytes(h.n, h.D, type);
+          scratch = scratch_on(*dy, bytes);
+        }
+        rc = f_norm_back8(dy->data_ptr(), type, h.n, h.D, h.D, h.data(), h.D, h.group, floats(h.scale),
+                          dh ? dh->data_ptr() : nullptr, xt, h.D, w ? w->data_ptr() : nullptr, wt, floats(rstd), dx.data_ptr(),
+                          static_cast<float*>(data_or_null(dw)), data_or_null(scratch), bytes, st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(dx), wrap_or_none(dw));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
+// A setting: a number in [low, high], or a plain fp32 tensor of u's shape and device.
+bool setting(PyObject* o, const at::Tensor& u, double low, double high, double& v, const at::Tensor*& rows) {
+  v = 0, rows = nullptr;
+  if (PyFloat_CheckExact(o) || PyLong_CheckExact(o)) return real(o, v) && v >= low && v <= high;
+  rows = plain(o);
+  return rows && rows->scalar_type() == at::kFloat && rows->device() == u.device() && rows->sizes() == u.sizes();
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p) -> (return code, token, logprob), or NOT_TAKEN
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 6 || !f_sample) return not_taken();
+  const at::Tensor *x = plain(a[0]), *u = plain(a[1]), *temps, *ks = nullptr, *ps, *mps;
+  if (!x || !u || x->dim() < 1 || x->numel() == 0 || u->scalar_type() != at::kFloat || u->device() != x->device() ||
+      u->sizes() != x->sizes().slice(0, x->dim() - 1))
+    return not_taken();
+  double temp, p, mp;
+  int64_t k = 0;
+  const int type = elem_type(*x);
+  if (type < 0 || !setting(a[2], *u, 0, 1.7e308, temp, temps) || !setting(a[4], *u, 0, 1, p, ps) ||
+      !setting(a[5], *u, 0, 1, mp, mps))
+    return not_taken();
+  if (PyLong_CheckExact(a[3])) {
+    if (!integer(a[3], k) || k < 0) return not_taken();
+  } else if (!(ks = plain(a[3])) || (ks->scalar_type() != at::kInt && ks->scalar_type() != at::kLong) ||
+             ks->device() != x->device() || ks->sizes() != u->sizes()) {
+    return not_taken();
+  }
+  try {
+    at::Tensor token, logprob;
+    int rc = kNotTaken;
+    {
+      NoGil g;
+      void* st;
+      if (stream_on(*x, st)) {
+        token = empty_on(*x, u->sizes(), at::kLong), logprob = empty_on(*x, u->sizes(), at::kFloat);
+        const int64_t V = x->size(-1);
+        rc = f_sample(x->data_ptr(), type, x->numel() / V, V, V, floats(u), temp, floats(temps), k, ks ? ks->data_ptr() : nullptr,
+                      ks && ks->scalar_type() == at::kLong, p, floats(ps), mp, floats(mps),
+                      static_cast<int64_t*>(token.data_ptr()), static_cast<float*>(logprob.data_ptr()), st);
+      }
+    }
+    if (rc == kNotTaken) return not_taken();
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(token), THPVariable_Wrap(logprob));
+  } catch (const std::exception&) {
+    return not_taken();
+  }
+}
+
 #define ELR_STR1(x) #x
 #define ELR_STR(x) ELR_STR1(x)
 #define ELR_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -548,6 +805,13 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "Addresses of the library'
                          {"norm", ELR_FAST(norm), METH_FASTCALL, "elr_rms_norm into new tensors."},
                          {"norm_back", ELR_FAST(norm_back), METH_FASTCALL, "elr_rms_norm_backward into new tensors."},
                          {"clip", ELR_FAST(clip), METH_FASTCALL, "elr_clip_grad_norm or elr_grad_norm."},
+                         {"bind_int8", bind_int8, METH_VARARGS, "Addresses of the entry points of int8 and sampling."},
+                         {"quantize", ELR_FAST(quantize), METH_FASTCALL, "elr_quantize_int8 into new tensors."},
+                         {"dequantize", ELR_FAST(dequantize), METH_FASTCALL, "elr_dequantize_int8 into a new tensor."},
+                         {"linear", ELR_FAST(linear), METH_FASTCALL, "elr_int8_linear into a new tensor."},
+                         {"weight_grad", ELR_FAST(weight_grad), METH_FASTCALL, "elr_int8_weight_grad into a new tensor."},
+                         {"norm_back_int8", ELR_FAST(norm_back_int8), METH_FASTCALL, "elr_rms_norm_backward_int8."},
+                         {"sample", ELR_FAST(sample), METH_FASTCALL, "elr_sample_tokens into new tensors."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,136 @@
+// The product of rows in 8-bit integers with a weight in 8-bit integers:  y[i, j] = sx_i sw_j sum_k x[i, k] w[j, k], a scale for each
+// row of x (token) and of w (output channel).  No counterpart in the reference.
+//
+// The sum is exact: int32 holds K products of at most 2^14 each for K < 2^17, which the entry point asks for.  It is widened to fp32
+// (one rounding), multiplied by sx_i and by sw_j and rounded to the output's type.
+#include "elr_int8.h"
+
+namespace elr {
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+typedef u32x4 u32x4_b __attribute__((aligned(1)));
+
+struct LinearArgs {
+  const int8_t *x, *w;
+  int64_t x_ld, w_ld;
+  const float *x_scale, *w_scale;
+  int64_t n, N;
+  int32_t K;
+  void* y;
+};
+
+// 16 bytes of a row at k, of which those up to K may be read; the rest are 0.
+__device__ __forceinline__ u32x4 load_k(const int8_t* row, int32_t k, int32_t K) {
+  if (k + 16 <= K) return *reinterpret_cast<const u32x4_b*>(row + k);
+  u32x4 r{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (k + j < K) r[j / 4] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j & 3));
+  return r;
+}
+
+template <class O>
+__device__ __forceinline__ O scaled(int32_t acc, float sx, float sw) {
+  return (O)((float)acc * sx * sw);
+}
+
+// Tiles of BM tokens x BN channels, 64 bytes of K at a time through LDS; four waves, each a quarter of the tile in matrix instructions of
+// 32 x 32 x 32.  Rows of any alignment.
+template <class O, int BM, int BN>
+__global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
+  constexpr int PITCH = 80, MT = BM / 64, NT = BN / 64;
+  __shared__ __attribute__((aligned(16))) uint8_t lx[BM * PITCH], lw[BN * PITCH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m0 = (int64_t)blockIdx.y * BM, n0 = (int64_t)blockIdx.x * BN;
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+  i32x16 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = i32x16{};
+  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+  for (int32_t k = 0; k < a.K; k += 64) {
+    u32x4 gx[MT], gw[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t row = m0 + r + i * 64;
+      gx[i] = row < a.n ? load_k(a.x + row * a.x_ld, k + c, a.K) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t row = n0 + r + j * 64;
+      gw[j] = row < a.N ? load_k(a.w + row * a.w_ld, k + c, a.K) : u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *reinterpret_cast<u32x4*>(lx + (r + i * 64) * PITCH + c) = gx[i];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *reinterpret_cast<u32x4*>(lw + (r + j * 64) * PITCH + c) = gw[j];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      i32x4 fx[MT], fw[NT];
+      const int at = (lane & 31) * PITCH + q * 32 + (lane >> 5) * 16;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4*>(lx + (wm + i * 32) * PITCH + at);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fw[j] = *reinterpret_cast<const i32x4*>(lw + (wn + j * 32) * PITCH + at);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t col = n0 + wn + j * 32 + (lane & 31);
+    const float sw = col < a.N ? a.w_scale[col] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int64_t row = m0 + wm + i * 32 + (q >> 2) * 8 + (lane >> 5) * 4 + (q & 3);
+        if (row < a.n && col < a.N) ((O*)a.y)[row * a.N + col] = scaled<O>(acc[i][j][q], a.x_scale[row], sw);
+      }
+  }
+}
+
+// ---- host side
+
+template <class O>
+static void linear(const LinearArgs& b, hipStream_t st) {
+  constexpr int64_t kRows = 65535 * (int64_t)128;      // gridDim.y
+  for (int64_t r = 0; r < b.n; r += kRows) {
+    LinearArgs a = b;
+    a.n = b.n - r < kRows ? b.n - r : kRows;
+    a.x = b.x + r * b.x_ld, a.x_scale = b.x_scale + r, a.y = (O*)b.y + r * b.N;
+    if (a.n <= 64) k_linear<O, 64, 128><<<dim3((unsigned)((a.N + 127) / 128), 1), 256, 0, st>>>(a);
+    else k_linear<O, 128, 128><<<dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.n + 127) / 128)), 256, 0, st>>>(a);
+  }
+}
+
+}  // namespace elr
+
+extern "C" int64_t elr_int8_linear_scratch_bytes(int64_t n, int64_t N, int64_t K) {
+  if (n < 0 || N < 0 || K < 0) return -1;
+  return 0;
+}
+
+extern "C" int elr_int8_linear(const int8_t* x, int64_t n, int64_t K, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t N,
+                               int64_t w_ld, const float* w_scale, void* y, int type, void* scratch, int64_t scratch_bytes,
+                               void* stream) {
+  using namespace elr;
+  if (n < 0 || N < 0 || K < 0 || x_ld < 0 || w_ld < 0 || !elem_type_ok(type)) return ELR_EINVAL;
+  if (K >= 1 << 17 || N > (int64_t)1 << 31) return ELR_EUNSUPPORTED;
+  if (n == 0 || N == 0) return ELR_OK;
+  if (!x_scale || !w_scale || !y || (K > 0 && (!x || !w)) || !elem_aligned(y, type) ||
+      (((uintptr_t)x_scale | (uintptr_t)w_scale) & 3u))
+    return ELR_EINVAL;
+  const LinearArgs a{x, w, x_ld, w_ld, x_scale, w_scale, n, N, (int32_t)K, y};
+  hipStream_t st = (hipStream_t)stream;
+  if (type == ELR_F32) linear<float>(a, st);
+  else if (type == ELR_F16) linear<_Float16>(a, st);
+  else linear<__bf16>(a, st);
+  return launch_status();
+}

@@ -20,7 +20,9 @@
 // under bf16: 16,384 of 1,024 40 us forward (5.0 TB/s) and 51 backward (4.6), of 4,096 206 (3.9) and 243 (3.9).  bf16 rows of
 // 20,480 (2,048 of them) 66 us (5.1 TB/s), and 245 backward (1.4), which reads such rows twice; of 100,000 (1,024), read twice
 // either way, 256 (3.2) and 630 (1.3).
-#include "elr_elem.h"
+#include "elr_int8.h"
+
+#include <type_traits>
 
 namespace elr {
 
@@ -371,12 +373,41 @@ struct NormBackArgs {
   void* dx;                       // h's type, contiguous
   float* part;                    // [gridDim.x][D] weight gradient of each block's rows, or NULL
   int nt;
+  const float* h_scale;           // int8 h: fp32 [n, groups], a scale for each 2^shift columns
+  int32_t groups, shift;
 };
 
-// E: dy's and the weight's type; R: h's, dh's and dx's.  Each team walks U rows at a time, `teams` apart.  (With the next rows'
+// A vector of h: of the residual's type, or int8 with its scale (a vector lies within one group).
+template <class E, class R, class H>
+struct HRaw {
+  ResRaw<E, R> v;
+};
+template <class E, class R>
+struct HRaw<E, R, int8_t> {
+  Int8Raw<E> q;
+  float s;
+};
+template <class E, class R, class H>
+__device__ __forceinline__ HRaw<E, R, H> h_load(const NormBackArgs& a, int64_t row, int64_t e, int64_t valid) {
+  HRaw<E, R, H> r;
+  if constexpr (sizeof(H) == 1) {
+    r.q = int8_load<E>((const int8_t*)a.h + row * a.h_ld + e, valid);
+    r.s = valid > 0 ? a.h_scale[row * a.groups + (e >> a.shift)] : 0.0f;
+  } else {
+    r.v = res_load<E, R>((const R*)a.h + row * a.h_ld + e, valid);
+  }
+  return r;
+}
+template <class E, class R, class H>
+__device__ __forceinline__ Frag<E> h_widen(const HRaw<E, R, H>& r) {
+  if constexpr (sizeof(H) == 1) return int8_widen<E>(r.q, r.s);
+  else return res_widen<E, R>(r.v);
+}
+
+// E: dy's and the weight's type; R: dh's and dx's; H: h's, R or int8_t.  Each team walks U rows at a time, `teams` apart.  (With the next rows'
 // loads in flight: 425,984 rows of 128 fp32 114 us either way, 16,384 of 4,096 bf16 95 us against 89.)  Its weight gradient
 // stays in registers until the end, then the block's teams are added in a fixed order.
-template <class E, class R, int T, int NV, int U>
+template <class E, class R, class H, int T, int NV, int U>
 __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a, int lg) {
   constexpr int VE = Elem<E>::VE;
   extern __shared__ float dwsum[];     // [D], only with a.part
@@ -399,7 +430,8 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
   }
   struct Rows {
     u32x4 dy[U][NV];
-    ResRaw<E, R> h[U][NV], dh[U][NV];
+    HRaw<E, R, H> h[U][NV];
+    ResRaw<E, R> dh[U][NV];
     float c[U];
   };
   const auto load = [&](Rows& x, int64_t b) {
@@ -413,7 +445,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
         const int e = (i * team + l) * VE;
         const int valid = live ? a.D - e : 0;
         x.dy[q][i] = load_raw<E, true>((const E*)a.dy + at * a.dy_ld + e, valid, 0.0f);
-        x.h[q][i] = res_load<E, R>((const R*)a.h + at * a.h_ld + e, valid);
+        x.h[q][i] = h_load<E, R, H>(a, at, e, valid);
         if (a.dh) x.dh[q][i] = res_load<E, R>((const R*)a.dh + at * a.dh_ld + e, valid);
       }
       x.c[q] = live ? a.rstd[at] : 0.0f;
@@ -430,7 +462,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         u[i] = widen<E>(x.dy[q][i]);
-        xh[i] = res_widen<E, R>(x.h[q][i]);
+        xh[i] = h_widen<E, R, H>(x.h[q][i]);
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           xh[i].v[j] = xh[i].v[j] * x.c[q];
@@ -497,7 +529,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void k_norm_back(NormBackArgs a,
 
 // Long rows: one block a row at a time, dx in a second pass; the weight gradient of a block's rows is accumulated in its
 // own row of `part` (each element by one thread).
-template <class E, class R>
+template <class E, class R, class H>
 __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
   constexpr int VE = Elem<E>::VE, T = 256;
   __shared__ float lds[2][T > 64 ? T / 64 : 1];
@@ -507,13 +539,12 @@ __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const E* dy = (const E*)a.dy + row * a.dy_ld;
-    const R* h = (const R*)a.h + row * a.h_ld;
     const R* dh = (const R*)a.dh + row * a.dh_ld;
     const float c = a.rstd[row];
     float dot = 0.0f;
     for (int64_t e = threadIdx.x * VE; e < a.D; e += T * VE) {
       const Frag<E> y = widen<E>(load_raw<E, false>(dy + e, a.D - e, 0.0f));
-      const Frag<E> q = res_widen<E, R>(res_load<E, R>(h + e, a.D - e));
+      const Frag<E> q = h_widen<E, R, H>(h_load<E, R, H>(a, row, e, a.D - e));
       const Frag<E> w = weight_at<E>(a.w, a.w_f32, e, a.D - e);
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
@@ -527,7 +558,7 @@ __global__ __launch_bounds__(256) void k_norm_back_long(NormBackArgs a) {
     turn ^= 1;
     for (int64_t e = threadIdx.x * VE; e < a.D; e += T * VE) {
       const Frag<E> y = widen<E>(load_raw<E, false>(dy + e, a.D - e, 0.0f));
-      const Frag<E> q = res_widen<E, R>(res_load<E, R>(h + e, a.D - e));
+      const Frag<E> q = h_widen<E, R, H>(h_load<E, R, H>(a, row, e, a.D - e));
       const Frag<E> w = weight_at<E>(a.w, a.w_f32, e, a.D - e);
       Frag<E> f;
 #pragma unroll
@@ -641,24 +672,57 @@ static int64_t back_blocks(int64_t n, int64_t D, int type) {
   return b < most ? b : most;
 }
 
-template <class E, class R>
+template <class E, class R, class H>
 static void launch_norm_back(const NormBackArgs& a, unsigned blocks, hipStream_t st) {
   const Team t = team_of((a.D + Elem<E>::VE - 1) / Elem<E>::VE, 2);
   const size_t lds = a.part ? (size_t)a.D * 4 : 0;
   switch (t.T * 8 + t.NV) {
-    case 64 * 8 + 1: k_norm_back<E, R, 64, 1, 1><<<blocks, 256, lds, st>>>(a, t.lg); break;
-    case 64 * 8 + 2: k_norm_back<E, R, 64, 2, 2><<<blocks, 256, lds, st>>>(a, 6); break;
-    case 256 * 8 + 1: k_norm_back<E, R, 256, 1, 2><<<blocks, 256, 0, st>>>(a, 6); break;
-    case 512 * 8 + 1: k_norm_back<E, R, 512, 1, 1><<<blocks, 512, 0, st>>>(a, 6); break;
-    case 1024 * 8 + 1: k_norm_back<E, R, 1024, 1, 1><<<blocks, 1024, 0, st>>>(a, 6); break;
+    case 64 * 8 + 1: k_norm_back<E, R, H, 64, 1, 1><<<blocks, 256, lds, st>>>(a, t.lg); break;
+    case 64 * 8 + 2: k_norm_back<E, R, H, 64, 2, 2><<<blocks, 256, lds, st>>>(a, 6); break;
+    case 256 * 8 + 1: k_norm_back<E, R, H, 256, 1, 2><<<blocks, 256, 0, st>>>(a, 6); break;
+    case 512 * 8 + 1: k_norm_back<E, R, H, 512, 1, 1><<<blocks, 512, 0, st>>>(a, 6); break;
+    case 1024 * 8 + 1: k_norm_back<E, R, H, 1024, 1, 1><<<blocks, 1024, 0, st>>>(a, 6); break;
     case 1024 * 8 + 2:
       if constexpr (sizeof(E) == sizeof(R)) {
-        k_norm_back<E, R, 1024, 2, 1><<<blocks, 1024, 0, st>>>(a, 6);
+        k_norm_back<E, R, H, 1024, 2, 1><<<blocks, 1024, 0, st>>>(a, 6);
         break;
       }
       [[fallthrough]];   // (its registers would spill)
-    default: k_norm_back_long<E, R><<<blocks, 256, 0, st>>>(a); break;
+    default: k_norm_back_long<E, R, H><<<blocks, 256, 0, st>>>(a); break;
   }
+}
+
+// The backward behind both entry points, for checked rows: Q8 for h in int8, else of dx's type.
+template <bool Q8>
+static int norm_back(NormBackArgs a, int type, int x_type, float* dweight, void* scratch, int64_t scratch_bytes,
+                     hipStream_t st) {
+  const int64_t n = a.n, D = a.D;
+  if (n == 0 && !dweight) return ELR_OK;
+  const int64_t blocks = back_blocks(n, D, type);
+  if (dweight && n > 0 && (!scratch || scratch_bytes < blocks * D * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
+  a.part = !dweight ? nullptr : blocks == 1 ? dweight : (float*)scratch;
+  a.nt = n * D * elem_size(x_type) > kKeepBytes;
+  if (n > 0) {
+    const auto go = [&](auto e, auto r) {
+      typedef decltype(e) E;
+      typedef decltype(r) R;
+      launch_norm_back<E, R, typename std::conditional<Q8, int8_t, R>::type>(a, (unsigned)blocks, st);
+    };
+    const bool wide = x_type == ELR_F32;
+    switch (type) {
+      case ELR_F32: go(float(), float()); break;
+      case ELR_F16: wide ? go(_Float16(), float()) : go(_Float16(), _Float16()); break;
+      default: wide ? go(__bf16(), float()) : go(__bf16(), __bf16()); break;
+    }
+  }
+  if (dweight && (n == 0 || blocks > 1)) {   // no rows: zeros
+    for (int64_t e = 0; e < D; e += kDwColumns) {
+      const int64_t m = D - e < kDwColumns ? D - e : kDwColumns;
+      k_norm_dw<<<(unsigned)((m + 31) / 32), 1024, 0, st>>>(n > 0 ? (const float*)scratch + e : nullptr,
+                                                           n > 0 ? (int)blocks : 0, (int32_t)D, (int32_t)m, dweight + e);
+    }
+  }
+  return launch_status();
 }
 
 static int check_norm(int64_t n, int64_t D, int type, int res_type, int w_type) {
@@ -709,38 +773,32 @@ extern "C" int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_
   using namespace elr;
   if (int rc = check_norm(n, D, type, h_type, w_type)) return rc;
   if (dy_ld < 0 || h_ld < 0 || dh_ld < 0) return ELR_EINVAL;
-  hipStream_t st = (hipStream_t)stream;
   if (n > 0) {
     if (!dy || !h || !rstd || !dx) return ELR_EINVAL;
     if (!elem_aligned(dy, type) || !elem_aligned(h, h_type) || !elem_aligned(dh, h_type) || !elem_aligned(dx, h_type) ||
         !elem_aligned(weight, w_type))
       return ELR_EINVAL;
   }
-  if (n == 0 && !dweight) return ELR_OK;
-  const int64_t blocks = back_blocks(n, D, type);
-  if (dweight && n > 0 && (!scratch || scratch_bytes < blocks * D * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const NormBackArgs a{dy, h, dh, weight, dy_ld, h_ld, dh_ld, rstd, n, (int32_t)D, w_type == ELR_F32, dx,
-                       !dweight ? nullptr : blocks == 1 ? dweight : (float*)scratch, n * D * elem_size(h_type) > kKeepBytes};
+                       nullptr, 0, nullptr, 1, 31};
+  return norm_back<false>(a, type, h_type, dweight, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+extern "C" int elr_rms_norm_backward_int8(const void* dy, int type, int64_t n, int64_t D, int64_t dy_ld, const int8_t* h,
+                                          int64_t h_ld, int64_t group, const float* h_scale, const void* dh, int x_type,
+                                          int64_t dh_ld, const void* weight, int w_type, const float* rstd, void* dx,
+                                          float* dweight, void* scratch, int64_t scratch_bytes, void* stream) {
+  using namespace elr;
+  if (int rc = check_norm(n, D, type, x_type, w_type)) return rc;
+  if (dy_ld < 0 || h_ld < 0 || dh_ld < 0 || group < 0) return ELR_EINVAL;
+  if (!int8_group_ok(group)) return ELR_EUNSUPPORTED;
   if (n > 0) {
-    const bool wide = h_type == ELR_F32;
-    switch (type) {
-      case ELR_F32: launch_norm_back<float, float>(a, (unsigned)blocks, st); break;
-      case ELR_F16:
-        wide ? launch_norm_back<_Float16, float>(a, (unsigned)blocks, st)
-             : launch_norm_back<_Float16, _Float16>(a, (unsigned)blocks, st);
-        break;
-      default:
-        wide ? launch_norm_back<__bf16, float>(a, (unsigned)blocks, st)
-             : launch_norm_back<__bf16, __bf16>(a, (unsigned)blocks, st);
-        break;
-    }
+    if (!dy || !h || !h_scale || !rstd || !dx) return ELR_EINVAL;
+    if (!elem_aligned(dy, type) || !elem_aligned(dh, x_type) || !elem_aligned(dx, x_type) || !elem_aligned(weight, w_type) ||
+        ((uintptr_t)h_scale & 3u))
+      return ELR_EINVAL;
   }
-  if (dweight && (n == 0 || blocks > 1)) {   // no rows: zeros
-    for (int64_t e = 0; e < D; e += kDwColumns) {
-      const int64_t m = D - e < kDwColumns ? D - e : kDwColumns;
-      k_norm_dw<<<(unsigned)((m + 31) / 32), 1024, 0, st>>>(n > 0 ? (const float*)scratch + e : nullptr,
-                                                           n > 0 ? (int)blocks : 0, (int32_t)D, (int32_t)m, dweight + e);
-    }
-  }
-  return launch_status();
+  const NormBackArgs a{dy, h, dh, weight, dy_ld, h_ld, dh_ld, rstd, n, (int32_t)D, w_type == ELR_F32, dx,
+                       nullptr, 0, h_scale, (int32_t)int8_groups(D, group), int8_shift(group)};
+  return norm_back<true>(a, type, x_type, dweight, scratch, scratch_bytes, (hipStream_t)stream);
 }

@@ -4,8 +4,9 @@ counterpart in the reference.
     rms_norm(x, weight, eps=1e-6, residual=None) -> Norm              y = h rstd weight, h = x + residual
     rms_norm_fp8(x, weight, eps=1e-6, residual=None, group=0) -> NormFp8    y as e4m3 values and float32 scales
     rms_norm_backward(dy, h, weight, rstd, dh=None) -> (dx, dweight)
+    rms_norm_backward_int8(dy, h, weight, rstd, dh=None) -> (dx, dweight)   the same with h kept in 8 bits (int8.Int8Rows)
 
-They run the HIP kernels behind elr_rms_norm and elr_rms_norm_backward (elara_amd/csrc/norms.hip) on torch's current
+They run the HIP kernels behind elr_rms_norm, elr_rms_norm_backward and elr_rms_norm_backward_int8 (elara_amd/csrc/norms.hip) on torch's current
 stream: one launch forward (each row is read and written once; rows of more than 4,096 16-byte vectors are read again), two
 backward (one where the rows are few).  Neither registers with autograd: results are detached.
 """
@@ -13,7 +14,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib
+from . import _lib, int8
 
 FP8 = torch.float8_e4m3fn
 GROUPS = (32, 64, 128, 256)
@@ -138,4 +139,44 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dweight=True):
                 _lib.ptr(dhr), _ld(dhr) if dhr is not None else D, _lib.ptr(w), wt, rstd.data_ptr(), dx.data_ptr(),
                 _lib.ptr(dw), _lib.ptr(scratch), nbytes, _lib.raw_stream(dev))
         _lib.check(rc, 'elr_rms_norm_backward')
+    return dx, dw
+
+
+def rms_norm_backward_int8(dy, h, weight, rstd, dh=None, need_dweight=True):
+    """rms_norm_backward with h as int8.Int8Rows of dy's shape, as int8.quantize kept it (any group); rstd: the forward's, of the
+    unrounded h.  dh: dy's shape, in dy's type or float32, or None.  dx has dh's type, dy's without dh."""
+    r = (_lib._host or _lib.host()).norm_back_int8(dy, *h, weight, rstd, dh, int(need_dweight))
+    if r != _lib.NOT_TAKEN:
+        _lib.check(r[0], 'elr_rms_norm_backward_int8')
+        return r[1:]
+    dyr = _rows(dy, 'dy', tuple(_lib.ETYPE))
+    q, q_ld, scale, group = int8.parts(h, 'h')
+    if h.q.shape != dy.shape or q.device != dy.device:
+        raise RuntimeError(f'h.q must have shape {tuple(dy.shape)} on {dy.device}')
+    n, D = dyr.shape
+    dev = dy.device
+    w, wt = _weight(weight, dy)
+    if not (rstd.is_cuda and rstd.device == dev and rstd.dtype == torch.float32 and rstd.shape == dy.shape[:-1]):
+        raise RuntimeError(f'rstd must be a cuda float32 tensor of shape {tuple(dy.shape[:-1])} on {dev}')
+    rstd = rstd.contiguous()
+    dhr, xt = None, dy.dtype
+    if dh is not None:
+        if dh.shape != dy.shape or dh.device != dev:
+            raise RuntimeError(f'dh must have shape {tuple(dy.shape)} on {dev}')
+        dhr, xt = _rows(dh, 'dh', (dy.dtype, torch.float32)), dh.dtype
+    L = _lib.lib()
+    dx = torch.empty(dy.shape, dtype=xt, device=dev)
+    dw = scratch = None
+    nbytes = 0
+    if need_dweight:
+        dw = torch.empty(D, dtype=torch.float32, device=dev)
+        nbytes = L.elr_rms_norm_backward_scratch_bytes(n, D, _lib.ETYPE[dy.dtype])
+        scratch = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+    if n or need_dweight:
+        with _lib.on_device(dev):
+            rc = L.elr_rms_norm_backward_int8(
+                dyr.data_ptr(), _lib.ETYPE[dy.dtype], n, D, _ld(dyr), q.data_ptr(), q_ld, group, scale.data_ptr(),
+                _lib.ptr(dhr), _lib.ETYPE[xt], _ld(dhr) if dhr is not None else D, _lib.ptr(w), wt, rstd.data_ptr(),
+                dx.data_ptr(), _lib.ptr(dw), _lib.ptr(scratch), nbytes, _lib.raw_stream(dev))
+        _lib.check(rc, 'elr_rms_norm_backward_int8')
     return dx, dw

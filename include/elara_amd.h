@@ -787,6 +787,68 @@ int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_t D, int64_
                           void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
+ * Rows in 8-bit integers (no counterpart in the reference): int8 values q and fp32 scales, x = q scale, a scale for each
+ * row (group = 0; scale [n]) or for each `group` of 32, 64, 128 or 256 columns, the last of a row shorter where that does
+ * not divide D (scale [n, ceil(D / group)]).  With a = max|x| over a row or group:
+ *   pow2 = 0: scale = a / 127 in fp32, 1 where that is 0;  pow2 = 1: the smallest power of two s with 127 s >= a, 2^-126 at
+ *   least, 1 for a = 0;  q = x / scale rounded once to the nearest integer, ties to even, in [-127, 127].
+ * A NaN or an infinity gives its row or group scale NaN and q = 0.
+ *   x of `type`, rows x_ld elements apart; q [n, D] and scale contiguous and not overlapping x.
+ * elr_dequantize_int8: x = q scale in fp32, rounded to `type`, contiguous; rows of q q_ld bytes apart.
+ * ------------------------------------------------------------------------------------------------------- */
+int elr_quantize_int8(const void* x, int type, int64_t n, int64_t D, int64_t x_ld, int64_t group, int pow2, int8_t* q,
+                      float* scale, void* stream);
+int elr_dequantize_int8(const int8_t* q, int64_t n, int64_t D, int64_t q_ld, int64_t group, const float* scale, void* x,
+                        int type, void* stream);
+
+/* y[i, j] = x_scale[i] w_scale[j] sum_k x[i, k] w[j, k]: the product of int8 rows x [n, K] with an int8 weight w [N, K], a
+ * scale for each token and each channel.  The sum is exact (int32: K < 2^17, else ELR_EUNSUPPORTED), then widened to fp32,
+ * multiplied by x_scale and by w_scale and rounded to `type`.  Rows of x and w x_ld and w_ld bytes apart; y [n, N]
+ * contiguous, not overlapping x or w.  K = 0 gives zeros times the scales.  scratch of
+ * elr_int8_linear_scratch_bytes(n, N, K) bytes, 16-byte aligned (may be 0; -1: bad argument). */
+int64_t elr_int8_linear_scratch_bytes(int64_t n, int64_t N, int64_t K);
+int elr_int8_linear(const int8_t* x, int64_t n, int64_t K, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t N,
+                    int64_t w_ld, const float* w_scale, void* y, int type, void* scratch, int64_t scratch_bytes,
+                    void* stream);
+
+/* The weight gradient of a linear layer from its input kept in 8-bit integers: dw[j, k] = sum_i dy[i, j] x[i, k], x = q scale
+ * in bf16 (exact where the scales are powers of two), dy (of `type`) unrounded, sums in fp32 in an order that depends on the
+ * sizes alone.  dw fp32 [N, K], or [K, N] with transposed, contiguous; n = 0 gives zeros.  Rows of dy dy_ld elements, of q
+ * q_ld bytes apart; scales as above, over K.  scratch of elr_int8_weight_grad_scratch_bytes bytes, 16-byte aligned (may be
+ * 0; -1: bad argument). */
+int64_t elr_int8_weight_grad_scratch_bytes(int64_t n, int64_t N, int64_t K, int type);
+int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t N, int64_t dy_ld, const int8_t* q, int64_t K,
+                         int64_t q_ld, int64_t group, const float* scale, float* dw, int transposed, void* scratch,
+                         int64_t scratch_bytes, void* stream);
+
+/* elr_rms_norm_backward with h = q scale kept in 8-bit integers (scales as above, over D); dh (or NULL) and dx have x_type =
+ * type or ELR_F32, dx is contiguous and may be dh where that is contiguous too.  scratch of
+ * elr_rms_norm_backward_scratch_bytes(n, D, type) bytes, only with dweight. */
+int elr_rms_norm_backward_int8(const void* dy, int type, int64_t n, int64_t D, int64_t dy_ld, const int8_t* h, int64_t h_ld,
+                               int64_t group, const float* h_scale, const void* dh, int x_type, int64_t dh_ld,
+                               const void* weight, int w_type, const float* rstd, void* dx, float* dweight, void* scratch,
+                               int64_t scratch_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * A token drawn for each row of logits, from a given number in [0, 1) (no counterpart in the reference).  For a row x of V
+ * logits with maximum m:  e = exp((x - m) / temperature);  the order: larger first, ties by the lower id, -0 equal to +0;
+ *   kept: the first top_k of the order (0, or V and more: all); of these, those before which in the order less than top_p of
+ *   their mass lies (1: all; the first always); of these, those with e >= min_p;
+ *   token = the first kept id, in the order of ids, at which the sum of e over kept ids exceeds u times their whole sum S;
+ *   logprob = log(e[token] / S).  temperature = 0: the first of the order, logprob 0.
+ * Sums are of 64-bit integers (e in fp64 times a power of two): the same for every launch, and an e below 2^-44 or so of the
+ * largest is never drawn.  A row of nothing but -inf: token -1, logprob -inf.  A NaN or +inf in a row, a negative or NaN
+ * temperature or a NaN u: token -1, logprob NaN.  u outside [0, 1) counts as the nearest in it.
+ *   logits of `type`, row i at logits + i * ld elements; u fp32 [n]; each setting a value, or one for each row where its
+ *   pointer is not NULL (fp32; top_k int32, or int64 with top_k_64; there values out of range count as the nearest in it,
+ *   a NaN as no limit, and negative top_k as 0); token int64 [n], logprob fp32 [n].
+ * ------------------------------------------------------------------------------------------------------- */
+int elr_sample_tokens(const void* logits, int type, int64_t n, int64_t V, int64_t ld, const float* u, double temperature,
+                      const float* temperature_rows, int64_t top_k, const void* top_k_rows, int top_k_64, double top_p,
+                      const float* top_p_rows, double min_p, const float* min_p_rows, int64_t* token, float* logprob,
+                      void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
  * The global norm of many gradients, and clipping by it (no counterpart in the reference).
  *   norm = (sum |g|^p)^(1/p) over all elements of all n tensors, p = 1, 2, or 0 for the largest |g| (summed in fp64);
  *   clip: out = g min(1, max_norm / (norm + eps)) for each tensor.
