@@ -188,7 +188,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       }
     }
     __syncthreads();
-    return sh.id;
+    const uint32_t id = sh.id;
+    __syncthreads();      // (the next call clears it)
+    return id;
   };
 
   // The threshold (thr, thr_id) at which the order, from its largest on and within the present threshold, has reached `target`: places,

@@ -137,6 +137,23 @@ def test_ties_go_to_the_lowest_ids(dev, dtype):
 
 
 @pytest.mark.gpu
+def test_many_rows_with_ties_at_the_threshold(dev):
+    """Searches that follow one another in a block (for the ties of a threshold, then for the token), over thousands of rows."""
+    sp = _sp()
+    n, V = 6000, 20_000
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randint(0, 12, (n, V), generator=g, device=dev).bfloat16()
+    u = torch.rand(n, generator=g, device=dev)
+    first = (x == x.amax(-1, keepdim=True)).int().argmax(-1)
+    assert torch.equal(sp.sample_tokens(x, u, temperature=0.0).token, first)
+    assert torch.equal(sp.sample_tokens(x, u, top_k=1).token, first)
+    for k in (40, 300):                                       # the first k ids with the largest value, alike in weight
+        at = torch.nonzero(x == 11)[:, 1].split((x == 11).sum(-1).tolist())
+        want = torch.stack([a[min(int(k * float(v)), k - 1)] for a, v in zip(at, u.double().tolist())])
+        assert torch.equal(sp.sample_tokens(x, u, top_k=k).token, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('V', [50, 777, 4096, 33_000])
 def test_settings_by_row(dev, V, dtype):
