@@ -10,7 +10,6 @@
 namespace elr {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 struct WgradArgs {
   const void* dy;
@@ -42,51 +41,184 @@ __device__ __forceinline__ void split_bf16(float x, __bf16 (&p)[P]) {
   }
 }
 
-// Tiles of 64 x 64 of dW, 32 tokens at a time; four waves, a 32 x 32 part each.
+// 16 int8 of a row, those at and past `valid` (any number; <= 0: none read) as 0.
+__device__ __forceinline__ u32x4 int8x16(const int8_t* p, int64_t valid) {
+  typedef u32x4 u32x4_b __attribute__((aligned(1)));
+  if (valid >= 16) return *reinterpret_cast<const u32x4_b*>(p);
+  u32x4 r{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < valid) r[j / 4] |= (uint32_t)(uint8_t)p[j] << (8 * (j & 3));
+  return r;
+}
+
+// The tile of a block.  Blocks go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets a compact part of the tiles, columns of
+// at most 8 tiles one after another, so that its blocks share rows of both operands.
+__device__ __forceinline__ int32_t tile_of(uint32_t b, int32_t tiles_m, int32_t tiles_n) {
+  const uint32_t count = (uint32_t)tiles_m * (uint32_t)tiles_n;
+  const uint32_t full = count / 8 * 8;
+  const uint32_t i = b < full ? b % 8 * (count / 8) + b / 8 : b;      // the i-th in the order of tiles
+  const uint32_t band = 8 * (uint32_t)tiles_n, first = i / band * 8;  // bands of 8 rows of tiles, each by columns
+  const uint32_t rows = (uint32_t)tiles_m - first < 8 ? (uint32_t)tiles_m - first : 8, in = i % band;
+  return (int32_t)((first + in % rows) * (uint32_t)tiles_n + in / rows);
+}
+
+// Staged loads.  A token's row of a tile lies in LDS as it lies in memory (PITCH elements apart, so that four tokens' rows fall into
+// different banks); the products' operands, eight tokens of a column a lane, come from LDS by its transposing read, which gives lane i of
+// 16 the four tokens of column i.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+__device__ __forceinline__ bf16x8 tokens_of(const __bf16* p, int pitch) {   // p: this lane's place in the first four of eight rows
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * pitch));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// 8 elements of a row from e on, those outside [0, valid) as 0.
 template <class E>
-__global__ __launch_bounds__(256) void k_wgrad(WgradArgs a) {
-  constexpr int P = kParts<E>;
-  __shared__ __bf16 ly[P][32][64 + 2], lx[32][64 + 2];
+struct Row8 {
+  u32x4 v[8 / Elem<E>::VE];
+};
+template <class E>
+__device__ __forceinline__ Row8<E> load8(const E* p, int64_t valid) {
+  Row8<E> r;
+#pragma unroll
+  for (int i = 0; i < 8 / Elem<E>::VE; ++i) r.v[i] = load_raw<E, false>(p + i * Elem<E>::VE, valid - i * Elem<E>::VE, 0.0f);
+  return r;
+}
+
+// Tiles of BM x BN of dW, 32 tokens a step, two LDS buffers: while one is multiplied the next step's rows are on their way into registers,
+// from where they go, in bf16, into the other.  WM x WN waves, each a part of the tile in products of 32 x 32 x 16.
+template <class E, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
+  constexpr int P = kParts<E>, T = WM * WN * 64, BT = 32, PM = BM + 16, PN = BN + 16;
+  constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
+  constexpr int RY = BT * BM / 8 / T, RX = BT * BN / 16 / T;       // row pieces of a thread: 8 of dy, 16 of x
+  static_assert(RY >= 1 && RX >= 1 && RY * T * 8 == BT * BM && RX * T * 16 == BT * BN, "whole pieces");
+  extern __shared__ __attribute__((aligned(16))) __bf16 lds[];     // [2][P][BT][PM], then [2][BT][PN]
+  __bf16* const ly = lds;
+  __bf16* const lx = lds + 2 * P * BT * PM;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+  const int32_t tile = tile_of(blockIdx.x, tiles_m, tiles_n);
+  const int32_t m0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const int64_t from = (int64_t)blockIdx.z * a.per_split, to = from + a.per_split < a.n ? from + a.per_split : a.n;
-  f32x16 acc{};
-  const int c = threadIdx.x & 63;
-  for (int64_t i0 = from; i0 < to; i0 += 32) {
-    __syncthreads();
-    for (int r = wave; r < 32; r += 4) {
-      const int64_t i = i0 + r;
-      __bf16 p[P];
-      split_bf16<P>(i < to && m0 + c < a.N ? (float)((const E*)a.dy)[i * a.dy_ld + m0 + c] : 0.0f, p);
+  f32x16 acc[MT][NT];
 #pragma unroll
-      for (int t = 0; t < P; ++t) ly[t][r][c] = p[t];
-      const bool in = i < to && n0 + c < a.K;
-      lx[r][c] = (__bf16)(in ? (float)a.q[i * a.q_ld + n0 + c] * a.scale[i * a.groups + ((n0 + c) >> a.shift)] : 0.0f);
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
+  Row8<E> gy[RY];
+  u32x4 gx[RX];
+  float gs[RX];
+  const auto load = [&](int64_t i0) {
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BM / 8), c = m0 + at % (BM / 8) * 8;
+      const bool in = i0 + t < to;
+      gy[r] = load8<E>((const E*)a.dy + (in && c < a.N ? (i0 + t) * a.dy_ld + c : 0), in ? a.N - c : 0);
     }
-    __syncthreads();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8 fx;
-      const int k = h * 16 + (lane >> 5) * 8;
+    for (int r = 0; r < RX; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BN / 16), c = n0 + at % (BN / 16) * 16;
+      const bool in = i0 + t < to && c < a.K;
+      const int8_t* p = a.q + (in ? (i0 + t) * a.q_ld + c : 0);
+      gx[r] = int8x16(p, in ? a.K - c : 0);
+      gs[r] = in ? a.scale[(i0 + t) * a.groups + (c >> a.shift)] : 0.0f;     // (16 columns lie within one group)
+    }
+  };
+  const auto store = [&](int buf) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) fx[j] = lx[k + j][wn + (lane & 31)];
+    for (int r = 0; r < RY; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BM / 8), c = at % (BM / 8) * 8;
+      __bf16* p = ly + (buf * P * BT + t) * PM + c;
+      if constexpr (P == 1) {
+        *reinterpret_cast<u32x4*>(p) = gy[r].v[0];
+      } else {
+        __bf16 part[8][P];
 #pragma unroll
-      for (int t = 0; t < P; ++t) {
-        bf16x8 fy;
+        for (int i = 0; i < 8 / Elem<E>::VE; ++i) {
+          const Frag<E> f = widen<E>(gy[r].v[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) fy[j] = ly[t][k + j][wm + (lane & 31)];
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy, fx, acc, 0, 0, 0);
+          for (int j = 0; j < Elem<E>::VE; ++j) split_bf16<P>(f.v[j], part[i * Elem<E>::VE + j]);
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          bf16x8 v;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = part[j][q];
+          *reinterpret_cast<bf16x8*>(p + q * BT * PM) = v;
+        }
       }
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BN / 16), c = at % (BN / 16) * 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x8 f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(gx[r][2 * h + j / 4] >> (8 * (j & 3))) * gs[r];
+        *reinterpret_cast<bf16x8*>(lx + (buf * BT + t) * PN + c + 8 * h) = __builtin_convertvector(f, bf16x8);
+      }
+    }
+  };
+  // this lane's place in a 16 x 32 block of tokens and columns
+  const int tr = (lane >> 5) * 8 + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  const auto multiply = [&](int buf) {
+#pragma unroll
+    for (int h = 0; h < BT / 16; ++h) {
+      bf16x8 fx[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fx[j] = tokens_of(lx + (buf * BT + h * 16 + tr) * PN + wn + j * 32 + tc, PN);
+#pragma unroll
+      for (int q = P - 1; q >= 0; --q) {      // the smallest parts first
+        bf16x8 fy[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fy[i] = tokens_of(ly + ((buf * P + q) * BT + h * 16 + tr) * PM + wm + i * 32 + tc, PM);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[i], fx[j], acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  if (from < to) {
+    load(from);
+    store(0);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t i0 = from; i0 < to; i0 += BT) {
+      const bool more = i0 + BT < to;
+      if (more) load(i0 + BT);
+      multiply(buf);
+      if (more) store(buf ^ 1);
+      __syncthreads();
+      buf ^= 1;
     }
   }
   float* out = a.out + (int64_t)blockIdx.z * a.N * a.K;
-  const int32_t col = n0 + wn + (lane & 31);
 #pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    const int32_t row = m0 + wm + (q >> 2) * 8 + (lane >> 5) * 4 + (q & 3);
-    if (row < a.N && col < a.K) out[a.transposed ? (int64_t)col * a.N + row : (int64_t)row * a.K + col] = acc[q];
-  }
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int32_t col = n0 + wn + j * 32 + (lane & 31);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int32_t row = m0 + wm + i * 32 + q * 8 + (lane >> 5) * 4;
+        if (col >= a.K) continue;
+        if (a.transposed) {
+          store_raw<float, false>(out + (int64_t)col * a.N + row,
+                                  __builtin_bit_cast(u32x4, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                                                  acc[i][j][4 * q + 3]}), a.N - row);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (row + t < a.N) out[(int64_t)(row + t) * a.K + col] = acc[i][j][4 * q + t];
+        }
+      }
+    }
 }
 
 // out = the sum of the splits' parts, in their order.
@@ -100,16 +232,33 @@ __global__ __launch_bounds__(256) void k_wgrad_join(const float* part, int split
 
 // ---- host side
 
-static int64_t wgrad_splits(int64_t n, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + 63) / 64) * ((K + 63) / 64);
-  int64_t s = (512 + tiles - 1) / tiles, most = n / 256;
-  if (s > most) s = most;
-  return s < 1 ? 1 : s > 64 ? 64 : s;
+// Tiles and splits of the tokens.  256 x 256 where such tiles alone nearly fill the chip, else 128 x 128 with the tokens split so that
+// about two blocks a CU run, of 256 tokens at least.
+struct WgradPlan {
+  int tile;
+  int64_t tiles_m, tiles_n, splits;
+};
+static WgradPlan wgrad_plan(int64_t n, int64_t N, int64_t K) {
+  const auto tiles = [](int64_t x, int64_t t) { return (x + t - 1) / t; };
+  if (tiles(N, 256) * tiles(K, 256) >= 192) return {256, tiles(N, 256), tiles(K, 256), 1};
+  const int64_t m = tiles(N, 128), k = tiles(K, 128), most = n / 256 < 64 ? n / 256 : 64;
+  int64_t s = 512 / (m * k);
+  s = s > most ? most : s;
+  return {128, m, k, s < 1 ? 1 : s};
+}
+
+template <class E, int B, int WM, int WN>
+static void launch_wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
+  constexpr int kLds = 2 * (kParts<E> + 1) * 32 * (B + 16) * 2;
+  static_assert(kLds <= 160 << 10, "LDS of a CU");
+  k_wgrad<E, B, B, WM, WN><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), WM * WN * 64, kLds, st>>>(
+      a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
 }
 
 template <class E>
-static void wgrad(const WgradArgs& a, int splits, hipStream_t st) {
-  k_wgrad<E><<<dim3((unsigned)((a.K + 63) / 64), (unsigned)((a.N + 63) / 64), (unsigned)splits), 256, 0, st>>>(a);
+static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
+  if (p.tile == 256) launch_wgrad<E, 256, 2, 4>(a, p, st);
+  else launch_wgrad<E, 128, 2, 2>(a, p, st);
 }
 
 }  // namespace elr
@@ -117,7 +266,7 @@ static void wgrad(const WgradArgs& a, int splits, hipStream_t st) {
 extern "C" int64_t elr_int8_weight_grad_scratch_bytes(int64_t n, int64_t N, int64_t K, int type) {
   if (n < 0 || N < 0 || K < 0 || !elr::elem_type_ok(type)) return -1;
   if (N == 0 || K == 0) return 0;
-  const int64_t s = elr::wgrad_splits(n, N, K);
+  const int64_t s = elr::wgrad_plan(n, N, K).splits;
   return s > 1 ? s * N * K * 4 : 0;
 }
 
@@ -130,14 +279,15 @@ extern "C" int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t
   if (N == 0 || K == 0) return ELR_OK;
   if (!dw || ((uintptr_t)dw & 3u) || (n > 0 && (!dy || !q || !scale || !elem_aligned(dy, type) || ((uintptr_t)scale & 3u))))
     return ELR_EINVAL;
-  const int64_t splits = wgrad_splits(n, N, K);
+  const WgradPlan plan = wgrad_plan(n, N, K);
+  const int64_t splits = plan.splits;
   if (splits > 1 && (!scratch || scratch_bytes < splits * N * K * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const WgradArgs a{dy, q, scale, dy_ld, q_ld, n, ((n + splits - 1) / splits + 31) / 32 * 32, (int32_t)N, (int32_t)K,
                     (int32_t)int8_groups(K, group), int8_shift(group), splits > 1 ? (float*)scratch : dw, transposed};
   hipStream_t st = (hipStream_t)stream;
-  if (type == ELR_F32) wgrad<float>(a, (int)splits, st);
-  else if (type == ELR_F16) wgrad<_Float16>(a, (int)splits, st);
-  else wgrad<__bf16>(a, (int)splits, st);
+  if (type == ELR_F32) wgrad<float>(a, plan, st);
+  else if (type == ELR_F16) wgrad<_Float16>(a, plan, st);
+  else wgrad<__bf16>(a, plan, st);
   if (splits > 1) k_wgrad_join<<<grid_for(N * K, 256), 256, 0, st>>>((const float*)scratch, (int)splits, N * K, dw);
   return launch_status();
 }
