@@ -41,17 +41,6 @@ __device__ __forceinline__ void split_bf16(float x, __bf16 (&p)[P]) {
   }
 }
 
-// 16 int8 of a row, those at and past `valid` (any number; <= 0: none read) as 0.
-__device__ __forceinline__ u32x4 int8x16(const int8_t* p, int64_t valid) {
-  typedef u32x4 u32x4_b __attribute__((aligned(1)));
-  if (valid >= 16) return *reinterpret_cast<const u32x4_b*>(p);
-  u32x4 r{0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (j < valid) r[j / 4] |= (uint32_t)(uint8_t)p[j] << (8 * (j & 3));
-  return r;
-}
-
 // The tile of a block.  Blocks go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets a compact part of the tiles, columns of
 // at most 8 tiles one after another, so that its blocks share rows of both operands.
 __device__ __forceinline__ int32_t tile_of(uint32_t b, int32_t tiles_m, int32_t tiles_n) {
@@ -88,14 +77,20 @@ __device__ __forceinline__ Row8<E> load8(const E* p, int64_t valid) {
   return r;
 }
 
-// Tiles of BM x BN of dW, 32 tokens a step, two LDS buffers: while one is multiplied the next step's rows are on their way into registers,
-// from where they go, in bf16, into the other.  WM x WN waves, each a part of the tile in products of 32 x 32 x 16.
-template <class E, int BM, int BN, int WM, int WN>
+// Tiles of BM x BN of dW, 32 tokens a step, two LDS buffers; the rows of the next two steps are on their way into registers, from where
+// they go, in bf16, into the buffer that is not multiplied.  WM x WN waves, each a part of the tile in products of 32 x 32 x 16.
+// Rows in LDS are 64 bytes longer than the tile's: two neighbouring blocks of 4 tokens x 16 columns then take all 64 banks once.
+//
+// Edges.  No load in the loop is conditional (a branch around a load ends in a wait for it).  A piece of 8 columns that the matrix ends
+// within is loaded 8 columns from the end and only its own columns are stored; pieces past the end are loaded from there too and not
+// stored: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
+// NARROW: a matrix of less than 8 columns, loaded by element.
+template <class E, int BM, int BN, int WM, int WN, bool NARROW>
 __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
-  constexpr int P = kParts<E>, T = WM * WN * 64, BT = 32, PM = BM + 16, PN = BN + 16;
+  constexpr int P = kParts<E>, T = WM * WN * 64, BT = 32, PM = BM + 32, PN = BN + 32;
   constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
-  constexpr int RY = BT * BM / 8 / T, RX = BT * BN / 16 / T;       // row pieces of a thread: 8 of dy, 16 of x
-  static_assert(RY >= 1 && RX >= 1 && RY * T * 8 == BT * BM && RX * T * 16 == BT * BN, "whole pieces");
+  constexpr int RY = BT * BM / 8 / T, RX = BT * BN / 8 / T;       // row pieces of 8 of a thread
+  static_assert(RY >= 1 && RX >= 1 && RY * T * 8 == BT * BM && RX * T * 8 == BT * BN, "whole pieces");
   extern __shared__ __attribute__((aligned(16))) __bf16 lds[];     // [2][P][BT][PM], then [2][BT][PN]
   __bf16* const ly = lds;
   __bf16* const lx = lds + 2 * P * BT * PM;
@@ -109,59 +104,88 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
-  Row8<E> gy[RY];
-  u32x4 gx[RX];
-  float gs[RX];
-  const auto load = [&](int64_t i0) {
+  struct Step {
+    Row8<E> y[RY];
+    u32x2 x[RX];
+    float s[RX];
+  };
+  const int32_t last = (int32_t)(to - from) - 1;                   // of the split's tokens, by their number in it
+  const E* const dy = (const E*)a.dy + from * a.dy_ld;
+  const int8_t* const q = a.q + from * a.q_ld;
+  const float* const scale = a.scale + from * a.groups;
+  // the first column of the piece at c of a matrix of `cols` columns, as it is loaded
+  const auto piece = [](int32_t c, int32_t cols) { return NARROW ? c : c < cols - 8 ? c : cols - 8; };
+  const auto load = [&](Step& g, int32_t i0) {
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const int at = r * T + threadIdx.x, i = i0 + at / (BM / 8), c = m0 + at % (BM / 8) * 8;
+      const E* p = dy + (int64_t)(i < last ? i : last) * a.dy_ld + piece(c, a.N);
+      if constexpr (NARROW) {
+        g.y[r] = load8<E>(c < a.N ? p : dy, a.N - c);
+      } else {
+        const u32x4_u* v = reinterpret_cast<const u32x4_u*>(p);
+#pragma unroll
+        for (int k = 0; k < 8 / Elem<E>::VE; ++k) g.y[r].v[k] = v[k];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {      // (8 columns lie within one group)
+      const int at = r * T + threadIdx.x, i = i0 + at / (BN / 8), c = n0 + at % (BN / 8) * 8;
+      const int64_t row = i < last ? i : last;
+      const int8_t* p = q + row * a.q_ld + piece(c, a.K);
+      if constexpr (NARROW) {
+        const Int8Raw<__bf16> v = int8_load<__bf16>(c < a.K ? p : q, a.K - c);
+        g.x[r] = u32x2{v.v[0], v.v[1]};
+      } else {
+        typedef u32x2 u32x2_b __attribute__((aligned(1)));
+        g.x[r] = *reinterpret_cast<const u32x2_b*>(p);
+      }
+      g.s[r] = scale[row * a.groups + ((c < a.K ? c : 0) >> a.shift)];
+    }
+  };
+  // eight values to a row in LDS, from column c of the tile that starts at `first`
+  const auto put = [&](__bf16* row, int32_t first, int32_t c, int32_t cols, bf16x8 v) {
+    if (NARROW || c <= cols - 8) {
+      *reinterpret_cast<bf16x8*>(row + (c - first)) = v;
+    } else if (c < cols) {
+#pragma unroll
+      for (int j = 1; j < 8; ++j)
+        if (cols - 8 + j >= c) row[cols - 8 + j - first] = v[j];
+    }
+  };
+  const auto store = [&](const Step& g, int32_t i0, int buf) {
 #pragma unroll
     for (int r = 0; r < RY; ++r) {
       const int at = r * T + threadIdx.x, t = at / (BM / 8), c = m0 + at % (BM / 8) * 8;
-      const bool in = i0 + t < to;
-      gy[r] = load8<E>((const E*)a.dy + (in && c < a.N ? (i0 + t) * a.dy_ld + c : 0), in ? a.N - c : 0);
-    }
-#pragma unroll
-    for (int r = 0; r < RX; ++r) {
-      const int at = r * T + threadIdx.x, t = at / (BN / 16), c = n0 + at % (BN / 16) * 16;
-      const bool in = i0 + t < to && c < a.K;
-      const int8_t* p = a.q + (in ? (i0 + t) * a.q_ld + c : 0);
-      gx[r] = int8x16(p, in ? a.K - c : 0);
-      gs[r] = in ? a.scale[(i0 + t) * a.groups + (c >> a.shift)] : 0.0f;     // (16 columns lie within one group)
-    }
-  };
-  const auto store = [&](int buf) {
-#pragma unroll
-    for (int r = 0; r < RY; ++r) {
-      const int at = r * T + threadIdx.x, t = at / (BM / 8), c = at % (BM / 8) * 8;
-      __bf16* p = ly + (buf * P * BT + t) * PM + c;
+      const bool live = i0 + t <= last;
+      __bf16* row = ly + (buf * P * BT + t) * PM;
       if constexpr (P == 1) {
-        *reinterpret_cast<u32x4*>(p) = gy[r].v[0];
+        put(row, m0, c, a.N, __builtin_bit_cast(bf16x8, live ? g.y[r].v[0] : u32x4{0, 0, 0, 0}));
       } else {
         __bf16 part[8][P];
 #pragma unroll
         for (int i = 0; i < 8 / Elem<E>::VE; ++i) {
-          const Frag<E> f = widen<E>(gy[r].v[i]);
+          const Frag<E> f = widen<E>(live ? g.y[r].v[i] : u32x4{0, 0, 0, 0});
 #pragma unroll
           for (int j = 0; j < Elem<E>::VE; ++j) split_bf16<P>(f.v[j], part[i * Elem<E>::VE + j]);
         }
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
+        for (int k = 0; k < P; ++k) {
           bf16x8 v;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = part[j][q];
-          *reinterpret_cast<bf16x8*>(p + q * BT * PM) = v;
+          for (int j = 0; j < 8; ++j) v[j] = part[j][k];
+          put(row + k * BT * PM, m0, c, a.N, v);
         }
       }
     }
 #pragma unroll
     for (int r = 0; r < RX; ++r) {
-      const int at = r * T + threadIdx.x, t = at / (BN / 16), c = at % (BN / 16) * 16;
+      const int at = r * T + threadIdx.x, t = at / (BN / 8), c = n0 + at % (BN / 8) * 8;
+      const float sc = i0 + t <= last ? g.s[r] : 0.0f;
+      f32x8 f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x8 f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(gx[r][2 * h + j / 4] >> (8 * (j & 3))) * gs[r];
-        *reinterpret_cast<bf16x8*>(lx + (buf * BT + t) * PN + c + 8 * h) = __builtin_convertvector(f, bf16x8);
-      }
+      for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(g.x[r][j / 4] >> (8 * (j & 3))) * sc;
+      put(lx + (buf * BT + t) * PN, n0, c, a.K, __builtin_convertvector(f, bf16x8));
     }
   };
   // this lane's place in a 16 x 32 block of tokens and columns
@@ -185,17 +209,19 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
     }
   };
   if (from < to) {
-    load(from);
-    store(0);
+    Step g[2];
+    load(g[0], 0);
+    load(g[1], BT);
+    store(g[0], 0, 0);
     __syncthreads();
-    int buf = 0;
-    for (int64_t i0 = from; i0 < to; i0 += BT) {
-      const bool more = i0 + BT < to;
-      if (more) load(i0 + BT);
-      multiply(buf);
-      if (more) store(buf ^ 1);
-      __syncthreads();
-      buf ^= 1;
+    for (int32_t i = 0; i <= last; i += 2 * BT) {      // (a second half past the end multiplies zeros)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load(g[h], i + (h + 2) * BT);
+        multiply(h);
+        store(g[h ^ 1], i + (h + 1) * BT, h ^ 1);
+        __syncthreads();
+      }
     }
   }
   float* out = a.out + (int64_t)blockIdx.z * a.N * a.K;
@@ -240,24 +266,29 @@ struct WgradPlan {
 };
 static WgradPlan wgrad_plan(int64_t n, int64_t N, int64_t K) {
   const auto tiles = [](int64_t x, int64_t t) { return (x + t - 1) / t; };
-  if (tiles(N, 256) * tiles(K, 256) >= 192) return {256, tiles(N, 256), tiles(K, 256), 1};
+  if (N >= 8 && K >= 8 && tiles(N, 256) * tiles(K, 256) >= 192) return {256, tiles(N, 256), tiles(K, 256), 1};
   const int64_t m = tiles(N, 128), k = tiles(K, 128), most = n / 256 < 64 ? n / 256 : 64;
   int64_t s = 512 / (m * k);
   s = s > most ? most : s;
   return {128, m, k, s < 1 ? 1 : s};
 }
 
+template <class E, int B>
+constexpr int kWgradLds = 2 * (kParts<E> + 1) * 32 * (B + 32) * 2;
+
 template <class E, int B, int WM, int WN>
 static void launch_wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
-  constexpr int kLds = 2 * (kParts<E> + 1) * 32 * (B + 16) * 2;
-  static_assert(kLds <= 160 << 10, "LDS of a CU");
-  k_wgrad<E, B, B, WM, WN><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), WM * WN * 64, kLds, st>>>(
-      a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
+  static_assert(kWgradLds<E, B> <= 160 << 10, "LDS of a CU");
+  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits);
+  k_wgrad<E, B, B, WM, WN, false><<<grid, WM * WN * 64, kWgradLds<E, B>, st>>>(a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
 }
 
 template <class E>
 static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
-  if (p.tile == 256) launch_wgrad<E, 256, 2, 4>(a, p, st);
+  if (a.N < 8 || a.K < 8)
+    k_wgrad<E, 128, 128, 2, 2, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128>, st>>>(
+        a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
+  else if (p.tile == 256) launch_wgrad<E, 256, 2, 4>(a, p, st);
   else launch_wgrad<E, 128, 2, 2>(a, p, st);
 }
 
