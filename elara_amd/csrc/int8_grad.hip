@@ -7,6 +7,8 @@
 // not finite: the value first, then zeros.
 #include "elr_int8.h"
 
+#include <type_traits>
+
 namespace elr {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -77,14 +79,29 @@ __device__ __forceinline__ Row8<E> load8(const E* p, int64_t valid) {
   return r;
 }
 
+// Order of a step: half of the reads of operands, then between any two products some of the conversions for the next step (the matrix
+// unit works on a product for 32 cycles, of which its issue takes 4) and the rest of the reads.
+template <int PRODUCTS, int READS>
+__device__ __forceinline__ void interleave() {
+  constexpr int kVmem = 0x20, kMfma = 0x8, kValu = 0x2, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kVmem, 64, 0);
+  __builtin_amdgcn_sched_group_barrier(kRead, READS / 2, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, (READS + PRODUCTS - 1) / PRODUCTS, 0);
+  }
+}
+
 // Tiles of BM x BN of dW, 32 tokens a step, two LDS buffers; the rows of the next two steps are on their way into registers, from where
 // they go, in bf16, into the buffer that is not multiplied.  WM x WN waves, each a part of the tile in products of 32 x 32 x 16.
 // Rows in LDS are 64 bytes longer than the tile's: two neighbouring blocks of 4 tokens x 16 columns then take all 64 banks once.
 //
 // Edges.  No load in the loop is conditional (a branch around a load ends in a wait for it).  A piece of 8 columns that the matrix ends
-// within is loaded 8 columns from the end and only its own columns are stored; pieces past the end are loaded from there too and not
-// stored: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
-// NARROW: a matrix of less than 8 columns, loaded by element.
+// within is loaded from 8 columns before the end on, and its own columns are then stored again in their place; pieces past the end are
+// loaded from there too: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
+// NARROW: a matrix of less than 8 columns, or with rows far apart, loaded with checks.
 template <class E, int BM, int BN, int WM, int WN, bool NARROW>
 __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
   constexpr int P = kParts<E>, T = WM * WN * 64, BT = 32, PM = BM + 32, PN = BN + 32;
@@ -110,82 +127,129 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
     float s[RX];
   };
   const int32_t last = (int32_t)(to - from) - 1;                   // of the split's tokens, by their number in it
-  const E* const dy = (const E*)a.dy + from * a.dy_ld;
-  const int8_t* const q = a.q + from * a.q_ld;
-  const float* const scale = a.scale + from * a.groups;
   // the first column of the piece at c of a matrix of `cols` columns, as it is loaded
-  const auto piece = [](int32_t c, int32_t cols) { return NARROW ? c : c < cols - 8 ? c : cols - 8; };
-  const auto load = [&](Step& g, int32_t i0) {
-#pragma unroll
-    for (int r = 0; r < RY; ++r) {
-      const int at = r * T + threadIdx.x, i = i0 + at / (BM / 8), c = m0 + at % (BM / 8) * 8;
-      const E* p = dy + (int64_t)(i < last ? i : last) * a.dy_ld + piece(c, a.N);
-      if constexpr (NARROW) {
-        g.y[r] = load8<E>(c < a.N ? p : dy, a.N - c);
-      } else {
-        const u32x4_u* v = reinterpret_cast<const u32x4_u*>(p);
-#pragma unroll
-        for (int k = 0; k < 8 / Elem<E>::VE; ++k) g.y[r].v[k] = v[k];
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < RX; ++r) {      // (8 columns lie within one group)
-      const int at = r * T + threadIdx.x, i = i0 + at / (BN / 8), c = n0 + at % (BN / 8) * 8;
-      const int64_t row = i < last ? i : last;
-      const int8_t* p = q + row * a.q_ld + piece(c, a.K);
-      if constexpr (NARROW) {
-        const Int8Raw<__bf16> v = int8_load<__bf16>(c < a.K ? p : q, a.K - c);
-        g.x[r] = u32x2{v.v[0], v.v[1]};
-      } else {
-        typedef u32x2 u32x2_b __attribute__((aligned(1)));
-        g.x[r] = *reinterpret_cast<const u32x2_b*>(p);
-      }
-      g.s[r] = scale[row * a.groups + ((c < a.K ? c : 0) >> a.shift)];
-    }
-  };
-  // eight values to a row in LDS, from column c of the tile that starts at `first`
-  const auto put = [&](__bf16* row, int32_t first, int32_t c, int32_t cols, bf16x8 v) {
-    if (NARROW || c <= cols - 8) {
-      *reinterpret_cast<bf16x8*>(row + (c - first)) = v;
-    } else if (c < cols) {
-#pragma unroll
-      for (int j = 1; j < 8; ++j)
-        if (cols - 8 + j >= c) row[cols - 8 + j - first] = v[j];
-    }
-  };
-  const auto store = [&](const Step& g, int32_t i0, int buf) {
+  const auto piece = [](int32_t c, int32_t cols) { return NARROW ? (c < cols ? c : 0) : c < cols - 8 ? c : cols - 8; };
+  // Places of this thread's pieces from a step's first token on: 32 bits beside an address that the step's waves share (NARROW: 64).
+  typedef typename std::conditional<NARROW, int64_t, uint32_t>::type off_t;
+  off_t oy[RY], ox[RX], os[RX];
+  const auto places = [&](int32_t most) {      // tokens past the most-th: that one
 #pragma unroll
     for (int r = 0; r < RY; ++r) {
       const int at = r * T + threadIdx.x, t = at / (BM / 8), c = m0 + at % (BM / 8) * 8;
-      const bool live = i0 + t <= last;
-      __bf16* row = ly + (buf * P * BT + t) * PM;
-      if constexpr (P == 1) {
-        put(row, m0, c, a.N, __builtin_bit_cast(bf16x8, live ? g.y[r].v[0] : u32x4{0, 0, 0, 0}));
+      oy[r] = ((off_t)(t < most ? t : most) * (off_t)a.dy_ld + (off_t)piece(c, a.N)) * (off_t)sizeof(E);
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BN / 8), c = n0 + at % (BN / 8) * 8, tt = t < most ? t : most;
+      ox[r] = (off_t)tt * (off_t)a.q_ld + (off_t)piece(c, a.K);
+      os[r] = ((off_t)tt * (off_t)a.groups + (off_t)((c < a.K ? c : 0) >> a.shift)) * 4;      // (8 columns lie within one group)
+    }
+  };
+  places(BT);
+  const auto load = [&](Step& g, int32_t i0) {
+    if (i0 + BT - 1 > last) {                  // the last steps
+      i0 = i0 < last ? i0 : last;
+      places(last - i0);
+    }
+    const char* const dy = (const char*)a.dy + (from + i0) * a.dy_ld * (int64_t)sizeof(E);
+    const char* const q = (const char*)a.q + (from + i0) * a.q_ld;
+    const char* const scale = (const char*)(a.scale + (from + i0) * a.groups);
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      if constexpr (NARROW) {
+        const int c = m0 + (r * T + threadIdx.x) % (BM / 8) * 8;
+        g.y[r] = load8<E>((const E*)(dy + oy[r]), a.N - c);
       } else {
-        __bf16 part[8][P];
+#pragma unroll
+        for (int k = 0; k < 8 / Elem<E>::VE; ++k) g.y[r].v[k] = *reinterpret_cast<const u32x4_u*>(dy + oy[r] + 16 * k);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {
+      if constexpr (NARROW) {
+        const int c = n0 + (r * T + threadIdx.x) % (BN / 8) * 8;
+        const Int8Raw<__bf16> v = int8_load<__bf16>((const int8_t*)(q + ox[r]), a.K - c);
+        g.x[r] = u32x2{v.v[0], v.v[1]};
+      } else {
+        typedef u32x2 u32x2_b __attribute__((aligned(1)));
+        g.x[r] = *reinterpret_cast<const u32x2_b*>(q + ox[r]);
+      }
+      g.s[r] = *reinterpret_cast<const float*>(scale + os[r]);
+    }
+  };
+  // A step's rows in bf16, tokens past the end zero.
+  struct Rows {
+    bf16x8 y[RY][P], x[RX];
+  };
+  const auto convert = [&](Step& g, int32_t i0) {
+    Rows w;
+    if (i0 + BT - 1 > last) {
+#pragma unroll
+      for (int r = 0; r < RY; ++r)
+        if (i0 + (int)(r * T + threadIdx.x) / (BM / 8) > last)
+#pragma unroll
+          for (int k = 0; k < 8 / Elem<E>::VE; ++k) g.y[r].v[k] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < RX; ++r)
+        if (i0 + (int)(r * T + threadIdx.x) / (BN / 8) > last) g.s[r] = 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      if constexpr (P == 1) {
+        w.y[r][0] = __builtin_bit_cast(bf16x8, g.y[r].v[0]);
+      } else {
 #pragma unroll
         for (int i = 0; i < 8 / Elem<E>::VE; ++i) {
-          const Frag<E> f = widen<E>(live ? g.y[r].v[i] : u32x4{0, 0, 0, 0});
+          const Frag<E> f = widen<E>(g.y[r].v[i]);
 #pragma unroll
-          for (int j = 0; j < Elem<E>::VE; ++j) split_bf16<P>(f.v[j], part[i * Elem<E>::VE + j]);
-        }
+          for (int j = 0; j < Elem<E>::VE; ++j) {
+            __bf16 part[P];
+            split_bf16<P>(f.v[j], part);
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-          bf16x8 v;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = part[j][k];
-          put(row + k * BT * PM, m0, c, a.N, v);
+            for (int k = 0; k < P; ++k) w.y[r][k][i * Elem<E>::VE + j] = part[k];
+          }
         }
       }
     }
 #pragma unroll
     for (int r = 0; r < RX; ++r) {
-      const int at = r * T + threadIdx.x, t = at / (BN / 8), c = n0 + at % (BN / 8) * 8;
-      const float sc = i0 + t <= last ? g.s[r] : 0.0f;
       f32x8 f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(g.x[r][j / 4] >> (8 * (j & 3))) * sc;
-      put(lx + (buf * BT + t) * PN, n0, c, a.K, __builtin_convertvector(f, bf16x8));
+      for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)(g.x[r][j / 4] >> (8 * (j & 3))) * g.s[r];
+      w.x[r] = __builtin_convertvector(f, bf16x8);
+    }
+    return w;
+  };
+  const bool ends = !NARROW && ((m0 + BM > a.N && a.N % 8) || (n0 + BN > a.K && a.K % 8));   // a piece that a matrix ends within
+  const auto store = [&](const Rows& w, int buf) {
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BM / 8), c = at % (BM / 8) * 8;
+#pragma unroll
+      for (int k = 0; k < P; ++k) *reinterpret_cast<bf16x8*>(ly + ((buf * P + k) * BT + t) * PM + c) = w.y[r][k];
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BN / 8), c = at % (BN / 8) * 8;
+      *reinterpret_cast<bf16x8*>(lx + (buf * BT + t) * PN + c) = w.x[r];
+    }
+    if (!ends) return;
+    const auto again = [](__bf16* row, int c, int end, bf16x8 v) {      // columns c..end of a piece that was loaded from end - 8 on
+      if (c < end && c + 8 > end)
+#pragma unroll
+        for (int j = 1; j < 8; ++j)
+          if (end - 8 + j >= c) row[end - 8 + j] = v[j];
+    };
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BM / 8), c = at % (BM / 8) * 8;
+#pragma unroll
+      for (int k = 0; k < P; ++k) again(ly + ((buf * P + k) * BT + t) * PM, c, a.N - m0, w.y[r][k]);
+    }
+#pragma unroll
+    for (int r = 0; r < RX; ++r) {
+      const int at = r * T + threadIdx.x, t = at / (BN / 8), c = at % (BN / 8) * 8;
+      again(lx + (buf * BT + t) * PN, c, a.K - n0, w.x[r]);
     }
   };
   // this lane's place in a 16 x 32 block of tokens and columns
@@ -212,14 +276,16 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
     Step g[2];
     load(g[0], 0);
     load(g[1], BT);
-    store(g[0], 0, 0);
+    store(convert(g[0], 0), 0);
     __syncthreads();
     for (int32_t i = 0; i <= last; i += 2 * BT) {      // (a second half past the end multiplies zeros)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         load(g[h], i + (h + 2) * BT);
+        const Rows w = convert(g[h ^ 1], i + (h + 1) * BT);
         multiply(h);
-        store(g[h ^ 1], i + (h + 1) * BT, h ^ 1);
+        interleave<MT * NT * P * BT / 16, (MT * P + NT) * BT / 8>();
+        store(w, h ^ 1);
         __syncthreads();
       }
     }
@@ -264,14 +330,16 @@ struct WgradPlan {
   int tile;
   int64_t tiles_m, tiles_n, splits;
 };
-static WgradPlan wgrad_plan(int64_t n, int64_t N, int64_t K) {
+static WgradPlan wgrad_plan(int64_t n, int64_t N, int64_t K, int type) {
   const auto tiles = [](int64_t x, int64_t t) { return (x + t - 1) / t; };
-  if (N >= 8 && K >= 8 && tiles(N, 256) * tiles(K, 256) >= 192) return {256, tiles(N, 256), tiles(K, 256), 1};
+  if (type == ELR_BF16 && tiles(N, 256) * tiles(K, 256) >= 192) return {256, tiles(N, 256), tiles(K, 256), 1};
   const int64_t m = tiles(N, 128), k = tiles(K, 128), most = n / 256 < 64 ? n / 256 : 64;
   int64_t s = 512 / (m * k);
   s = s > most ? most : s;
   return {128, m, k, s < 1 ? 1 : s};
 }
+
+constexpr int64_t kNearRows = 1 << 24;      // strides of rows whose 32 lie within 32-bit offsets
 
 template <class E, int B>
 constexpr int kWgradLds = 2 * (kParts<E> + 1) * 32 * (B + 32) * 2;
@@ -285,10 +353,11 @@ static void launch_wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st)
 
 template <class E>
 static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
-  if (a.N < 8 || a.K < 8)
+  if (a.N < 8 || a.K < 8 || a.dy_ld > kNearRows || a.q_ld > kNearRows)
     k_wgrad<E, 128, 128, 2, 2, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128>, st>>>(
         a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
-  else if (p.tile == 256) launch_wgrad<E, 256, 2, 4>(a, p, st);
+  else if constexpr (kParts<E> == 1)
+    p.tile == 256 ? launch_wgrad<E, 256, 2, 4>(a, p, st) : launch_wgrad<E, 128, 2, 2>(a, p, st);
   else launch_wgrad<E, 128, 2, 2>(a, p, st);
 }
 
@@ -297,7 +366,7 @@ static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
 extern "C" int64_t elr_int8_weight_grad_scratch_bytes(int64_t n, int64_t N, int64_t K, int type) {
   if (n < 0 || N < 0 || K < 0 || !elr::elem_type_ok(type)) return -1;
   if (N == 0 || K == 0) return 0;
-  const int64_t s = elr::wgrad_plan(n, N, K).splits;
+  const int64_t s = elr::wgrad_plan(n, N, K, type).splits;
   return s > 1 ? s * N * K * 4 : 0;
 }
 
@@ -310,7 +379,7 @@ extern "C" int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t
   if (N == 0 || K == 0) return ELR_OK;
   if (!dw || ((uintptr_t)dw & 3u) || (n > 0 && (!dy || !q || !scale || !elem_aligned(dy, type) || ((uintptr_t)scale & 3u))))
     return ELR_EINVAL;
-  const WgradPlan plan = wgrad_plan(n, N, K);
+  const WgradPlan plan = wgrad_plan(n, N, K, type);
   const int64_t splits = plan.splits;
   if (splits > 1 && (!scratch || scratch_bytes < splits * N * K * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const WgradArgs a{dy, q, scale, dy_ld, q_ld, n, ((n + splits - 1) / splits + 31) / 32 * 32, (int32_t)N, (int32_t)K,
