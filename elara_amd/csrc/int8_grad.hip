@@ -79,18 +79,19 @@ __device__ __forceinline__ Row8<E> load8(const E* p, int64_t valid) {
   return r;
 }
 
-// Order of a step: half of the reads of operands, then between any two products some of the conversions for the next step (the matrix
-// unit works on a product for 32 cycles, of which its issue takes 4) and the rest of the reads.
-template <int PRODUCTS, int READS>
+// Order of half a step: the first reads of operands, then between any two products some of the conversions for the next step (the matrix
+// unit works on a product for 32 cycles, of which its issue takes 4) and of the remaining reads.
+template <int PRODUCTS, int READS, int VALU>
 __device__ __forceinline__ void interleave() {
   constexpr int kVmem = 0x20, kMfma = 0x8, kValu = 0x2, kRead = 0x100;
+  constexpr int kFirst = READS / 2 < 12 ? READS / 2 : 12, kEach = (READS - kFirst + PRODUCTS - 1) / PRODUCTS;
   __builtin_amdgcn_sched_group_barrier(kVmem, 64, 0);
-  __builtin_amdgcn_sched_group_barrier(kRead, READS / 2, 0);
+  __builtin_amdgcn_sched_group_barrier(kRead, kFirst, 0);
 #pragma unroll
   for (int i = 0; i < PRODUCTS; ++i) {
     __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
-    __builtin_amdgcn_sched_group_barrier(kRead, (READS + PRODUCTS - 1) / PRODUCTS, 0);
+    if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(kValu, VALU, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, kEach, 0);
   }
 }
 
@@ -102,9 +103,9 @@ __device__ __forceinline__ void interleave() {
 // within is loaded from 8 columns before the end on, and its own columns are then stored again in their place; pieces past the end are
 // loaded from there too: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
 // NARROW: a matrix of less than 8 columns, or with rows far apart, loaded with checks.
-template <class E, int BM, int BN, int WM, int WN, bool NARROW>
+template <class E, int BM, int BN, int BT, int WM, int WN, bool NARROW>
 __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
-  constexpr int P = kParts<E>, T = WM * WN * 64, BT = 32, PM = BM + 32, PN = BN + 32;
+  constexpr int P = kParts<E>, T = WM * WN * 64, PM = BM + 32, PN = BN + 32;
   constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
   constexpr int RY = BT * BM / 8 / T, RX = BT * BN / 8 / T;       // row pieces of 8 of a thread
   static_assert(RY >= 1 && RX >= 1 && RY * T * 8 == BT * BM && RX * T * 8 == BT * BN, "whole pieces");
@@ -254,9 +255,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
   };
   // this lane's place in a 16 x 32 block of tokens and columns
   const int tr = (lane >> 5) * 8 + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-  const auto multiply = [&](int buf) {
+  const auto multiply = [&](int buf, int half) {
 #pragma unroll
-    for (int h = 0; h < BT / 16; ++h) {
+    for (int h = half * (BT / 32); h < (half + 1) * (BT / 32); ++h) {
       bf16x8 fx[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) fx[j] = tokens_of(lx + (buf * BT + h * 16 + tr) * PN + wn + j * 32 + tc, PN);
@@ -273,21 +274,21 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
     }
   };
   if (from < to) {
-    Step g[2];
-    load(g[0], 0);
-    load(g[1], BT);
-    store(convert(g[0], 0), 0);
+    Step g;
+    load(g, 0);
+    store(convert(g, 0), 0);
     __syncthreads();
-    for (int32_t i = 0; i <= last; i += 2 * BT) {      // (a second half past the end multiplies zeros)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        load(g[h], i + (h + 2) * BT);
-        const Rows w = convert(g[h ^ 1], i + (h + 1) * BT);
-        multiply(h);
-        interleave<MT * NT * P * BT / 16, (MT * P + NT) * BT / 8>();
-        store(w, h ^ 1);
-        __syncthreads();
-      }
+    constexpr int kProducts = MT * NT * P * BT / 32, kReads = (MT * P + NT) * BT / 16;      // of half a step
+    int buf = 0;
+    for (int32_t i = 0; i <= last; i += BT, buf ^= 1) {
+      load(g, i + BT);
+      multiply(buf, 0);
+      interleave<kProducts, kReads, 0>();
+      const Rows w = convert(g, i + BT);
+      multiply(buf, 1);
+      interleave<kProducts, kReads, (RX * 28 + (P > 1 ? RY * 16 * P : 0) + kProducts - 1) / kProducts>();
+      store(w, buf ^ 1);
+      __syncthreads();
     }
   }
   float* out = a.out + (int64_t)blockIdx.z * a.N * a.K;
@@ -341,24 +342,24 @@ static WgradPlan wgrad_plan(int64_t n, int64_t N, int64_t K, int type) {
 
 constexpr int64_t kNearRows = 1 << 24;      // strides of rows whose 32 lie within 32-bit offsets
 
-template <class E, int B>
-constexpr int kWgradLds = 2 * (kParts<E> + 1) * 32 * (B + 32) * 2;
+template <class E, int B, int BT>
+constexpr int kWgradLds = 2 * (kParts<E> + 1) * BT * (B + 32) * 2;
 
-template <class E, int B, int WM, int WN>
+template <class E, int B, int BT, int WM, int WN>
 static void launch_wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
-  static_assert(kWgradLds<E, B> <= 160 << 10, "LDS of a CU");
+  static_assert(kWgradLds<E, B, BT> <= 160 << 10, "LDS of a CU");
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits);
-  k_wgrad<E, B, B, WM, WN, false><<<grid, WM * WN * 64, kWgradLds<E, B>, st>>>(a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
+  k_wgrad<E, B, B, BT, WM, WN, false><<<grid, WM * WN * 64, kWgradLds<E, B, BT>, st>>>(a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
 }
 
 template <class E>
 static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
   if (a.N < 8 || a.K < 8 || a.dy_ld > kNearRows || a.q_ld > kNearRows)
-    k_wgrad<E, 128, 128, 2, 2, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128>, st>>>(
+    k_wgrad<E, 128, 128, 32, 2, 2, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128, 32>, st>>>(
         a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
   else if constexpr (kParts<E> == 1)
-    p.tile == 256 ? launch_wgrad<E, 256, 2, 4>(a, p, st) : launch_wgrad<E, 128, 2, 2>(a, p, st);
-  else launch_wgrad<E, 128, 2, 2>(a, p, st);
+    p.tile == 256 ? launch_wgrad<E, 256, 64, 2, 4>(a, p, st) : launch_wgrad<E, 128, 32, 2, 2>(a, p, st);
+  else launch_wgrad<E, 128, 32, 2, 2>(a, p, st);
 }
 
 }  // namespace elr
