@@ -30,6 +30,13 @@ __device__ __forceinline__ u32x4 load_k(const int8_t* row, int32_t k, int32_t K)
   return r;
 }
 
+// 16 bytes a lane from p into LDS, one lane's after the other's from `to` (the same in the wave) on; loads_done waits for them.
+__device__ __forceinline__ void to_lds(const int8_t* p, int8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)to, 16,
+                                   0, 0);
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <class O>
 __device__ __forceinline__ O scaled(int32_t acc, float sx, float sw) {
   return (O)((float)acc * sx * sw);
@@ -96,7 +103,114 @@ __global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
   }
 }
 
+// The tile of a block.  Blocks go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets a compact part of the tiles, bands of 8 rows
+// of tiles one column after another, so that its blocks share rows of both operands.
+__device__ __forceinline__ int64_t tile_of(uint32_t b, uint32_t tiles_m, uint32_t tiles_n, uint32_t& n) {
+  const uint32_t count = tiles_m * tiles_n, full = count / 8 * 8;
+  const uint32_t i = b < full ? b % 8 * (count / 8) + b / 8 : b;
+  const uint32_t band = 8 * tiles_n, first = i / band * 8;
+  const uint32_t rows = tiles_m - first < 8 ? tiles_m - first : 8, in = i % band;
+  n = in / rows;
+  return first + in % rows;
+}
+
+// What rows past an end are read from, in pieces of 16 bytes.
+__device__ const u32x4 kZeros = {0, 0, 0, 0};
+
+// Tiles of BM x BN, 128 bytes of K a step, two LDS buffers.  The rows come straight from memory into LDS, 16 bytes a lane, for the next
+// step while this one is multiplied; WM x WN waves, each a part of the tile in products of 32 x 32 x 32.
+// A wave's load fills 8 rows of 128 bytes.  Piece c of row r lies in place c ^ (r / 2 % 8) of its row in LDS, so that the 16 lanes that read
+// a piece of 16 rows at a time find them in different banks (r % 8 instead: half of LDS's cycles were conflicts).  Rows past an end repeat the last (their outputs are not stored); pieces past K
+// are read from zeros.  Rows and strides are multiples of 16 bytes.
+template <class O, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
+  constexpr int W = WM * WN, BK = 128, MT = BM / WM / 32, NT = BN / WN / 32;
+  constexpr int LX = BM / 8 / W, LW = BN / 8 / W;          // loads of a wave for each operand
+  extern __shared__ __attribute__((aligned(16))) int8_t tile_lds[];    // [2][BM + BN][BK]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t tn;
+  const int64_t m0 = tile_of(blockIdx.x, tiles_m, tiles_n, tn) * BM, n0 = (int64_t)tn * BN;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  i32x16 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = i32x16{};
+  static_assert(W % 2 == 0, "a wave's rows: 8 of 16");
+  const int piece = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;      // this lane's piece of the row that it loads
+  const int8_t *const x = a.x + m0 * a.x_ld, *const w = a.w + n0 * a.w_ld;
+  uint32_t ox[LX], ow[LW];                                  // its rows' places behind these
+#pragma unroll
+  for (int l = 0; l < LX; ++l) {
+    const int64_t r = (l * W + wave) * 8 + (lane >> 3);
+    ox[l] = (uint32_t)((m0 + r < a.n ? r : a.n - 1 - m0) * a.x_ld) + piece;
+  }
+#pragma unroll
+  for (int l = 0; l < LW; ++l) {
+    const int64_t r = (l * W + wave) * 8 + (lane >> 3);
+    ow[l] = (uint32_t)((n0 + r < a.N ? r : a.N - 1 - n0) * a.w_ld) + piece;
+  }
+  const auto load = [&](int32_t k, int buf) {
+    int8_t* const to = tile_lds + buf * (BM + BN) * BK + wave * 8 * BK;
+    if (k + BK <= a.K) {
+#pragma unroll
+      for (int l = 0; l < LX; ++l) to_lds(x + k + ox[l], to + l * W * 8 * BK);
+#pragma unroll
+      for (int l = 0; l < LW; ++l) to_lds(w + k + ow[l], to + (BM + l * W * 8) * BK);
+    } else {
+      const uintptr_t in = k + piece < a.K ? ~(uintptr_t)0 : 0, zeros = (uintptr_t)&kZeros & ~in;
+#pragma unroll
+      for (int l = 0; l < LX; ++l) to_lds((const int8_t*)(((uintptr_t)(x + k + ox[l]) & in) | zeros), to + l * W * 8 * BK);
+#pragma unroll
+      for (int l = 0; l < LW; ++l)
+        to_lds((const int8_t*)(((uintptr_t)(w + k + ow[l]) & in) | zeros), to + (BM + l * W * 8) * BK);
+    }
+  };
+  load(0, 0);
+  int buf = 0;
+  for (int32_t k = 0; k < a.K; k += BK, buf ^= 1) {
+    loads_done();
+    __syncthreads();
+    if (k + BK < a.K) load(k + BK, buf ^ 1);
+    const int8_t* const from = tile_lds + buf * (BM + BN) * BK + (lane & 31) * BK;
+#pragma unroll
+    for (int q = 0; q < BK / 32; ++q) {
+      const int at = ((q * 2 + (lane >> 5)) ^ (lane >> 1 & 7)) * 16;
+      i32x4 fx[MT], fw[NT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4*>(from + (wm + i * 32) * BK + at);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fw[j] = *reinterpret_cast<const i32x4*>(from + (BM + wn + j * 32) * BK + at);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
+    }
+    // the first operands, then one of the next ones' reads behind each product
+    __builtin_amdgcn_sched_group_barrier(0x100, MT + NT, 0);
+#pragma unroll
+    for (int q = 0; q < BK / 32 * MT * NT; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t col = n0 + wn + j * 32 + (lane & 31);
+    const float sw = col < a.N ? a.w_scale[col] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int64_t row = m0 + wm + i * 32 + (q >> 2) * 8 + (lane >> 5) * 4 + (q & 3);
+        if (row < a.n && col < a.N) ((O*)a.y)[row * a.N + col] = scaled<O>(acc[i][j][q], a.x_scale[row], sw);
+      }
+  }
+}
+
 // ---- host side
+
+constexpr int64_t kNearRows = 1 << 23;      // strides of rows whose 256 lie within 32-bit offsets
 
 template <class O>
 static void linear(const LinearArgs& b, hipStream_t st) {
@@ -105,8 +219,21 @@ static void linear(const LinearArgs& b, hipStream_t st) {
     LinearArgs a = b;
     a.n = b.n - r < kRows ? b.n - r : kRows;
     a.x = b.x + r * b.x_ld, a.x_scale = b.x_scale + r, a.y = (O*)b.y + r * b.N;
-    if (a.n <= 64) k_linear<O, 64, 128><<<dim3((unsigned)((a.N + 127) / 128), 1), 256, 0, st>>>(a);
-    else k_linear<O, 128, 128><<<dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.n + 127) / 128)), 256, 0, st>>>(a);
+    const bool whole = a.K % 16 == 0 && a.K > 0 && (a.x_ld | a.w_ld) % 16 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15u) == 0 &&
+                       a.x_ld <= kNearRows && a.w_ld <= kNearRows;
+    const auto tiles = [](int64_t x, int64_t t) { return (unsigned)((x + t - 1) / t); };
+    if (whole && a.n > 64) {
+      if (tiles(a.n, 256) * (uint64_t)tiles(a.N, 256) >= 192)
+        k_linear_tiles<O, 256, 256, 2, 4><<<tiles(a.n, 256) * tiles(a.N, 256), 512, 2 * 512 * 128, st>>>(a, tiles(a.n, 256),
+                                                                                                         tiles(a.N, 256));
+      else
+        k_linear_tiles<O, 128, 128, 2, 2><<<tiles(a.n, 128) * tiles(a.N, 128), 256, 2 * 256 * 128, st>>>(a, tiles(a.n, 128),
+                                                                                                         tiles(a.N, 128));
+    } else if (a.n <= 64) {
+      k_linear<O, 64, 128><<<dim3(tiles(a.N, 128), 1), 256, 0, st>>>(a);
+    } else {
+      k_linear<O, 128, 128><<<dim3(tiles(a.N, 128), tiles(a.n, 128)), 256, 0, st>>>(a);
+    }
   }
 }
 
