@@ -37,17 +37,71 @@ __device__ __forceinline__ void to_lds(const int8_t* p, int8_t* to) {
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// What a wave's lanes wrote to LDS before is there for its own reads after.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <class O>
 __device__ __forceinline__ O scaled(int32_t acc, float sx, float sw) {
   return (O)((float)acc * sx * sw);
 }
+
+// A wave's outputs, MT x NT blocks of 32 tokens (a lane each) x 32 channels (four neighbouring ones a register quad), scaled and stored.
+// They pass through LDS, 32 tokens at a time in a part of the wave's own, so that memory gets rows of NT * 32 channels in pieces of 16 bytes
+// (stored from the registers, two bytes a lane, 8,192 x 16,384 outputs took 150 us longer than their bytes).
+template <class O, int MT, int NT>
+struct Outputs {
+  static constexpr int kRow = NT * 32 * (int)sizeof(O) + 16, kBytes = 32 * kRow;      // LDS of a wave
+  __device__ static __forceinline__ void store(const LinearArgs& a, int64_t m0, int64_t n0, const i32x16 (&acc)[MT][NT], int8_t* lds) {
+    constexpr int VO = 16 / (int)sizeof(O), PIECES = NT * 32 / VO;    // outputs of a piece, pieces of a row
+    typedef O O4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, ch = (lane >> 5) * 4;
+    f32x4 sw[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t c = n0 + j * 32 + q * 8 + ch;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sw[j][q][t] = a.w_scale[c + t < a.N ? c + t : a.N - 1];
+      }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t row = m0 + i * 32 + (lane & 31);
+      const float sx = a.x_scale[row < a.n ? row : a.n - 1];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          O4 v;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) v[t] = scaled<O>(acc[i][j][4 * q + t], sx, sw[j][q][t]);
+          *reinterpret_cast<O4*>(lds + (lane & 31) * kRow + (j * 32 + q * 8 + ch) * (int)sizeof(O)) = v;
+        }
+      wave_lds();
+#pragma unroll
+      for (int p = 0; p < 32 * PIECES / 64; ++p) {
+        const int at = p * 64 + lane, r = at / PIECES, c = at % PIECES * VO;
+        const int64_t to = m0 + i * 32 + r;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * kRow + c * (int)sizeof(O));
+        if (to < a.n) store_raw<O, false>((O*)a.y + to * a.N + n0 + c, v, a.N - n0 - c);
+      }
+      wave_lds();
+    }
+  }
+};
 
 // Tiles of BM tokens x BN channels, 64 bytes of K at a time through LDS; four waves, each a quarter of the tile in matrix instructions of
 // 32 x 32 x 32.  Rows of any alignment.
 template <class O, int BM, int BN>
 __global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
   constexpr int PITCH = 80, MT = BM / 64, NT = BN / 64;
-  __shared__ __attribute__((aligned(16))) uint8_t lx[BM * PITCH], lw[BN * PITCH];
+  constexpr int kTile = (BM + BN) * PITCH, kOut = 4 * Outputs<O, MT, NT>::kBytes;
+  __shared__ __attribute__((aligned(16))) int8_t lds[kTile > kOut ? kTile : kOut];
+  int8_t *const lx = lds, *const lw = lds + BM * PITCH;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m0 = (int64_t)blockIdx.y * BM, n0 = (int64_t)blockIdx.x * BN;
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
@@ -86,21 +140,11 @@ __global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
     }
   }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t col = n0 + wn + j * 32 + (lane & 31);
-    const float sw = col < a.N ? a.w_scale[col] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int64_t row = m0 + wm + i * 32 + (q >> 2) * 8 + (lane >> 5) * 4 + (q & 3);
-        if (row < a.n && col < a.N) ((O*)a.y)[row * a.N + col] = scaled<O>(acc[i][j][q], a.x_scale[row], sw);
-      }
-  }
+  __syncthreads();
+  Outputs<O, MT, NT>::store(a, m0 + wm, n0 + wn, acc, lds + wave * Outputs<O, MT, NT>::kBytes);
 }
 
 // The tile of a block.  Blocks go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets a compact part of the tiles, bands of 8 rows
@@ -126,6 +170,7 @@ template <class O, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr int W = WM * WN, BK = 128, MT = BM / WM / 32, NT = BN / WN / 32;
   constexpr int LX = BM / 8 / W, LW = BN / 8 / W;          // loads of a wave for each operand
+  static_assert(W * Outputs<O, MT, NT>::kBytes <= 2 * (BM + BN) * BK, "the outputs' LDS");
   extern __shared__ __attribute__((aligned(16))) int8_t tile_lds[];    // [2][BM + BN][BK]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t tn;
@@ -184,7 +229,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uin
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
     }
     // the first operands, then one of the next ones' reads behind each product
     __builtin_amdgcn_sched_group_barrier(0x100, MT + NT, 0);
@@ -194,18 +239,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uin
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
   }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t col = n0 + wn + j * 32 + (lane & 31);
-    const float sw = col < a.N ? a.w_scale[col] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int64_t row = m0 + wm + i * 32 + (q >> 2) * 8 + (lane >> 5) * 4 + (q & 3);
-        if (row < a.n && col < a.N) ((O*)a.y)[row * a.N + col] = scaled<O>(acc[i][j][q], a.x_scale[row], sw);
-      }
-  }
+  __syncthreads();
+  Outputs<O, MT, NT>::store(a, m0 + wm, n0 + wn, acc, tile_lds + wave * Outputs<O, MT, NT>::kBytes);
 }
 
 // ---- host side
