@@ -20,22 +20,31 @@ struct LinearArgs {
   void* y;
 };
 
-// 16 bytes of a row at k, of which those up to K may be read; the rest are 0.
+// 16 bytes of a row at k, of which those up to K may be read; the rest are 0.  A row's end: its last 16 bytes, shifted (no branch, no
+// loads byte by byte but for rows of less than 16).
 __device__ __forceinline__ u32x4 load_k(const int8_t* row, int32_t k, int32_t K) {
-  if (k + 16 <= K) return *reinterpret_cast<const u32x4_b*>(row + k);
+  if (K >= 16) {
+    const int32_t at = k < K - 16 ? k : K - 16, s = k - at;
+    const unsigned __int128 v = __builtin_bit_cast(unsigned __int128, *reinterpret_cast<const u32x4_b*>(row + at));
+    return __builtin_bit_cast(u32x4, s < 16 ? v >> (8 * s) : (unsigned __int128)0);
+  }
   u32x4 r{0, 0, 0, 0};
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < 15; ++j)
     if (k + j < K) r[j / 4] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j & 3));
   return r;
 }
 
-// 16 bytes a lane from p into LDS, one lane's after the other's from `to` (the same in the wave) on; loads_done waits for them.
+// 16 bytes a lane from p into LDS, one lane's after the other's from `to` (the same in the wave) on; loads_done waits for all
+// but the LATER last of them.
 __device__ __forceinline__ void to_lds(const int8_t* p, int8_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)to, 16,
                                    0, 0);
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void loads_done() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+}
 
 // What a wave's lanes wrote to LDS before is there for its own reads after.
 __device__ __forceinline__ void wave_lds() {
@@ -94,14 +103,14 @@ struct Outputs {
   }
 };
 
-// Tiles of BM tokens x BN channels, 64 bytes of K at a time through LDS; four waves, each a quarter of the tile in matrix instructions of
-// 32 x 32 x 32.  Rows of any alignment.
+// Tiles of BM tokens x BN channels for rows of any alignment, 128 bytes of K a step, two LDS buffers; the next step's rows are on their
+// way into registers while this one is multiplied.  Four waves, each a quarter of the tile in products of 32 x 32 x 32.  Rows past an end repeat
+// the last (their outputs are not stored).
 template <class O, int BM, int BN>
 __global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
-  constexpr int PITCH = 80, MT = BM / 64, NT = BN / 64;
+  constexpr int BK = 128, PITCH = BK + 16, MT = BM / 64, NT = BN / 64;
   constexpr int kTile = (BM + BN) * PITCH, kOut = 4 * Outputs<O, MT, NT>::kBytes;
-  __shared__ __attribute__((aligned(16))) int8_t lds[kTile > kOut ? kTile : kOut];
-  int8_t *const lx = lds, *const lw = lds + BM * PITCH;
+  __shared__ __attribute__((aligned(16))) int8_t lds[2 * kTile > kOut ? 2 * kTile : kOut];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m0 = (int64_t)blockIdx.y * BM, n0 = (int64_t)blockIdx.x * BN;
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
@@ -110,41 +119,137 @@ __global__ __launch_bounds__(256) void k_linear(LinearArgs a) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = i32x16{};
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-  for (int32_t k = 0; k < a.K; k += 64) {
-    u32x4 gx[MT], gw[NT];
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 16;
+  constexpr int LX = BM / 32, LW = BN / 32;
+  const int8_t* p[LX + LW];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int64_t row = m0 + r + i * 64;
-      gx[i] = row < a.n ? load_k(a.x + row * a.x_ld, k + c, a.K) : u32x4{0, 0, 0, 0};
+  for (int i = 0; i < LX; ++i) p[i] = a.x + (m0 + r + i * 32 < a.n ? m0 + r + i * 32 : a.n - 1) * a.x_ld;
+#pragma unroll
+  for (int j = 0; j < LW; ++j) p[LX + j] = a.w + (n0 + r + j * 32 < a.N ? n0 + r + j * 32 : a.N - 1) * a.w_ld;
+  u32x4 g[LX + LW];
+  const auto load = [&](int32_t k) {
+    if (k + BK <= a.K) {
+#pragma unroll
+      for (int i = 0; i < LX + LW; ++i) g[i] = *reinterpret_cast<const u32x4_b*>(p[i] + k + c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LX + LW; ++i) g[i] = load_k(p[i], k + c, a.K);
     }
+  };
+  const auto store = [&](int8_t* to) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t row = n0 + r + j * 64;
-      gw[j] = row < a.N ? load_k(a.w + row * a.w_ld, k + c, a.K) : u32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < LX + LW; ++i) *reinterpret_cast<u32x4*>(to + (r + i * 32) * PITCH + c) = g[i];
+  };
+  load(0);
+  store(lds);
+  int8_t* buf = lds;
+  for (int32_t k = 0; k < a.K; k += BK) {
     __syncthreads();
+    const bool more = k + BK < a.K;
+    if (more) load(k + BK);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) *reinterpret_cast<u32x4*>(lx + (r + i * 64) * PITCH + c) = gx[i];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) *reinterpret_cast<u32x4*>(lw + (r + j * 64) * PITCH + c) = gw[j];
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < BK / 32; ++q) {
       i32x4 fx[MT], fw[NT];
-      const int at = (lane & 31) * PITCH + q * 32 + (lane >> 5) * 16;
+      const int8_t* const at = buf + (lane & 31) * PITCH + q * 32 + (lane >> 5) * 16;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4*>(lx + (wm + i * 32) * PITCH + at);
+      for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4*>(at + (wm + i * 32) * PITCH);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fw[j] = *reinterpret_cast<const i32x4*>(lw + (wn + j * 32) * PITCH + at);
+      for (int j = 0; j < NT; ++j) fw[j] = *reinterpret_cast<const i32x4*>(at + (BM + wn + j * 32) * PITCH);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
     }
+    buf = buf == lds ? lds + kTile : lds;
+    if (more) store(buf);
   }
   __syncthreads();
   Outputs<O, MT, NT>::store(a, m0 + wm, n0 + wn, acc, lds + wave * Outputs<O, MT, NT>::kBytes);
+}
+
+// Few tokens (16 TB at most): the weight is read once, straight into registers, and there are no tiles to share.  Eight waves a block: `kw` of
+// them take turns at 64 U bytes of K for the same 16 C channels, the others take further channels; the weight's rows are the products'
+// first operand (16 x 16 x 64), so that a lane holds four neighbouring channels of a token.  The waves' sums, of whole numbers, are added in
+// LDS.  Rows of any alignment; those past an end repeat the last.
+template <class O, int TB, int C>
+__global__ __launch_bounds__(512) void k_linear_few(LinearArgs a, int32_t kw) {
+  constexpr int U = 8 / C;                       // steps of K in flight
+  __shared__ __attribute__((aligned(16))) int32_t sums[8 * 16 * C * 16 * TB];      // [channels of the block][16 TB]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int group = wave / kw, channels = 16 * C * (8 / kw);
+  const int64_t n0 = (int64_t)blockIdx.x * channels;
+  for (int i = threadIdx.x; i < channels * 16 * TB; i += 512) sums[i] = 0;
+  __syncthreads();
+  const int32_t c = (lane >> 4) * 16;
+  const int8_t *pw[C], *px[TB];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int64_t row = n0 + group * 16 * C + i * 16 + (lane & 15);
+    pw[i] = a.w + (row < a.N ? row : a.N - 1) * a.w_ld + c;
+  }
+#pragma unroll
+  for (int t = 0; t < TB; ++t) px[t] = a.x + (t * 16 + (lane & 15) < a.n ? t * 16 + (lane & 15) : a.n - 1) * a.x_ld + c;
+  i32x4 acc[C][TB];
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+#pragma unroll
+    for (int t = 0; t < TB; ++t) acc[i][t] = i32x4{0, 0, 0, 0};
+  const auto multiply = [&](const i32x4 (&w)[C], const i32x4 (&x)[TB]) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[t], acc[i][t], 0, 0, 0);
+  };
+  for (int32_t k = wave % kw * U * 64; k < a.K; k += kw * U * 64) {
+    if (k + U * 64 <= a.K) {
+      i32x4 w[U][C], x[U][TB];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[u][i] = __builtin_bit_cast(i32x4, __builtin_nontemporal_load((const u32x4_b*)(pw[i] + k + u * 64)));
+#pragma unroll
+        for (int t = 0; t < TB; ++t) x[u][t] = __builtin_bit_cast(i32x4, *(const u32x4_b*)(px[t] + k + u * 64));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) multiply(w[u], x[u]);
+    } else {
+      for (int32_t e = k; e < a.K; e += 64) {
+        i32x4 w[C], x[TB];
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[i] = __builtin_bit_cast(i32x4, load_k(pw[i] - c, e + c, a.K));
+#pragma unroll
+        for (int t = 0; t < TB; ++t) x[t] = __builtin_bit_cast(i32x4, load_k(px[t] - c, e + c, a.K));
+        multiply(w, x);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        atomicAdd(&sums[(t * 16 + (lane & 15)) * channels + group * 16 * C + i * 16 + (lane >> 4) * 4 + q], acc[i][t][q]);
+  __syncthreads();
+  typedef O O4 __attribute__((ext_vector_type(4)));
+  typedef O4 O4_u __attribute__((aligned(sizeof(O))));
+  for (int i = threadIdx.x; i < 16 * TB * channels / 4; i += 512) {
+    const int row = i / (channels / 4), ch = i % (channels / 4) * 4;
+    const int64_t col = n0 + ch;
+    if (row >= a.n || col >= a.N) continue;
+    const float sx = a.x_scale[row];
+    O* y = (O*)a.y + row * a.N + col;
+    O4 v;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = scaled<O>(sums[row * channels + ch + q], sx, a.w_scale[col + q < a.N ? col + q : a.N - 1]);
+    if (col + 4 <= a.N) {
+      *reinterpret_cast<O4_u*>(y) = v;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        if (col + q < a.N) y[q] = v[q];
+    }
+  }
 }
 
 // The tile of a block.  Blocks go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets a compact part of the tiles, bands of 8 rows
@@ -161,17 +266,17 @@ __device__ __forceinline__ int64_t tile_of(uint32_t b, uint32_t tiles_m, uint32_
 // What rows past an end are read from, in pieces of 16 bytes.
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
-// Tiles of BM x BN, 128 bytes of K a step, two LDS buffers.  The rows come straight from memory into LDS, 16 bytes a lane, for the next
-// step while this one is multiplied; WM x WN waves, each a part of the tile in products of 32 x 32 x 32.
+// Tiles of BM x BN, 128 bytes of K a step, NB LDS buffers.  The rows come straight from memory into LDS, 16 bytes a lane, NB - 1 steps ahead
+// of the one that is multiplied; WM x WN waves, each a part of the tile in products of 32 x 32 x 32.
 // A wave's load fills 8 rows of 128 bytes.  Piece c of row r lies in place c ^ (r / 2 % 8) of its row in LDS, so that the 16 lanes that read
 // a piece of 16 rows at a time find them in different banks (r % 8 instead: half of LDS's cycles were conflicts).  Rows past an end repeat the last (their outputs are not stored); pieces past K
 // are read from zeros.  Rows and strides are multiples of 16 bytes.
-template <class O, int BM, int BN, int WM, int WN>
+template <class O, int BM, int BN, int WM, int WN, int NB>
 __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
   constexpr int W = WM * WN, BK = 128, MT = BM / WM / 32, NT = BN / WN / 32;
   constexpr int LX = BM / 8 / W, LW = BN / 8 / W;          // loads of a wave for each operand
-  static_assert(W * Outputs<O, MT, NT>::kBytes <= 2 * (BM + BN) * BK, "the outputs' LDS");
-  extern __shared__ __attribute__((aligned(16))) int8_t tile_lds[];    // [2][BM + BN][BK]
+  static_assert(W * Outputs<O, MT, NT>::kBytes <= NB * (BM + BN) * BK, "the outputs' LDS");
+  extern __shared__ __attribute__((aligned(16))) int8_t tile_lds[];    // [NB][BM + BN][BK]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t tn;
   const int64_t m0 = tile_of(blockIdx.x, tiles_m, tiles_n, tn) * BM, n0 = (int64_t)tn * BN;
@@ -211,12 +316,13 @@ __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uin
         to_lds((const int8_t*)(((uintptr_t)(w + k + ow[l]) & in) | zeros), to + (BM + l * W * 8) * BK);
     }
   };
-  load(0, 0);
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) load(i * BK, i);
   int buf = 0;
-  for (int32_t k = 0; k < a.K; k += BK, buf ^= 1) {
-    loads_done();
+  for (int32_t k = 0; k < a.K; k += BK, buf = buf + 1 < NB ? buf + 1 : 0) {
+    loads_done<(NB - 2) * (LX + LW)>();          // this step's
     __syncthreads();
-    if (k + BK < a.K) load(k + BK, buf ^ 1);
+    if (NB > 2 || k + BK < a.K) load(k + (NB - 1) * BK, buf > 0 ? buf - 1 : NB - 1);     // (past K zeros: the wait above counts loads)
     const int8_t* const from = tile_lds + buf * (BM + BN) * BK + (lane & 31) * BK;
 #pragma unroll
     for (int q = 0; q < BK / 32; ++q) {
@@ -245,7 +351,24 @@ __global__ __launch_bounds__(WM * WN * 64) void k_linear_tiles(LinearArgs a, uin
 
 // ---- host side
 
+// Few tokens: waves that share channels, so that each has a few steps of K; channels a wave.
+template <class O, int TB>
+static void few(const LinearArgs& a, hipStream_t st) {
+  int kw = 8;
+  while (kw > 1 && a.K < kw * 256) kw /= 2;
+  const auto blocks = [&](int c) { return (a.N + 16 * c * (8 / kw) - 1) / (16 * c * (8 / kw)); };
+  if (blocks(4 / TB) >= 512) k_linear_few<O, TB, 4 / TB><<<(unsigned)blocks(4 / TB), 512, 0, st>>>(a, kw);
+  else if (blocks(2 / TB) >= 512) k_linear_few<O, TB, 2 / TB><<<(unsigned)blocks(2 / TB), 512, 0, st>>>(a, kw);
+  else k_linear_few<O, TB, 1><<<(unsigned)blocks(1), 512, 0, st>>>(a, kw);
+}
+
 constexpr int64_t kNearRows = 1 << 23;      // strides of rows whose 256 lie within 32-bit offsets
+
+template <class O, int B, int WM, int WN, int NB>
+static void launch_tiles(const LinearArgs& a, hipStream_t st) {
+  const uint32_t m = (uint32_t)((a.n + B - 1) / B), n = (uint32_t)((a.N + B - 1) / B);
+  k_linear_tiles<O, B, B, WM, WN, NB><<<m * n, WM * WN * 64, NB * 2 * B * 128, st>>>(a, m, n);
+}
 
 template <class O>
 static void linear(const LinearArgs& b, hipStream_t st) {
@@ -257,13 +380,12 @@ static void linear(const LinearArgs& b, hipStream_t st) {
     const bool whole = a.K % 16 == 0 && a.K > 0 && (a.x_ld | a.w_ld) % 16 == 0 && (((uintptr_t)a.x | (uintptr_t)a.w) & 15u) == 0 &&
                        a.x_ld <= kNearRows && a.w_ld <= kNearRows;
     const auto tiles = [](int64_t x, int64_t t) { return (unsigned)((x + t - 1) / t); };
-    if (whole && a.n > 64) {
-      if (tiles(a.n, 256) * (uint64_t)tiles(a.N, 256) >= 192)
-        k_linear_tiles<O, 256, 256, 2, 4><<<tiles(a.n, 256) * tiles(a.N, 256), 512, 2 * 512 * 128, st>>>(a, tiles(a.n, 256),
-                                                                                                         tiles(a.N, 256));
-      else
-        k_linear_tiles<O, 128, 128, 2, 2><<<tiles(a.n, 128) * tiles(a.N, 128), 256, 2 * 256 * 128, st>>>(a, tiles(a.n, 128),
-                                                                                                         tiles(a.N, 128));
+    if (a.n <= 32) {
+      a.n <= 16 ? few<O, 1>(a, st) : few<O, 2>(a, st);
+    } else if (whole) {
+      if (tiles(a.n, 256) * (uint64_t)tiles(a.N, 256) >= 192) launch_tiles<O, 256, 2, 4, 2>(a, st);
+      else if (a.n > 64 && tiles(a.n, 128) * (uint64_t)tiles(a.N, 128) >= 256) launch_tiles<O, 128, 2, 2, 2>(a, st);
+      else launch_tiles<O, 64, 2, 2, 4>(a, st);
     } else if (a.n <= 64) {
       k_linear<O, 64, 128><<<dim3(tiles(a.N, 128), 1), 256, 0, st>>>(a);
     } else {
