@@ -15,8 +15,13 @@
 
 namespace elr {
 
-constexpr int kSegs = 1024;          // partial sums of a row in the order of ids
+typedef unsigned long long u64;
+
+constexpr int kSegs = 512;           // partial sums of a row in the order of ids
 constexpr int kDigit = 11;           // bits of a selection pass
+constexpr int kList = 512;           // candidates that are ranked among themselves
+constexpr int kBins = 1024;          // bins of a row by distance from its maximum, 1/16 of a factor 2 in e wide
+constexpr int kWeightBits = 51;      // of the largest weight
 
 struct SampleArgs {
   const void* x;
@@ -41,38 +46,77 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) >> (32 - kKeyBits<E>);
 }
+template <class E>
+__device__ __forceinline__ float value_of_key(uint32_t key) {
+  constexpr int kDrop = 32 - kKeyBits<E>;
+  const uint32_t o = key << kDrop;
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o >> kDrop << kDrop);
+}
 
+// 2^(z + shift) for z <= 0, rounded to an integer below 2^52.  2^f, |f| <= 1/2, by the polynomial through the ten Chebyshev points
+// (1.9e-14 of the value); the sum with 1.5 2^52 rounds z, the one with 2^52 the result.  About 20 instructions of fp64, which runs at
+// the rate of fp32 here; a NaN (0 times infinity: an infinite temperature) counts as no weight.
+__device__ __forceinline__ u64 weight_of(double z, int shift) {
+  constexpr double kRound = 0x1.8p52;
+  z = __builtin_fmax(z, -200.0);
+  const double t = z + kRound, f = z - (t - kRound);
+  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+  double p = 0x1.b6571d9fbc782p-24;
+  p = __builtin_fma(p, f, 0x1.63ef9699f65f0p-20);
+  p = __builtin_fma(p, f, 0x1.ffcb7678dfe12p-17);
+  p = __builtin_fma(p, f, 0x1.43088e257f900p-13);
+  p = __builtin_fma(p, f, 0x1.5d87fe908f6f7p-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab72b175e9p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08d704411ap-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_bit_cast(uint64_t, __builtin_ldexp(p, n + shift) + 0x1p52) & 0xFFFFFFFFFFFFFu;
+}
+
+struct Candidate {
+  u64 at;        // key in the high half, ~id in the low: larger comes first
+  u64 w;
+};
 struct SampleShared {
-  uint32_t count[1 << kDigit];
-  unsigned long long mass[1 << kDigit];
-  unsigned long long seg[kSegs];
+  union {
+    struct {
+      uint32_t count[1 << kDigit];
+      u64 mass[1 << kDigit];
+    } radix;
+    struct {
+      u64 mass[kBins];
+      uint32_t count[kBins];
+      Candidate list[kList];
+    } bins;
+  };
+  u64 seg[kSegs];
   float fmax[16];
-  uint32_t bin, bin_count;
-  unsigned long long above_count, above_mass, bin_mass;
-  unsigned long long total;
-  uint32_t id;
-  unsigned long long rest;
+  u64 sums[16];
+  uint32_t bin, bin_count, listed, bound;
+  u64 above, bin_mass, total, rest;
+  uint32_t id, thr, thr_id;
   int seg_at;
 };
 
-__device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long x) {
+__device__ __forceinline__ u64 wave_sum_u64(u64 x) {
   for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
   return x;
 }
 // Inclusive sums over the lanes.
-__device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long x, int lane) {
+__device__ __forceinline__ u64 wave_scan_u64(u64 x, int lane) {
   for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long y = __shfl_up(x, o, 64);
+    const u64 y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
   return x;
 }
 
-// One row by a block of T threads; every pass reads it again (from the caches).
-template <class E, int T>
+// One row by a block of T threads.  NV > 0: the row's vectors of a thread stay in registers for the search of candidates; the passes that
+// some rows need beyond it read the row again (from the caches).
+template <class E, int T, int NV>
 __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   constexpr int VE = Elem<E>::VE, W = T / 64;
-  typedef unsigned long long u64;
   __shared__ SampleShared sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
@@ -87,22 +131,37 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         f(s, (int)(e < a.V ? e : a.V), widen<E>(load_raw<E, false>(x + (e < a.V ? e : 0), a.V - e, kNone)));
       }
   };
-  // the row's maximum; NaN or +inf in the row show in it
-  float m = kNone;
-  each([&](int, int, const Frag<E>& f) {
+  // the row's maximum (NaN or +inf in the row show in it), and the thread's
+  u32x4 raw[NV > 0 ? NV : 1];
+  float own_max = kNone;
+  if constexpr (NV > 0) {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) m = max_nan(m, f.v[j]);
-  });
-  m = lanes_max_nan(m, 64);
-  if (lane == 0) sh.fmax[wave] = m;
-  __syncthreads();
+    for (int i = 0; i < NV; ++i) {
+      const int64_t e = ((int64_t)i * T + threadIdx.x) * VE;
+      raw[i] = load_raw<E, true>(x + (e < a.V ? e : 0), a.V - e, kNone);
+    }
 #pragma unroll
-  for (int i = 0; i < W; ++i) m = max_nan(m, sh.fmax[i]);
+    for (int i = 0; i < NV; ++i) {
+      const Frag<E> f = widen<E>(raw[i]);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) own_max = max_nan(own_max, f.v[j]);
+    }
+  } else {
+    each([&](int, int, const Frag<E>& f) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) own_max = max_nan(own_max, f.v[j]);
+    });
+  }
+  float m = lanes_max_nan(own_max, 64);
+  if constexpr (T > 64) {
+    if (lane == 0) sh.fmax[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max_nan(m, sh.fmax[i]);
+  }
   const double temp = a.temperature_rows ? (double)a.temperature_rows[row] : a.temperature;
   const double top_p = a.top_p_rows ? (double)a.top_p_rows[row] : a.top_p;
   const double min_p = a.min_p_rows ? (double)a.min_p_rows[row] : a.min_p;
-  const int64_t top_k = !a.top_k_rows ? a.top_k
-                        : a.top_k_64 ? ((const int64_t*)a.top_k_rows)[row] : ((const int32_t*)a.top_k_rows)[row];
   const double u = (double)a.u[row];
   if (!(m < __builtin_inff()) || !(temp >= 0.0) || u != u || m == kNone) {
     if (threadIdx.x == 0) {
@@ -112,17 +171,198 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     return;
   }
   const bool greedy = temp == 0.0;
-  const double inv_t = greedy ? 0.0 : 1.0 / temp, unit = __builtin_ldexp(1.0, a.shift);
-  const auto weight = [&](float v) -> u64 {
-    if (v == kNone) return 0;
-    return (u64)__builtin_rint(exp(((double)v - (double)m) * inv_t) * unit);
-  };
+  int64_t top_k = !a.top_k_rows ? a.top_k
+                  : a.top_k_64 ? ((const int64_t*)a.top_k_rows)[row] : ((const int32_t*)a.top_k_rows)[row];
+  if (greedy) top_k = 1;
+  const bool by_k = top_k > 0 && top_k < a.V, by_p = !greedy && top_p < 1.0;
+  const double inv_t = greedy ? 0.0 : 1.0 / temp, per_e = inv_t * 0x1.71547652b82fep+0;      // to powers of two
+  const auto weight = [&](float v) -> u64 { return weight_of(((double)v - (double)m) * per_e, a.shift); };
+  const double low = greedy || !(min_p > 0.0) ? -__builtin_inf() : log(min_p < 1.0 ? min_p : 1.0) * temp;
+  const auto near = [&](float v) { return !((double)v - (double)m < low); };
   uint32_t thr = 0, thr_id = 0xFFFFFFFFu;     // kept: a larger key, or this key and no larger id
   const auto in_order = [&](uint32_t key, uint32_t id) { return key > thr || (key == thr && id <= thr_id); };
 
-  // The first id at which the running sum of f over the ids exceeds t (t below the whole sum), and the sum before it; sh.total holds
-  // the whole sum when t_of is called.
+  // The sum of one value a thread; every thread gets it.
+  const auto block_sum = [&](u64 v) {
+    v = wave_sum_u64(v);
+    if constexpr (T == 64) return v;
+    __syncthreads();
+    if (lane == 0) sh.sums[wave] = v;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) all += sh.sums[i];
+    return all;
+  };
+  const auto share = [](double part, u64 all) {      // the least whole mass that reaches the part of `all`
+    const u64 t = (u64)__builtin_ceil((part > 0.0 ? part : 0.0) * (double)all);
+    return t < 1 ? (u64)1 : t > all ? all : t;
+  };
+  const auto place = [&](u64 all) {                  // u of `all`, below it
+    const u64 t = u > 0.0 ? (u64)__builtin_floor(u * (double)all) : 0;
+    return t < all ? t : all - 1;
+  };
+  const auto answer = [&](uint32_t id, float v, u64 all) {
+    a.token[row] = id;
+    a.logprob[row] = greedy ? 0.0f
+                            : (float)(((double)v - (double)m) * inv_t - log((double)all * __builtin_ldexp(1.0, -a.shift)));
+  };
+
+  // The elements for which f(value, id) holds into the list, in any order; their number (more than kList: not all of them are there).
+  const auto take = [&](float v, uint32_t id) {
+    const uint32_t at = atomicAdd(&sh.listed, 1u);
+    if (at < kList) sh.bins.list[at].at = (u64)key_of<E>(v) << 32 | (uint32_t)~id;
+  };
+  const auto list_begin = [&] {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+  };
+  const auto list_end = [&]() -> int {
+    __syncthreads();
+    const int n = (int)(sh.listed < kList ? sh.listed : kList + 1);
+    if (n <= kList)
+      for (int i = threadIdx.x; i < n; i += T) sh.bins.list[i].w = weight(value_of_key<E>((uint32_t)(sh.bins.list[i].at >> 32)));
+    __syncthreads();
+    return n;
+  };
+  constexpr int kOwn = (kList + T - 1) / T;          // of the list, a thread's
+  // Places in the order and mass before each of a thread's candidates, among the list's.
+  const auto rank = [&](int n, uint32_t (&before)[kOwn], u64 (&mass)[kOwn]) {
+    u64 at[kOwn];
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+      at[q] = (int)threadIdx.x + q * T < n ? sh.bins.list[threadIdx.x + q * T].at : ~0ull;
+      before[q] = 0, mass[q] = 0;
+    }
+    for (int j = 0; j < n; ++j) {
+      const Candidate c = sh.bins.list[j];
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q)
+        if (kOwn == 1 || q * T < n) {
+          before[q] += c.at > at[q];
+          mass[q] += c.at > at[q] ? c.w : 0;
+        }
+    }
+  };
+
+  // ---- rows whose candidates a bound leaves few of: the k-th largest of 256 threads' maxima (a lower bound of the k-th largest
+  // element), or the smallest value that min_p lets through
+  const bool few = by_k && top_k <= (T >= 256 ? 192 : 48);
+  if (few || (low > -__builtin_inf() && !(by_k && by_p))) {
+    float bound = kNone;
+    if (few) {
+      constexpr int N = T >= 256 ? 4 : 1;            // maxima a lane of the first wave looks at
+      constexpr int G = T > 256 ? T / 256 : 1;       // threads of one
+      float g = own_max;
+      if constexpr (G > 1) g = lanes_max_nan(g, G);
+      uint32_t* const maxima = (uint32_t*)sh.seg;
+      if (threadIdx.x % G == 0) maxima[threadIdx.x / G] = key_of<E>(g);
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t o[N], t = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = maxima[i * 64 + lane];
+#pragma unroll
+        for (int b = kKeyBits<E> - 1; b >= 0; --b) {
+          const uint32_t c = t | 1u << b;
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o[i] >= c));
+          if (n >= (int)top_k) t = c;
+        }
+        if (lane == 0) sh.bound = t;
+      }
+      __syncthreads();
+      bound = value_of_key<E>(sh.bound);
+    }
+    // (a row that top_p cuts without top_k needs min_p's candidates alone, but the mass of all)
+    u64 all = 0;
+    if (by_p && !by_k) {
+      each([&](int, int e, const Frag<E>& v) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) all += e + j < a.V ? weight(v.v[j]) : 0;
+      });
+      all = block_sum(all);
+    }
+    list_begin();
+    const auto looked = [&](float v, uint32_t id) {
+      if ((few ? v >= bound : near(v)) && id < (uint32_t)a.V) take(v, id);
+    };
+    if constexpr (NV > 0) {
+      if (few ? own_max >= bound : near(own_max)) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          asm("" : "+v"(raw[i]));      // (widened again: the fp32 values of the first pass would take the registers)
+          const Frag<E> f = widen<E>(raw[i]);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) looked(f.v[j], (uint32_t)((i * T + threadIdx.x) * VE + j));
+        }
+      }
+    } else {
+      each([&](int, int e, const Frag<E>& v) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) looked(v.v[j], (uint32_t)(e + j));
+      });
+    }
+    const int n = list_end();
+    if (n <= kList) {
+      uint32_t before[kOwn];
+      u64 mass[kOwn], w[kOwn], at[kOwn];
+      rank(n, before, mass);
+      u64 sum = 0;
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) {
+        const int i = threadIdx.x + q * T;
+        at[q] = i < n ? sh.bins.list[i].at : 0, w[q] = i < n ? sh.bins.list[i].w : 0;
+        if (i >= n || (by_k && before[q] >= (uint64_t)top_k)) before[q] = 0xFFFFFFFFu, w[q] = 0;
+        sum += w[q];
+      }
+      if (by_p) {
+        const u64 target = share(top_p, by_k ? block_sum(sum) : all);
+        sum = 0;
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) {
+          if (mass[q] >= target) w[q] = 0;
+          sum += w[q];
+        }
+      }
+      if (low > -__builtin_inf()) {
+        sum = 0;
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q) {
+          if (!near(value_of_key<E>((uint32_t)(at[q] >> 32)))) w[q] = 0;
+          sum += w[q];
+        }
+      }
+      sum = block_sum(sum);
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q)
+        if ((int)threadIdx.x + q * T < n) sh.bins.list[threadIdx.x + q * T].w = w[q];
+      __syncthreads();
+      const u64 t = place(sum);
+      u64 upto[kOwn];
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q) upto[q] = 0;
+      for (int j = 0; j < n; ++j) {
+        const Candidate c = sh.bins.list[j];
+#pragma unroll
+        for (int q = 0; q < kOwn; ++q)
+          if (kOwn == 1 || q * T < n) upto[q] += (uint32_t)c.at > (uint32_t)at[q] ? c.w : 0;      // (a smaller id)
+      }
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q)
+        if (w[q] > 0 && upto[q] <= t && t - upto[q] < w[q]) answer(~(uint32_t)at[q], value_of_key<E>((uint32_t)(at[q] >> 32)), sum);
+      return;
+    }
+  }
+
+  // ---- the other rows
+  // The first id at which the running sum of f over the ids exceeds t (t below the whole sum); sh.total holds the whole sum, from which
+  // t_of makes t.
   const auto locate = [&](const auto& f, const auto& t_of) {
+    __syncthreads();
     for (int i = threadIdx.x; i < kSegs; i += T) sh.seg[i] = 0;
     if (threadIdx.x == 0) sh.seg_at = 0, sh.id = 0, sh.rest = 0;
     __syncthreads();
@@ -136,24 +376,26 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       }
       at = s;
 #pragma unroll
-      for (int j = 0; j < VE; ++j)
-        if (e + j < a.V) acc += f(v.v[j], (uint32_t)(e + j));
+      for (int j = 0; j < VE; ++j) {
+        const u64 w = f(v.v[j], (uint32_t)(e + j));
+        acc += e + j < a.V ? w : 0;
+      }
     });
     if (at >= 0) {
       const u64 r = wave_sum_u64(acc);
-      if (lane == 0 && at < kSegs) sh.seg[at] = r;
+      if (lane == 0) sh.seg[at] = r;
     }
     __syncthreads();
     if (wave == 0) {
+      constexpr int N = kSegs / 64;
       u64 own = 0;
-      for (int i = 0; i < kSegs / 64; ++i) own += sh.seg[lane * (kSegs / 64) + i];
-      const u64 upto = wave_scan_u64(own, lane);
-      const u64 all = __shfl(upto, 63, 64);
+      for (int i = 0; i < N; ++i) own += sh.seg[lane * N + i];
+      const u64 upto = wave_scan_u64(own, lane), all = __shfl(upto, 63, 64);
       if (lane == 0) sh.total = all;
       const u64 t = t_of(all);
       if (upto > t && upto - own <= t) {
         u64 before = upto - own;
-        int s = lane * (kSegs / 64);
+        int s = lane * N;
         while (before + sh.seg[s] <= t) before += sh.seg[s++];
         sh.seg_at = s;
         sh.rest = t - before;
@@ -194,24 +436,24 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   };
 
   // The threshold (thr, thr_id) at which the order, from its largest on and within the present threshold, has reached `target`: places,
-  // or mass.  t_of gives the target from the whole mass.
+  // or mass.  By digits of the key, whatever the row holds.
   const auto search = [&](bool by_mass, u64 target) {
     uint32_t prefix = 0;
     u64 above = 0;
     int bits = kKeyBits<E>;
     while (bits > 0) {
-      const int take = bits < kDigit ? bits : kDigit, low = bits - take;
+      const int take_bits = bits < kDigit ? bits : kDigit, shift = bits - take_bits;
       __syncthreads();
-      for (int i = threadIdx.x; i < 1 << kDigit; i += T) sh.count[i] = 0, sh.mass[i] = 0;
+      for (int i = threadIdx.x; i < 1 << kDigit; i += T) sh.radix.count[i] = 0, sh.radix.mass[i] = 0;
       __syncthreads();
       each([&](int, int e, const Frag<E>& v) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           const uint32_t key = key_of<E>(v.v[j]);
           if (e + j < a.V && (bits == kKeyBits<E> || key >> bits == prefix) && in_order(key, (uint32_t)(e + j))) {
-            const uint32_t d = key >> low & ((1u << take) - 1);
-            atomicAdd(&sh.count[d], 1u);
-            if (by_mass) atomicAdd(&sh.mass[d], weight(v.v[j]));
+            const uint32_t d = key >> shift & ((1u << take_bits) - 1);
+            atomicAdd(&sh.radix.count[d], 1u);
+            if (by_mass) atomicAdd(&sh.radix.mass[d], weight(v.v[j]));
           }
         }
       });
@@ -221,17 +463,16 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         u64 own = 0;
         for (int i = 0; i < N; ++i) {
           const int d = (1 << kDigit) - 1 - (lane * N + i);
-          own += by_mass ? sh.mass[d] : sh.count[d];
+          own += by_mass ? sh.radix.mass[d] : sh.radix.count[d];
         }
         const u64 upto = wave_scan_u64(own, lane) + above;
         if (upto >= target && upto - own < target) {
           u64 before = upto - own;
-          int i = 0;
-          for (;; ++i) {
+          for (int i = 0; i < N; ++i) {
             const int d = (1 << kDigit) - 1 - (lane * N + i);
-            const u64 v = by_mass ? sh.mass[d] : sh.count[d];
+            const u64 v = by_mass ? sh.radix.mass[d] : sh.radix.count[d];
             if (before + v >= target) {
-              sh.bin = (uint32_t)d, sh.bin_count = sh.count[d], sh.bin_mass = v, sh.above_mass = before;
+              sh.bin = (uint32_t)d, sh.bin_count = sh.radix.count[d], sh.bin_mass = v, sh.above = before;
               break;
             }
             before += v;
@@ -239,15 +480,14 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         }
       }
       __syncthreads();
-      prefix = prefix << take | sh.bin;
-      above = sh.above_mass;
-      bits = low;
+      prefix = prefix << take_bits | sh.bin;
+      above = sh.above;
+      bits = shift;
     }
     // ties at the threshold: the first `need` of them by id
     const u64 of = sh.bin_mass, n_ties = sh.bin_count;
     const u64 each_w = by_mass ? of / n_ties : 1;
     const u64 need = (target - above + each_w - 1) / each_w;
-    __syncthreads();
     uint32_t id = 0xFFFFFFFFu;
     if (need < n_ties)
       id = locate([&](float v, uint32_t i) -> u64 { const uint32_t k = key_of<E>(v); return k == prefix && in_order(k, i); },
@@ -256,50 +496,121 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     thr = prefix, thr_id = id;
   };
 
-  if (greedy) {
-    search(false, 1);
-    const uint32_t id = locate([&](float v, uint32_t i) -> u64 { return in_order(key_of<E>(v), i); }, [](u64) { return (u64)0; });
-    if (threadIdx.x == 0) a.token[row] = id, a.logprob[row] = 0.0f;
-    return;
-  }
-  if (top_k > 0 && top_k < a.V) search(false, (u64)top_k);
-  if (top_p < 1.0) {
-    u64 part = 0;
+  // Counts and masses by bins of distance from the maximum; then the bin in which places or mass reach a target, and the threshold from
+  // that bin's elements alone, ranked among themselves.
+  const float to_bin = (float)(per_e * -16.0);
+  const auto bin_of = [&](float v) {
+    const float d = (v - m) * to_bin;
+    return d < (float)kBins ? (int)d : kBins - 1;      // (a NaN, of an infinite temperature: the last)
+  };
+  const auto bins = [&](bool with_mass) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += T) sh.bins.count[i] = 0, sh.bins.mass[i] = 0;
+    __syncthreads();
     each([&](int, int e, const Frag<E>& v) {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
-        if (e + j < a.V && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) part += weight(v.v[j]);
+        if (e + j < a.V) {
+          const int b = bin_of(v.v[j]);
+          atomicAdd(&sh.bins.count[b], 1u);
+          if (with_mass) {
+            const u64 w = weight(v.v[j]);
+            if (w) atomicAdd(&sh.bins.mass[b], w);
+          }
+        }
     });
-    part = wave_sum_u64(part);
     __syncthreads();
-    if (lane == 0) sh.seg[wave] = part;
-    __syncthreads();
-    u64 all = 0;
-    for (int i = 0; i < W; ++i) all += sh.seg[i];
-    u64 target = (u64)__builtin_ceil((top_p > 0.0 ? top_p : 0.0) * (double)all);
-    target = target < 1 ? 1 : target > all ? all : target;
-    __syncthreads();
-    search(true, target);
-  }
-  const double low = min_p > 0.0 ? log(min_p < 1.0 ? min_p : 1.0) * temp : -__builtin_inf();
-  const auto kept = [&](float v, uint32_t id) -> u64 {
-    return in_order(key_of<E>(v), id) && !((double)v - (double)m < low) ? weight(v) : 0;
   };
-  const uint32_t id = locate(kept, [&](u64 all) {
-    const u64 t = u > 0.0 ? (u64)__builtin_floor(u * (double)all) : 0;
-    return t < all ? t : all - 1;
-  });
-  if (threadIdx.x == 0) {
-    a.token[row] = id;
-    const double z = ((double)to_f32(x[id]) - (double)m) * inv_t;
-    a.logprob[row] = (float)(z - log((double)sh.total * __builtin_ldexp(1.0, -a.shift)));
+  // sh.bin with sh.above before it and sh.above's mass in sh.bin_mass; false where too many elements lie in it.
+  u64 kept_mass = 0;                               // of the present threshold
+  const auto refine = [&](bool by_mass, u64 target) -> bool {
+    if (wave == 0) {
+      constexpr int N = kBins / 64;
+      u64 own = 0, own_mass = 0;
+      for (int i = 0; i < N; ++i) own += by_mass ? sh.bins.mass[lane * N + i] : sh.bins.count[lane * N + i];
+      for (int i = 0; i < N; ++i) own_mass += sh.bins.mass[lane * N + i];
+      const u64 upto = wave_scan_u64(own, lane), upto_mass = wave_scan_u64(own_mass, lane);
+      if (upto >= target && upto - own < target) {
+        u64 before = upto - own, mass = upto_mass - own_mass;
+        for (int i = 0; i < N; ++i) {
+          const int b = lane * N + i;
+          const u64 v = by_mass ? sh.bins.mass[b] : sh.bins.count[b];
+          if (before + v >= target) {
+            sh.bin = (uint32_t)b, sh.above = before, sh.bin_mass = mass, sh.bin_count = sh.bins.count[b];
+            break;
+          }
+          before += v, mass += sh.bins.mass[b];
+        }
+      }
+    }
+    __syncthreads();
+    const int b = (int)sh.bin;
+    const u64 above = sh.above, above_mass = sh.bin_mass;
+    if (sh.bin_count > kList) return false;
+    list_begin();
+    each([&](int, int e, const Frag<E>& v) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+        if (e + j < a.V && bin_of(v.v[j]) == b && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) take(v.v[j], (uint32_t)(e + j));
+    });
+    const int n = list_end();
+    uint32_t before[kOwn];
+    u64 mass[kOwn], part = 0;
+    rank(n, before, mass);
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+      const int i = threadIdx.x + q * T;
+      if (i >= n) continue;
+      const Candidate c = sh.bins.list[i];
+      const u64 from = above + (by_mass ? mass[q] : before[q]), size = by_mass ? c.w : 1;
+      if (from < target) part += c.w;
+      if (from < target && target - from <= size) sh.thr = (uint32_t)(c.at >> 32), sh.thr_id = ~(uint32_t)c.at;
+    }
+    kept_mass = above_mass + block_sum(part);
+    __syncthreads();
+    thr = sh.thr, thr_id = sh.thr_id;
+    return true;
+  };
+
+  if (by_k || by_p) {
+    bins(by_p);
+    if (by_k) {
+      if (!refine(false, (u64)top_k)) {
+        search(false, (u64)top_k);
+        kept_mass = ~0ull;
+      }
+    } else {
+      u64 part = 0;
+      for (int i = threadIdx.x; i < kBins; i += T) part += sh.bins.mass[i];
+      kept_mass = block_sum(part);
+    }
+    if (by_p) {
+      bool done = false;
+      if (kept_mass != ~0ull) {
+        done = refine(true, share(top_p, kept_mass));
+      } else {                                     // (the bins gave way to the search's)
+        u64 part = 0;
+        each([&](int, int e, const Frag<E>& v) {
+#pragma unroll
+          for (int j = 0; j < VE; ++j)
+            if (e + j < a.V && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) part += weight(v.v[j]);
+        });
+        kept_mass = block_sum(part);
+      }
+      if (!done) search(true, share(top_p, kept_mass));
+    }
   }
+  const auto kept = [&](float v, uint32_t id) -> u64 { return in_order(key_of<E>(v), id) && near(v) ? weight(v) : 0; };
+  const uint32_t id = locate(kept, place);
+  if (threadIdx.x == 0) answer(id, to_f32(x[id]), sh.total);
 }
 
 // ---- host side
 
 constexpr int64_t kSampleRows = (int64_t)1 << 21;
 
+// A block a row: a wave for rows of up to 256 vectors, four for up to 4,096 where there are rows enough to fill the chip with them, else
+// sixteen.
 template <class E>
 static void sample(const SampleArgs& b, hipStream_t st) {
   constexpr int VE = Elem<E>::VE;
@@ -315,9 +626,14 @@ static void sample(const SampleArgs& b, hipStream_t st) {
     const int64_t steps = (nvec + 63) / 64;
     a.per_seg = (int32_t)((steps + kSegs - 1) / kSegs);
     const unsigned rows = (unsigned)a.n;
-    if (nvec <= 64 * 4) k_sample<E, 64><<<rows, 64, 0, st>>>(a);
-    else if (nvec <= 256 * 8) k_sample<E, 256><<<rows, 256, 0, st>>>(a);
-    else k_sample<E, 1024><<<rows, 1024, 0, st>>>(a);
+    const bool many = a.n >= 512;
+    if (nvec <= 64) k_sample<E, 64, 1><<<rows, 64, 0, st>>>(a);
+    else if (nvec <= 256) k_sample<E, 64, 4><<<rows, 64, 0, st>>>(a);
+    else if (nvec <= 1024) k_sample<E, 256, 4><<<rows, 256, 0, st>>>(a);
+    else if (nvec <= 4096 && many) k_sample<E, 256, 16><<<rows, 256, 0, st>>>(a);
+    else if (nvec <= 4096) k_sample<E, 1024, 4><<<rows, 1024, 0, st>>>(a);
+    else if (nvec <= 16384) k_sample<E, 1024, 16><<<rows, 1024, 0, st>>>(a);
+    else k_sample<E, 1024, 0><<<rows, 1024, 0, st>>>(a);
   }
 }
 
@@ -338,7 +654,7 @@ extern "C" int elr_sample_tokens(const void* logits, int type, int64_t n, int64_
   if (!logits || !u || !token || !logprob || !elem_aligned(logits, type)) return ELR_EINVAL;
   int lg = 0;
   while (((int64_t)1 << lg) < V) ++lg;
-  const SampleArgs a{logits, ld, n, (int32_t)V, 62 - lg < 52 ? 62 - lg : 52, 1, u, temperature, top_p, min_p, top_k,
+  const SampleArgs a{logits, ld, n, (int32_t)V, 62 - lg < kWeightBits ? 62 - lg : kWeightBits, 1, u, temperature, top_p, min_p, top_k,
                      temperature_rows, top_p_rows, min_p_rows, top_k_rows, top_k_64, token, logprob};
   hipStream_t st = (hipStream_t)stream;
   if (type == ELR_F32) sample<float>(a, st);
