@@ -17,10 +17,14 @@ namespace elr {
 
 typedef unsigned long long u64;
 
-constexpr int kSegs = 512;           // partial sums of a row in the order of ids
-constexpr int kDigit = 11;           // bits of a selection pass
-constexpr int kList = 512;           // candidates that are ranked among themselves
-constexpr int kBins = 1024;          // bins of a row by distance from its maximum, 1/16 of a factor 2 in e wide
+// What a block of T threads keeps in LDS.  (A wave by itself works on rows of up to 2,048 elements: LDS bounds how many run at once.)
+template <int T>
+struct Shape {
+  static constexpr int kSegs = T > 64 ? 512 : 64;      // partial sums of a row in the order of ids
+  static constexpr int kDigit = T > 64 ? 11 : 8;       // bits of a selection pass
+  static constexpr int kList = T > 64 ? 512 : 256;     // candidates that are ranked among themselves
+  static constexpr int kBins = T > 64 ? 1024 : 256;    // bins of a row by distance from its maximum, up to 2^-32 in e
+};
 constexpr int kWeightBits = 51;      // of the largest weight
 
 struct SampleArgs {
@@ -78,7 +82,9 @@ struct Candidate {
   u64 at;        // key in the high half, ~id in the low: larger comes first
   u64 w;
 };
+template <int T>
 struct SampleShared {
+  static constexpr int kSegs = Shape<T>::kSegs, kDigit = Shape<T>::kDigit, kList = Shape<T>::kList, kBins = Shape<T>::kBins;
   union {
     struct {
       uint32_t count[1 << kDigit];
@@ -115,9 +121,10 @@ __device__ __forceinline__ u64 wave_scan_u64(u64 x, int lane) {
 // One row by a block of T threads.  NV > 0: the row's vectors of a thread stay in registers for the search of candidates; the passes that
 // some rows need beyond it read the row again (from the caches).
 template <class E, int T, int NV>
-__global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
+__global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
   constexpr int VE = Elem<E>::VE, W = T / 64;
-  __shared__ SampleShared sh;
+  constexpr int kSegs = Shape<T>::kSegs, kDigit = Shape<T>::kDigit, kList = Shape<T>::kList, kBins = Shape<T>::kBins;
+  __shared__ SampleShared<T> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
   const E* x = (const E*)a.x + row * a.ld;
@@ -125,15 +132,24 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
   const int nseg = (int)(((int64_t)a.V + (int64_t)64 * VE * a.per_seg - 1) / ((int64_t)64 * VE * a.per_seg));
   // f(segment, first id, VE values) over the wave's vectors; the segments are in the order of ids.
   const auto each = [&](const auto& f) {
-    for (int s = wave; s < nseg; s += W)
-      for (int j = 0; j < a.per_seg; ++j) {
-        const int64_t e = (((int64_t)s * a.per_seg + j) * 64 + lane) * VE;
-        f(s, (int)(e < a.V ? e : a.V), widen<E>(load_raw<E, false>(x + (e < a.V ? e : 0), a.V - e, kNone)));
-      }
+    int s = wave, j = 0;
+    const auto first = [&] { return (((int64_t)s * a.per_seg + j) * 64 + lane) * VE; };
+    const auto load = [&](int64_t e) { return load_raw<E, false>(x + (e < a.V ? e : 0), a.V - e, kNone); };
+    if (s >= nseg) return;
+    int64_t e = first();
+    u32x4 next = load(e);
+    while (s < nseg) {                 // (the next vector on its way)
+      const u32x4 now = next;
+      const int seg = s;
+      const int64_t at = e < a.V ? e : a.V;
+      if (++j == a.per_seg) j = 0, s += W;
+      if (s < nseg) next = load(e = first());
+      f(seg, (int)at, widen<E>(now));
+    }
   };
   // the row's maximum (NaN or +inf in the row show in it), and the thread's
-  u32x4 raw[NV > 0 ? NV : 1];
-  float own_max = kNone;
+  [[maybe_unused]] u32x4 raw[NV > 0 ? NV : 1];
+  [[maybe_unused]] float vec_max[NV > 0 ? NV : 1], own_max = kNone;
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -143,8 +159,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const Frag<E> f = widen<E>(raw[i]);
+      vec_max[i] = f.v[0];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) own_max = max_nan(own_max, f.v[j]);
+      for (int j = 1; j < VE; ++j) vec_max[i] = max_nan(vec_max[i], f.v[j]);
+      own_max = max_nan(own_max, vec_max[i]);
     }
   } else {
     each([&](int, int, const Frag<E>& f) {
@@ -290,9 +308,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       if ((few ? v >= bound : near(v)) && id < (uint32_t)a.V) take(v, id);
     };
     if constexpr (NV > 0) {
-      if (few ? own_max >= bound : near(own_max)) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+      for (int i = 0; i < NV; ++i) {
+        if (few ? vec_max[i] >= bound : near(vec_max[i])) {
           asm("" : "+v"(raw[i]));      // (widened again: the fp32 values of the first pass would take the registers)
           const Frag<E> f = widen<E>(raw[i]);
 #pragma unroll
@@ -498,7 +516,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
 
   // Counts and masses by bins of distance from the maximum; then the bin in which places or mass reach a target, and the threshold from
   // that bin's elements alone, ranked among themselves.
-  const float to_bin = (float)(per_e * -16.0);
+  const float to_bin = (float)(per_e * -(kBins / 32));
   const auto bin_of = [&](float v) {
     const float d = (v - m) * to_bin;
     return d < (float)kBins ? (int)d : kBins - 1;      // (a NaN, of an infinite temperature: the last)
@@ -512,7 +530,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
       for (int j = 0; j < VE; ++j)
         if (e + j < a.V) {
           const int b = bin_of(v.v[j]);
-          atomicAdd(&sh.bins.count[b], 1u);
+          if (by_k) atomicAdd(&sh.bins.count[b], 1u);
           if (with_mass) {
             const u64 w = weight(v.v[j]);
             if (w) atomicAdd(&sh.bins.mass[b], w);
@@ -521,7 +539,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     });
     __syncthreads();
   };
-  // sh.bin with sh.above before it and sh.above's mass in sh.bin_mass; false where too many elements lie in it.
+  // False where too many elements lie in the bin.
   u64 kept_mass = 0;                               // of the present threshold
   const auto refine = [&](bool by_mass, u64 target) -> bool {
     if (wave == 0) {
@@ -536,7 +554,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
           const int b = lane * N + i;
           const u64 v = by_mass ? sh.bins.mass[b] : sh.bins.count[b];
           if (before + v >= target) {
-            sh.bin = (uint32_t)b, sh.above = before, sh.bin_mass = mass, sh.bin_count = sh.bins.count[b];
+            sh.bin = (uint32_t)b, sh.above = before, sh.bin_mass = mass;
             break;
           }
           before += v, mass += sh.bins.mass[b];
@@ -546,7 +564,6 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
     __syncthreads();
     const int b = (int)sh.bin;
     const u64 above = sh.above, above_mass = sh.bin_mass;
-    if (sh.bin_count > kList) return false;
     list_begin();
     each([&](int, int e, const Frag<E>& v) {
 #pragma unroll
@@ -554,6 +571,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
         if (e + j < a.V && bin_of(v.v[j]) == b && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) take(v.v[j], (uint32_t)(e + j));
     });
     const int n = list_end();
+    if (n > kList) return false;
     uint32_t before[kOwn];
     u64 mass[kOwn], part = 0;
     rank(n, before, mass);
@@ -609,6 +627,12 @@ __global__ __launch_bounds__(T) void k_sample(SampleArgs a) {
 
 constexpr int64_t kSampleRows = (int64_t)1 << 21;
 
+template <class E, int T, int NV>
+static void launch_sample(SampleArgs& a, int64_t nvec, hipStream_t st) {
+  a.per_seg = (int32_t)(((nvec + 63) / 64 + Shape<T>::kSegs - 1) / Shape<T>::kSegs);
+  k_sample<E, T, NV><<<(unsigned)a.n, T, 0, st>>>(a);
+}
+
 // A block a row: a wave for rows of up to 256 vectors, four for up to 4,096 where there are rows enough to fill the chip with them, else
 // sixteen.
 template <class E>
@@ -623,17 +647,15 @@ static void sample(const SampleArgs& b, hipStream_t st) {
     if (b.top_p_rows) a.top_p_rows = b.top_p_rows + r;
     if (b.min_p_rows) a.min_p_rows = b.min_p_rows + r;
     if (b.top_k_rows) a.top_k_rows = (const char*)b.top_k_rows + r * (b.top_k_64 ? 8 : 4);
-    const int64_t steps = (nvec + 63) / 64;
-    a.per_seg = (int32_t)((steps + kSegs - 1) / kSegs);
-    const unsigned rows = (unsigned)a.n;
     const bool many = a.n >= 512;
-    if (nvec <= 64) k_sample<E, 64, 1><<<rows, 64, 0, st>>>(a);
-    else if (nvec <= 256) k_sample<E, 64, 4><<<rows, 64, 0, st>>>(a);
-    else if (nvec <= 1024) k_sample<E, 256, 4><<<rows, 256, 0, st>>>(a);
-    else if (nvec <= 4096 && many) k_sample<E, 256, 16><<<rows, 256, 0, st>>>(a);
-    else if (nvec <= 4096) k_sample<E, 1024, 4><<<rows, 1024, 0, st>>>(a);
-    else if (nvec <= 16384) k_sample<E, 1024, 16><<<rows, 1024, 0, st>>>(a);
-    else k_sample<E, 1024, 0><<<rows, 1024, 0, st>>>(a);
+    if (nvec <= 64) launch_sample<E, 64, 1>(a, nvec, st);
+    else if (nvec <= 256) launch_sample<E, 64, 4>(a, nvec, st);
+    else if (nvec <= 1024) launch_sample<E, 256, 4>(a, nvec, st);
+    else if (nvec <= 4096 && many) launch_sample<E, 256, 16>(a, nvec, st);
+    else if (nvec <= 4096) launch_sample<E, 1024, 4>(a, nvec, st);
+    else if (a.n > 256) launch_sample<E, 512, 0>(a, nvec, st);
+    else if (nvec <= 16384) launch_sample<E, 1024, 16>(a, nvec, st);
+    else launch_sample<E, 1024, 0>(a, nvec, st);
   }
 }
 
