@@ -50,11 +50,25 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) >> (32 - kKeyBits<E>);
 }
+__device__ __forceinline__ uint32_t order_of_value(float x) {      // (of fp32: the next value is the next number)
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of_order(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
 template <class E>
 __device__ __forceinline__ float value_of_key(uint32_t key) {
   constexpr int kDrop = 32 - kKeyBits<E>;
   const uint32_t o = key << kDrop;
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o >> kDrop << kDrop);
+}
+
+// a b + c with c in scalar registers (left to itself the compiler copies each constant into vector registers and overwrites the copy).
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
 }
 
 // 2^(z + shift) for z <= 0, rounded to an integer below 2^52.  2^f, |f| <= 1/2, by the polynomial through the ten Chebyshev points
@@ -66,14 +80,14 @@ __device__ __forceinline__ u64 weight_of(double z, int shift) {
   const double t = z + kRound, f = z - (t - kRound);
   const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
   double p = 0x1.b6571d9fbc782p-24;
-  p = __builtin_fma(p, f, 0x1.63ef9699f65f0p-20);
-  p = __builtin_fma(p, f, 0x1.ffcb7678dfe12p-17);
-  p = __builtin_fma(p, f, 0x1.43088e257f900p-13);
-  p = __builtin_fma(p, f, 0x1.5d87fe908f6f7p-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab72b175e9p-7);
-  p = __builtin_fma(p, f, 0x1.c6b08d704411ap-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff8149f2p-3);
-  p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = fma_const(p, f, 0x1.63ef9699f65f0p-20);
+  p = fma_const(p, f, 0x1.ffcb7678dfe12p-17);
+  p = fma_const(p, f, 0x1.43088e257f900p-13);
+  p = fma_const(p, f, 0x1.5d87fe908f6f7p-10);
+  p = fma_const(p, f, 0x1.3b2ab72b175e9p-7);
+  p = fma_const(p, f, 0x1.c6b08d704411ap-5);
+  p = fma_const(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma_const(p, f, 0x1.62e42fefa39f7p-1);
   p = __builtin_fma(p, f, 1.0);
   return __builtin_bit_cast(uint64_t, __builtin_ldexp(p, n + shift) + 0x1p52) & 0xFFFFFFFFFFFFFu;
 }
@@ -101,7 +115,8 @@ struct SampleShared {
   u64 sums[16];
   uint32_t bin, bin_count, listed, bound;
   u64 above, bin_mass, total, rest;
-  uint32_t id, thr, thr_id;
+  uint32_t id, thr_id;
+  float thr;
   int seg_at;
 };
 
@@ -130,21 +145,39 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
   const E* x = (const E*)a.x + row * a.ld;
   constexpr float kNone = -__builtin_inff();
   const int nseg = (int)(((int64_t)a.V + (int64_t)64 * VE * a.per_seg - 1) / ((int64_t)64 * VE * a.per_seg));
+  // The vector from id e on, and its values: unconditional loads (a branch around a load ends in a wait for it).  The row's last vector, and
+  // those past it, are the last VE elements, of which those before e count as -inf: no candidates, without weight.
+  constexpr bool kTiny = T == 64 && NV == 1;         // rows of less than a vector come here
+  const auto base = [&](int32_t e) { return e < a.V - VE ? e : a.V - VE < 0 ? 0 : a.V - VE; };
+  const auto load = [&](int32_t e) -> u32x4 {
+    if constexpr (kTiny)
+      if (a.V < VE) return load_raw<E, false>(x, e == 0 ? a.V : 0, kNone);
+    return *reinterpret_cast<const u32x4_u*>(x + base(e));
+  };
+  const auto values = [&](u32x4 r, int32_t e) {
+    Frag<E> f = widen<E>(r);
+    if (__builtin_amdgcn_readfirstlane(e - lane * VE) + 64 * VE > a.V) {      // (lanes hold neighbouring vectors)
+      const int32_t b = base(e);
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+        if (b + j < e) f.v[j] = kNone;
+    }
+    return f;
+  };
   // f(segment, first id, VE values) over the wave's vectors; the segments are in the order of ids.
   const auto each = [&](const auto& f) {
     int s = wave, j = 0;
-    const auto first = [&] { return (((int64_t)s * a.per_seg + j) * 64 + lane) * VE; };
-    const auto load = [&](int64_t e) { return load_raw<E, false>(x + (e < a.V ? e : 0), a.V - e, kNone); };
     if (s >= nseg) return;
-    int64_t e = first();
+    int32_t e = (s * a.per_seg * 64 + lane) * VE;
     u32x4 next = load(e);
     while (s < nseg) {                 // (the next vector on its way)
       const u32x4 now = next;
       const int seg = s;
-      const int64_t at = e < a.V ? e : a.V;
+      const int32_t at = e;
       if (++j == a.per_seg) j = 0, s += W;
-      if (s < nseg) next = load(e = first());
-      f(seg, (int)at, widen<E>(now));
+      e = ((s * a.per_seg + j) * 64 + lane) * VE;
+      next = load(e);                  // (past the row: its end again)
+      f(seg, base(at), values(now, at));
     }
   };
   // the row's maximum (NaN or +inf in the row show in it), and the thread's
@@ -153,15 +186,15 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t e = ((int64_t)i * T + threadIdx.x) * VE;
-      raw[i] = load_raw<E, true>(x + (e < a.V ? e : 0), a.V - e, kNone);
+      raw[i] = load((i * T + threadIdx.x) * VE);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const Frag<E> f = widen<E>(raw[i]);
+      const Frag<E> f = values(raw[i], (i * T + threadIdx.x) * VE);
       vec_max[i] = f.v[0];
 #pragma unroll
       for (int j = 1; j < VE; ++j) vec_max[i] = max_nan(vec_max[i], f.v[j]);
+      asm volatile("" : "+v"(vec_max[i]));    // (taken here: put off, all vectors' values would take the registers)
       own_max = max_nan(own_max, vec_max[i]);
     }
   } else {
@@ -196,9 +229,19 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
   const double inv_t = greedy ? 0.0 : 1.0 / temp, per_e = inv_t * 0x1.71547652b82fep+0;      // to powers of two
   const auto weight = [&](float v) -> u64 { return weight_of(((double)v - (double)m) * per_e, a.shift); };
   const double low = greedy || !(min_p > 0.0) ? -__builtin_inf() : log(min_p < 1.0 ? min_p : 1.0) * temp;
-  const auto near = [&](float v) { return !((double)v - (double)m < low); };
-  uint32_t thr = 0, thr_id = 0xFFFFFFFFu;     // kept: a larger key, or this key and no larger id
-  const auto in_order = [&](uint32_t key, uint32_t id) { return key > thr || (key == thr && id <= thr_id); };
+  // the smallest value that min_p lets through: m itself at most
+  float low_v = kNone;
+  if (low > -__builtin_inf()) {
+    low_v = (float)((double)m + low);
+    const auto step = [](float v, int by) { return value_of_order(order_of_value(v) + by); };
+    for (int i = 0; i < 4 && (double)low_v - (double)m < low; ++i) low_v = step(low_v, 1);
+    for (int i = 0; i < 4 && !((double)step(low_v, -1) - (double)m < low); ++i) low_v = step(low_v, -1);
+    low_v = low_v < m ? low_v : m;
+  }
+  const auto near = [&](float v) { return v >= low_v; };
+  float thr = kNone;                           // kept: a larger value, or this value and no larger id
+  uint32_t thr_id = 0xFFFFFFFFu;
+  const auto in_order = [&](float v, uint32_t id) { return (v > thr) | ((v == thr) & (id <= thr_id)); };
 
   // The sum of one value a thread; every thread gets it.
   const auto block_sum = [&](u64 v) {
@@ -297,24 +340,27 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     // (a row that top_p cuts without top_k needs min_p's candidates alone, but the mass of all)
     u64 all = 0;
     if (by_p && !by_k) {
-      each([&](int, int e, const Frag<E>& v) {
+      each([&](int, int, const Frag<E>& v) {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) all += e + j < a.V ? weight(v.v[j]) : 0;
+        for (int j = 0; j < VE; ++j) all += weight(v.v[j]);
       });
       all = block_sum(all);
     }
     list_begin();
+    if (!few) bound = low_v;
     const auto looked = [&](float v, uint32_t id) {
-      if ((few ? v >= bound : near(v)) && id < (uint32_t)a.V) take(v, id);
+      if ((v >= bound) & (v > kNone)) take(v, id);
     };
     if constexpr (NV > 0) {
+      int32_t tid = threadIdx.x;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (few ? vec_max[i] >= bound : near(vec_max[i])) {
-          asm("" : "+v"(raw[i]));      // (widened again: the fp32 values of the first pass would take the registers)
-          const Frag<E> f = widen<E>(raw[i]);
+        if (vec_max[i] >= bound) {
+          asm("" : "+v"(raw[i]), "+v"(tid));      // (widened again: what the first pass made would take the registers)
+          const int32_t e = (i * T + tid) * VE;
+          const Frag<E> f = values(raw[i], e);
 #pragma unroll
-          for (int j = 0; j < VE; ++j) looked(f.v[j], (uint32_t)((i * T + threadIdx.x) * VE + j));
+          for (int j = 0; j < VE; ++j) looked(f.v[j], (uint32_t)(base(e) + j));
         }
       }
     } else {
@@ -394,10 +440,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
       }
       at = s;
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const u64 w = f(v.v[j], (uint32_t)(e + j));
-        acc += e + j < a.V ? w : 0;
-      }
+      for (int j = 0; j < VE; ++j) acc += f(v.v[j], (uint32_t)(e + j));
     });
     if (at >= 0) {
       const u64 r = wave_sum_u64(acc);
@@ -424,12 +467,13 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     if (wave == 0) {
       u64 rest = sh.rest;
       for (int j = 0; j < a.per_seg; ++j) {
-        const int64_t e = (((int64_t)s * a.per_seg + j) * 64 + lane) * VE;
-        const Frag<E> v = widen<E>(load_raw<E, false>(x + (e < a.V ? e : 0), a.V - e, kNone));
+        int32_t e = ((s * a.per_seg + j) * 64 + lane) * VE;
+        const Frag<E> v = values(load(e), e);
+        e = base(e);
         u64 own = 0, w[VE];
 #pragma unroll
         for (int q = 0; q < VE; ++q) {
-          w[q] = e + q < a.V ? f(v.v[q], (uint32_t)(e + q)) : 0;
+          w[q] = f(v.v[q], (uint32_t)(e + q));
           own += w[q];
         }
         const u64 upto = wave_scan_u64(own, lane), all = __shfl(upto, 63, 64);
@@ -468,7 +512,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           const uint32_t key = key_of<E>(v.v[j]);
-          if (e + j < a.V && (bits == kKeyBits<E> || key >> bits == prefix) && in_order(key, (uint32_t)(e + j))) {
+          if ((bits == kKeyBits<E> || key >> bits == prefix) && in_order(v.v[j], (uint32_t)(e + j))) {
             const uint32_t d = key >> shift & ((1u << take_bits) - 1);
             atomicAdd(&sh.radix.count[d], 1u);
             if (by_mass) atomicAdd(&sh.radix.mass[d], weight(v.v[j]));
@@ -506,12 +550,12 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     const u64 of = sh.bin_mass, n_ties = sh.bin_count;
     const u64 each_w = by_mass ? of / n_ties : 1;
     const u64 need = (target - above + each_w - 1) / each_w;
+    const float at = value_of_key<E>(prefix);
     uint32_t id = 0xFFFFFFFFu;
     if (need < n_ties)
-      id = locate([&](float v, uint32_t i) -> u64 { const uint32_t k = key_of<E>(v); return k == prefix && in_order(k, i); },
-                  [&](u64) { return need - 1; });
-    else if (prefix == thr) id = thr_id;
-    thr = prefix, thr_id = id;
+      id = locate([&](float v, uint32_t i) -> u64 { return (v == at) & in_order(v, i); }, [&](u64) { return need - 1; });
+    else if (at == thr) id = thr_id;
+    thr = at, thr_id = id;
   };
 
   // Counts and masses by bins of distance from the maximum; then the bin in which places or mass reach a target, and the threshold from
@@ -525,10 +569,10 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += T) sh.bins.count[i] = 0, sh.bins.mass[i] = 0;
     __syncthreads();
-    each([&](int, int e, const Frag<E>& v) {
+    each([&](int, int, const Frag<E>& v) {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
-        if (e + j < a.V) {
+        if (v.v[j] > kNone) {
           const int b = bin_of(v.v[j]);
           if (by_k) atomicAdd(&sh.bins.count[b], 1u);
           if (with_mass) {
@@ -539,7 +583,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     });
     __syncthreads();
   };
-  // False where too many elements lie in the bin.
+  // False where too many elements lie in the bin.  A target beyond all there is leaves the threshold.
   u64 kept_mass = 0;                               // of the present threshold
   const auto refine = [&](bool by_mass, u64 target) -> bool {
     if (wave == 0) {
@@ -548,6 +592,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
       for (int i = 0; i < N; ++i) own += by_mass ? sh.bins.mass[lane * N + i] : sh.bins.count[lane * N + i];
       for (int i = 0; i < N; ++i) own_mass += sh.bins.mass[lane * N + i];
       const u64 upto = wave_scan_u64(own, lane), upto_mass = wave_scan_u64(own_mass, lane);
+      if (lane == 63) sh.bin = kBins, sh.bin_mass = upto_mass;
       if (upto >= target && upto - own < target) {
         u64 before = upto - own, mass = upto_mass - own_mass;
         for (int i = 0; i < N; ++i) {
@@ -564,11 +609,15 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     __syncthreads();
     const int b = (int)sh.bin;
     const u64 above = sh.above, above_mass = sh.bin_mass;
+    if (b == kBins) {
+      kept_mass = above_mass;
+      return true;
+    }
     list_begin();
     each([&](int, int e, const Frag<E>& v) {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
-        if (e + j < a.V && bin_of(v.v[j]) == b && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) take(v.v[j], (uint32_t)(e + j));
+        if ((v.v[j] > kNone) & (bin_of(v.v[j]) == b) & in_order(v.v[j], (uint32_t)(e + j))) take(v.v[j], (uint32_t)(e + j));
     });
     const int n = list_end();
     if (n > kList) return false;
@@ -582,7 +631,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
       const Candidate c = sh.bins.list[i];
       const u64 from = above + (by_mass ? mass[q] : before[q]), size = by_mass ? c.w : 1;
       if (from < target) part += c.w;
-      if (from < target && target - from <= size) sh.thr = (uint32_t)(c.at >> 32), sh.thr_id = ~(uint32_t)c.at;
+      if (from < target && target - from <= size) sh.thr = value_of_key<E>((uint32_t)(c.at >> 32)), sh.thr_id = ~(uint32_t)c.at;
     }
     kept_mass = above_mass + block_sum(part);
     __syncthreads();
@@ -610,15 +659,14 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
         u64 part = 0;
         each([&](int, int e, const Frag<E>& v) {
 #pragma unroll
-          for (int j = 0; j < VE; ++j)
-            if (e + j < a.V && in_order(key_of<E>(v.v[j]), (uint32_t)(e + j))) part += weight(v.v[j]);
+          for (int j = 0; j < VE; ++j) part += weight(in_order(v.v[j], (uint32_t)(e + j)) ? v.v[j] : kNone);
         });
         kept_mass = block_sum(part);
       }
       if (!done) search(true, share(top_p, kept_mass));
     }
   }
-  const auto kept = [&](float v, uint32_t id) -> u64 { return in_order(key_of<E>(v), id) && near(v) ? weight(v) : 0; };
+  const auto kept = [&](float v, uint32_t id) { return weight(near(v) & in_order(v, id) ? v : kNone); };
   const uint32_t id = locate(kept, place);
   if (threadIdx.x == 0) answer(id, to_f32(x[id]), sh.total);
 }
