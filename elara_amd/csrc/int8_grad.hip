@@ -2,9 +2,8 @@
 // for each row of x or each group of its columns; dW in fp32, [N, K] or transposed.  No counterpart in the reference.
 //
 // x = q scale in bf16 is exact where the scale is a power of two (q has 7 bits, bf16 holds 8), else rounded once to it.  dy in bf16 goes
-// into the products as it is; fp16 values are the sum of two bf16 parts (8 and 3 bits), fp32 values of three (8 bits each), each part
-// what the ones before leave of the value, exactly; so the products are exact and only the fp32 sums round.  Parts of a value that is
-// not finite: the value first, then zeros.
+// into the products as it is; fp16 values are the sum of two bf16 parts (8 and 3 bits), fp32 values of three (8 bits each), so the products
+// are exact and only the fp32 sums round.  (Bits of fp32 values below 2^-133 are lost; an infinity makes its outputs NaN.)
 #include "elr_int8.h"
 
 #include <type_traits>
@@ -26,20 +25,23 @@ struct WgradArgs {
 template <class E>
 constexpr int kParts = Elem<E>::kType == ELR_F32 ? 3 : Elem<E>::kType == ELR_F16 ? 2 : 1;
 
-// The bf16 parts of x, each cut off (not rounded: the largest fp32 values would become infinite); their sum is x.
+// Eight values in P bf16 parts, each cut off (not rounded: the largest fp32 values would become infinite) from what the ones before leave;
+// the parts' sum is the value.  (An infinity leaves a NaN.)
 template <int P>
-__device__ __forceinline__ void split_bf16(float x, __bf16 (&p)[P]) {
-  if constexpr (P == 1) {
-    p[0] = (__bf16)x;
-  } else {
-    const bool finite = __builtin_fabsf(x) < __builtin_inff();
-    p[0] = finite ? __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(x) >> 16)) : (__bf16)x;
-    float rest = x;
+__device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&p)[P]) {
+  float r[8];
 #pragma unroll
-    for (int i = 1; i < P; ++i) {
-      rest = finite ? rest - (float)p[i - 1] : 0.0f;
-      p[i] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(rest) >> 16));
-    }
+  for (int j = 0; j < 8; ++j) r[j] = x[j];
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)      // the high halves of two
+      w[j] = __builtin_amdgcn_perm(__float_as_uint(r[2 * j + 1]), __float_as_uint(r[2 * j]), 0x07060302u);
+    p[k] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + 1 < P) r[j] = r[j] - __uint_as_float(__float_as_uint(r[j]) & 0xFFFF0000u);
   }
 }
 
@@ -95,7 +97,7 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-// Tiles of BM x BN of dW, 32 tokens a step, two LDS buffers; the rows of the next two steps are on their way into registers, from where
+// Tiles of BM x BN of dW, BT tokens a step, two LDS buffers; the rows of the next AHEAD steps are on their way into registers, from where
 // they go, in bf16, into the buffer that is not multiplied.  WM x WN waves, each a part of the tile in products of 32 x 32 x 16.
 // Rows in LDS are 64 bytes longer than the tile's: two neighbouring blocks of 4 tokens x 16 columns then take all 64 banks once.
 //
@@ -103,7 +105,7 @@ __device__ __forceinline__ void interleave() {
 // within is loaded from 8 columns before the end on, and its own columns are then stored again in their place; pieces past the end are
 // loaded from there too: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
 // NARROW: a matrix of less than 8 columns, or with rows far apart, loaded with checks.
-template <class E, int BM, int BN, int BT, int WM, int WN, bool NARROW>
+template <class E, int BM, int BN, int BT, int WM, int WN, int AHEAD, bool NARROW>
 __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
   constexpr int P = kParts<E>, T = WM * WN * 64, PM = BM + 32, PN = BN + 32;
   constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
@@ -199,17 +201,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
       if constexpr (P == 1) {
         w.y[r][0] = __builtin_bit_cast(bf16x8, g.y[r].v[0]);
       } else {
+        float v[8];
 #pragma unroll
         for (int i = 0; i < 8 / Elem<E>::VE; ++i) {
           const Frag<E> f = widen<E>(g.y[r].v[i]);
 #pragma unroll
-          for (int j = 0; j < Elem<E>::VE; ++j) {
-            __bf16 part[P];
-            split_bf16<P>(f.v[j], part);
-#pragma unroll
-            for (int k = 0; k < P; ++k) w.y[r][k][i * Elem<E>::VE + j] = part[k];
-          }
+          for (int j = 0; j < Elem<E>::VE; ++j) v[i * Elem<E>::VE + j] = f.v[j];
         }
+        split_bf16<P>(v, w.y[r]);
       }
     }
 #pragma unroll
@@ -274,21 +273,28 @@ __global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t til
     }
   };
   if (from < to) {
-    Step g;
-    load(g, 0);
-    store(convert(g, 0), 0);
+    Step g[AHEAD];
+    load(g[0], 0);
+    store(convert(g[0], 0), 0);
+#pragma unroll
+    for (int s = 1; s < AHEAD; ++s) load(g[s], s * BT);
     __syncthreads();
     constexpr int kProducts = MT * NT * P * BT / 32, kReads = (MT * P + NT) * BT / 16;      // of half a step
     int buf = 0;
-    for (int32_t i = 0; i <= last; i += BT, buf ^= 1) {
-      load(g, i + BT);
-      multiply(buf, 0);
-      interleave<kProducts, kReads, 0>();
-      const Rows w = convert(g, i + BT);
-      multiply(buf, 1);
-      interleave<kProducts, kReads, (RX * 28 + (P > 1 ? RY * 16 * P : 0) + kProducts - 1) / kProducts>();
-      store(w, buf ^ 1);
-      __syncthreads();
+    for (int32_t i0 = 0; i0 <= last; i0 += AHEAD * BT) {
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s, buf ^= 1) {      // (steps past the end multiply zeros)
+        const int32_t i = i0 + s * BT;
+        load(g[s], i + AHEAD * BT);
+        multiply(buf, 0);
+        interleave<kProducts, kReads, 0>();
+        Step& next = g[(s + 1) % AHEAD];
+        const Rows w = convert(next, i + BT);
+        multiply(buf, 1);
+        interleave<kProducts, kReads, (RX * 28 + (P > 1 ? RY * 16 * P : 0) + kProducts - 1) / kProducts>();
+        store(w, buf ^ 1);
+        __syncthreads();
+      }
     }
   }
   float* out = a.out + (int64_t)blockIdx.z * a.N * a.K;
@@ -345,21 +351,22 @@ constexpr int64_t kNearRows = 1 << 24;      // strides of rows whose 32 lie with
 template <class E, int B, int BT>
 constexpr int kWgradLds = 2 * (kParts<E> + 1) * BT * (B + 32) * 2;
 
-template <class E, int B, int BT, int WM, int WN>
+template <class E, int B, int BT, int WM, int WN, int AHEAD>
 static void launch_wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
   static_assert(kWgradLds<E, B, BT> <= 160 << 10, "LDS of a CU");
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits);
-  k_wgrad<E, B, B, BT, WM, WN, false><<<grid, WM * WN * 64, kWgradLds<E, B, BT>, st>>>(a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
+  k_wgrad<E, B, B, BT, WM, WN, AHEAD, false><<<grid, WM * WN * 64, kWgradLds<E, B, BT>, st>>>(a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
 }
 
 template <class E>
 static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
+  constexpr int AH = 2;
   if (a.N < 8 || a.K < 8 || a.dy_ld > kNearRows || a.q_ld > kNearRows)
-    k_wgrad<E, 128, 128, 32, 2, 2, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128, 32>, st>>>(
+    k_wgrad<E, 128, 128, 32, 2, 2, 1, true><<<dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits), 256, kWgradLds<E, 128, 32>, st>>>(
         a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
   else if constexpr (kParts<E> == 1)
-    p.tile == 256 ? launch_wgrad<E, 256, 64, 2, 4>(a, p, st) : launch_wgrad<E, 128, 32, 2, 2>(a, p, st);
-  else launch_wgrad<E, 128, 32, 2, 2>(a, p, st);
+    p.tile == 256 ? launch_wgrad<E, 256, 64, 2, 4, 1>(a, p, st) : launch_wgrad<E, 128, 32, 2, 2, AH>(a, p, st);
+  else launch_wgrad<E, 128, 32, 2, 2, AH>(a, p, st);
 }
 
 }  // namespace elr
