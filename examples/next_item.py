@@ -11,9 +11,14 @@ One training step, and what runs it:
   clipping over all gradients          gradnorm.clip_grad_norm, 16-bit gradients into the fp32 that Adam reads
   update                               ops.gpu_adam (the batch's rows), ops.adam_rows_dense (the dense weights)
 
-Serving scores one session: rms_norm_fp8 before the output product and token_logprobs for the likeliest items.
+With keep8 the norms' inputs and outputs are kept for the backward pass in 8 bits (int8.quantize with power-of-two scales), and the
+backward pass reads them so: norms.rms_norm_backward_int8 and int8.weight_grad.  (The inner activation stays as it is: where it is
+positive has to be known exactly.)
 
-    python examples/next_item.py [--items 20000 --width 256 --batch 64 --length 32 --steps 100]
+Serving scores one session: rms_norm_fp8 before the output product and token_logprobs for the likeliest items; or draws its next item:
+the output product in 8-bit integers (int8.linear) and sampling.sample_tokens.
+
+    python examples/next_item.py [--items 20000 --width 256 --batch 64 --length 32 --steps 100 --keep8]
 
 The data is synthetic: sessions that walk the items by a fixed rule and jump at random now and then.
 """
@@ -26,19 +31,21 @@ from pathlib import Path
 import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
-from elara_amd import dedup, gradnorm, logprobs, norms, ops, synth  # noqa: E402
+from elara_amd import dedup, gradnorm, int8, logprobs, norms, ops, sampling, synth  # noqa: E402
 from elara_amd.gpu_ops import init_rows  # noqa: E402
 
 EPS = 1e-6
+GROUP = 128      # columns of a scale of what is kept in 8 bits
 
 
 class NextItem:
     """Weights are the w of (w, m, v) records, [rows, 3, width] fp32; activations and products have `dtype`."""
 
     def __init__(self, items, width, hidden=None, layers=2, dtype=torch.bfloat16, lr=1e-3, max_norm=1.0, entropy=1e-3,
-                 device='cuda:0', seed=0):
+                 device='cuda:0', seed=0, keep8=False):
         hidden = hidden or 2 * width
         self.items, self.dtype, self.hp, self.max_norm, self.beta = items, dtype, (lr, 0.9, 0.999, 1e-8), max_norm, entropy
+        self.keep8 = keep8
         dev = torch.device(device)
 
         def records(rows, cols, bound, first):
@@ -76,6 +83,8 @@ class NextItem:
             a, b = self._weight(w1), self._weight(w2)
             u = torch.relu(n.y @ a)
             add = u @ b
+            if self.keep8:
+                n = norms.Norm(int8.quantize(n.y, GROUP, pow2=True), int8.quantize(h, GROUP, pow2=True), n.rstd)
             kept.append((n, a, b, u))
         return add, h, kept
 
@@ -97,8 +106,12 @@ class NextItem:
             nrm, a, b, u = kept[i]
             db = u.t() @ dh
             du = (dh @ b.t()) * (u > 0)
-            da = nrm.y.t() @ du
-            dh, d_gain = norms.rms_norm_backward(du @ a.t(), nrm.h, self._gain(i), nrm.rstd, dh=dh)
+            if self.keep8:
+                da = int8.weight_grad(du, nrm.y, transposed=True)
+                dh, d_gain = norms.rms_norm_backward_int8(du @ a.t(), nrm.h, self._gain(i), nrm.rstd, dh=dh)
+            else:
+                da = nrm.y.t() @ du
+                dh, d_gain = norms.rms_norm_backward(du @ a.t(), nrm.h, self._gain(i), nrm.rstd, dh=dh)
             pairs = [da, db] + pairs
             gains = [d_gain] + gains
         rows, inverse = dedup.unique(ids, bound=self.items)
@@ -126,6 +139,18 @@ class NextItem:
         return r.top_id, r.top_logprob
 
 
+    def head8(self):
+        """The output weight in 8-bit integers with a scale for each item: made once for many draws."""
+        return int8.quantize(self._weight(self.head))
+
+    def draw(self, ids, u, head8, **settings):
+        """An item after each id, drawn with the numbers u [n] in [0, 1) and sampling.sample_tokens' settings, and its log
+        probability."""
+        add, h, _ = self.forward(ids)
+        x = int8.quantize(norms.rms_norm(add, self._gain(-1), EPS, residual=h).y)
+        return sampling.sample_tokens(int8.linear(x, head8, dtype=self.dtype), u, **settings)
+
+
 def sessions(gen, items, batch, length, jump=0.1):
     """[batch, length + 1] items: each follows from the one before by a fixed rule, or is a jump anywhere."""
     x = torch.empty(batch, length + 1, dtype=torch.int64)
@@ -145,9 +170,10 @@ def main(argv=None):
     ap.add_argument('--length', type=int, default=32)
     ap.add_argument('--steps', type=int, default=100)
     ap.add_argument('--lr', type=float, default=2e-3)
+    ap.add_argument('--keep8', action='store_true', help='keep the norms\' inputs and outputs in 8 bits for the backward pass')
     a = ap.parse_args(argv)
     gen = torch.Generator().manual_seed(0)
-    model = NextItem(a.items, a.width, lr=a.lr)
+    model = NextItem(a.items, a.width, lr=a.lr, keep8=a.keep8)
     losses, began = [], None
     for s in range(a.steps):
         x = sessions(gen, a.items, a.batch, a.length).cuda()
@@ -166,6 +192,8 @@ def main(argv=None):
     top, lp = model.likeliest(ids)
     for i, t, p in zip(ids.tolist(), top.tolist(), lp.tolist()):
         print(f'after item {i} (by the rule {(3 * i + 7) % a.items}): {t}  log probabilities {[round(v, 3) for v in p]}')
+    drawn = model.draw(ids.repeat(4), torch.rand(12, generator=gen).cuda(), model.head8(), temperature=0.8, top_k=50, top_p=0.95)
+    print(f'four draws after each: {drawn.token.view(4, 3).t().tolist()}')
     return [float(v) for v in losses]
 
 
