@@ -106,7 +106,7 @@ __device__ __forceinline__ void interleave() {
 // loaded from there too: what LDS holds in their place reaches outputs past the end alone.  Tokens past the end are loaded from the last one and zeroed.
 // NARROW: a matrix of less than 8 columns, or with rows far apart, loaded with checks.
 template <class E, int BM, int BN, int BT, int WM, int WN, int AHEAD, bool NARROW>
-__global__ __launch_bounds__(WM * WN * 64) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
+__global__ __launch_bounds__(WM * WN * 64, BM == 128 && WM * WN == 8 ? 4 : 1) void k_wgrad(WgradArgs a, int32_t tiles_m, int32_t tiles_n) {
   constexpr int P = kParts<E>, T = WM * WN * 64, PM = BM + 32, PN = BN + 32;
   constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
   constexpr int RY = BT * BM / 8 / T, RX = BT * BN / 8 / T;       // row pieces of 8 of a thread
@@ -386,7 +386,7 @@ static void wgrad(const WgradArgs& a, const WgradPlan& p, hipStream_t st) {
         a, (int32_t)p.tiles_m, (int32_t)p.tiles_n);
   else if constexpr (kParts<E> == 1)
     p.tile == 256 ? launch_wgrad<E, 256, 64, 2, 4, 1>(a, p, st) : launch_wgrad<E, 128, 32, 2, 2, AH>(a, p, st);
-  else launch_wgrad<E, 128, 32, 2, 2, AH>(a, p, st);
+  else launch_wgrad<E, 128, 32, 4, 2, AH>(a, p, st);
 }
 
 }  // namespace elr
