@@ -206,7 +206,7 @@ __global__ __launch_bounds__(512) void k_linear_few(LinearArgs a, int32_t kw) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) w[u][i] = __builtin_bit_cast(i32x4, __builtin_nontemporal_load((const u32x4_b*)(pw[i] + k + u * 64)));
+        for (int i = 0; i < C; ++i) w[u][i] = __builtin_bit_cast(i32x4, *(const u32x4_b*)(pw[i] + k + u * 64));
 #pragma unroll
         for (int t = 0; t < TB; ++t) x[u][t] = __builtin_bit_cast(i32x4, *(const u32x4_b*)(px[t] + k + u * 64));
       }
