@@ -109,6 +109,7 @@ struct SampleShared {
       uint32_t count[kBins];
       Candidate list[kList];
     } bins;
+    float step_max[kSegs];      // of a wave's vectors at a time (before the bins are filled)
   };
   u64 seg[kSegs];
   float fmax[16];
@@ -198,10 +199,21 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
       own_max = max_nan(own_max, vec_max[i]);
     }
   } else {
-    each([&](int, int, const Frag<E>& f) {
+    for (int s = wave; s * 64 * VE < a.V;) {          // eight vectors on their way
+      u32x4 v[8];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) own_max = max_nan(own_max, f.v[j]);
-    });
+      for (int i = 0; i < 8; ++i) v[i] = load(((s + i * W) * 64 + lane) * VE);
+#pragma unroll
+      for (int i = 0; i < 8; ++i, s += W) {
+        const Frag<E> f = values(v[i], (s * 64 + lane) * VE);
+        float vm = f.v[0];
+#pragma unroll
+        for (int j = 1; j < VE; ++j) vm = max_nan(vm, f.v[j]);
+        own_max = max_nan(own_max, vm);
+        vm = lanes_max_nan(vm, 64);
+        if (lane == 0 && s < kSegs) sh.step_max[s] = vm;
+      }
+    }
   }
   float m = lanes_max_nan(own_max, 64);
   if constexpr (T > 64) {
@@ -364,10 +376,13 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
         }
       }
     } else {
-      each([&](int, int e, const Frag<E>& v) {
+      for (int s = wave; s * 64 * VE < a.V; s += W)    // (the steps whose maximum reaches the bound are read again)
+        if (s >= kSegs || sh.step_max[s] >= bound) {
+          const int32_t e = (s * 64 + lane) * VE;
+          const Frag<E> f = values(load(e), e);
 #pragma unroll
-        for (int j = 0; j < VE; ++j) looked(v.v[j], (uint32_t)(e + j));
-      });
+          for (int j = 0; j < VE; ++j) looked(f.v[j], (uint32_t)(base(e) + j));
+        }
     }
     const int n = list_end();
     if (n <= kList) {
