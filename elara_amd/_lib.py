@@ -108,9 +108,7 @@ SIGNATURES = {
                                              c_i64, c_vp, ctypes.c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     'elr_quantize_int8': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_vp, c_vp, c_vp]),
     'elr_dequantize_int8': (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, ctypes.c_int, c_vp]),
-    'elr_int8_linear_scratch_bytes': (c_i64, [c_i64, c_i64, c_i64]),
-    'elr_int8_linear': (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, ctypes.c_int, c_vp,
-                                       c_i64, c_vp]),
+    'elr_int8_linear': (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, ctypes.c_int, c_vp]),
     'elr_int8_weight_grad_scratch_bytes': (c_i64, [c_i64, c_i64, c_i64, ctypes.c_int]),
     'elr_int8_weight_grad': (ctypes.c_int, [c_vp, ctypes.c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp,
                                             ctypes.c_int, c_vp, c_i64, c_vp]),
@@ -290,8 +288,8 @@ def host():
                 'rms_norm_backward_scratch_bytes', 'rms_norm_backward', 'grad_norm_scratch_bytes', 'grad_norm',
                 'clip_grad_norm')))
             h.bind_int8(*(ctypes.cast(getattr(L, 'elr_' + f), c_vp).value for f in (
-                'quantize_int8', 'dequantize_int8', 'int8_linear_scratch_bytes', 'int8_linear', 'int8_weight_grad_scratch_bytes',
-                'int8_weight_grad', 'rms_norm_backward_int8', 'sample_tokens')))
+                'quantize_int8', 'dequantize_int8', 'int8_linear', 'int8_weight_grad_scratch_bytes', 'int8_weight_grad',
+                'rms_norm_backward_int8', 'sample_tokens')))
         except ImportError as e:
             warnings.warn(f'elara_amd._hostcall is not used (small row-op calls take several microseconds longer): {e}',
                           stacklevel=3)

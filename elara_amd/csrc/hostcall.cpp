@@ -539,7 +539,6 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t na) {
 
 decltype(&elr_quantize_int8) f_quantize = nullptr;
 decltype(&elr_dequantize_int8) f_dequantize = nullptr;
-decltype(&elr_int8_linear_scratch_bytes) f_linear_bytes = nullptr;
 decltype(&elr_int8_linear) f_linear = nullptr;
 decltype(&elr_int8_weight_grad_scratch_bytes) f_wgrad_bytes = nullptr;
 decltype(&elr_int8_weight_grad) f_wgrad = nullptr;
@@ -547,12 +546,11 @@ decltype(&elr_rms_norm_backward_int8) f_norm_back8 = nullptr;
 decltype(&elr_sample_tokens) f_sample = nullptr;
 
 PyObject* bind_int8(PyObject*, PyObject* args) {
-  unsigned long long a[8];
-  if (!PyArg_ParseTuple(args, "KKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7)) return nullptr;
-  set_address(f_quantize, a[0]), set_address(f_dequantize, a[1]);
-  set_address(f_linear_bytes, a[2]), set_address(f_linear, a[3]);
-  set_address(f_wgrad_bytes, a[4]), set_address(f_wgrad, a[5]);
-  set_address(f_norm_back8, a[6]), set_address(f_sample, a[7]);
+  unsigned long long a[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6)) return nullptr;
+  set_address(f_quantize, a[0]), set_address(f_dequantize, a[1]), set_address(f_linear, a[2]);
+  set_address(f_wgrad_bytes, a[3]), set_address(f_wgrad, a[4]);
+  set_address(f_norm_back8, a[5]), set_address(f_sample, a[6]);
   Py_RETURN_NONE;
 }
 
@@ -653,10 +651,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t na) {
         std::vector<int64_t> shape(x.q->sizes().begin(), x.q->sizes().end());
         shape.back() = w.n;
         y = empty_on(*x.q, shape, scalar_type_of(type));
-        const int64_t bytes = f_linear_bytes(x.n, w.n, x.D);
-        const at::Tensor scratch = scratch_on(*x.q, bytes);
         rc = f_linear(x.data(), x.n, x.D, x.D, floats(x.scale), w.data(), w.n, w.D, floats(w.scale), y.data_ptr(),
-                      static_cast<int>(type), data_or_null(scratch), bytes, st);
+                      static_cast<int>(type), st);
       }
     }
     if (rc == kNotTaken) return not_taken();

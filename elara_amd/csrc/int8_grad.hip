@@ -409,6 +409,7 @@ extern "C" int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t
     return ELR_EINVAL;
   const WgradPlan plan = wgrad_plan(n, N, K, type);
   const int64_t splits = plan.splits;
+  if (n / splits >= (int64_t)1 << 30) return ELR_EUNSUPPORTED;
   if (splits > 1 && (!scratch || scratch_bytes < splits * N * K * 4 || ((uintptr_t)scratch & 3u))) return ELR_ECAPACITY;
   const WgradArgs a{dy, q, scale, dy_ld, q_ld, n, ((n + splits - 1) / splits + 31) / 32 * 32, (int32_t)N, (int32_t)K,
                     (int32_t)int8_groups(K, group), int8_shift(group), splits > 1 ? (float*)scratch : dw, transposed};

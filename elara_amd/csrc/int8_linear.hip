@@ -396,17 +396,11 @@ static void linear(const LinearArgs& b, hipStream_t st) {
 
 }  // namespace elr
 
-extern "C" int64_t elr_int8_linear_scratch_bytes(int64_t n, int64_t N, int64_t K) {
-  if (n < 0 || N < 0 || K < 0) return -1;
-  return 0;
-}
-
 extern "C" int elr_int8_linear(const int8_t* x, int64_t n, int64_t K, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t N,
-                               int64_t w_ld, const float* w_scale, void* y, int type, void* scratch, int64_t scratch_bytes,
-                               void* stream) {
+                               int64_t w_ld, const float* w_scale, void* y, int type, void* stream) {
   using namespace elr;
   if (n < 0 || N < 0 || K < 0 || x_ld < 0 || w_ld < 0 || !elem_type_ok(type)) return ELR_EINVAL;
-  if (K >= 1 << 17 || N > (int64_t)1 << 31) return ELR_EUNSUPPORTED;
+  if (K >= 1 << 17 || N > (int64_t)1 << 30) return ELR_EUNSUPPORTED;
   if (n == 0 || N == 0) return ELR_OK;
   if (!x_scale || !w_scale || !y || (K > 0 && (!x || !w)) || !elem_aligned(y, type) ||
       (((uintptr_t)x_scale | (uintptr_t)w_scale) & 3u))

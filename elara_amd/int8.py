@@ -124,14 +124,11 @@ def linear(x, w, dtype=torch.bfloat16):
     if K > K_MOST:
         raise RuntimeError(f'K must be at most {K_MOST}, got {K}')
     dev = xq.device
-    L = _lib.lib()
     y = torch.empty(x.q.shape[:-1] + (N,), dtype=dtype, device=dev)
     if n and N:
-        nbytes = L.elr_int8_linear_scratch_bytes(n, N, K)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _lib.on_device(dev):
-            rc = L.elr_int8_linear(xq.data_ptr(), n, K, x_ld, xs.data_ptr(), wq.data_ptr(), N, w_ld, ws.data_ptr(), y.data_ptr(),
-                                   _lib.ETYPE[dtype], _lib.ptr(scratch), nbytes, _lib.raw_stream(dev))
+            rc = _lib.lib().elr_int8_linear(xq.data_ptr(), n, K, x_ld, xs.data_ptr(), wq.data_ptr(), N, w_ld, ws.data_ptr(),
+                                            y.data_ptr(), _lib.ETYPE[dtype], _lib.raw_stream(dev))
         _lib.check(rc, 'elr_int8_linear')
     return y
 
@@ -140,7 +137,7 @@ def weight_grad(dy, x, transposed=False):
     """dy [..., N] cuda float32/float16/bfloat16 (any row stride): the gradient of x W^T; x: Int8Rows [..., K], the layer's input
     as it was kept (scales by row or by group).  Returns dy^T x, float32 [N, K], or [K, N] with transposed (the gradient of a weight
     that multiplies from the right).  dy is not rounded; x is q * scale in bfloat16, exact where the scales are powers of two; sums
-    are float32 in an order that depends on the sizes alone."""
+    are float32 in an order that depends on the sizes alone.  An infinity in dy leaves NaN or infinities in its row of dy^T x."""
     r = (_lib._host or _lib.host()).weight_grad(dy, *x, int(transposed))
     if r != _lib.NOT_TAKEN:
         _lib.check(r[0], 'elr_int8_weight_grad')

@@ -7,6 +7,7 @@ It runs the HIP kernel behind elr_sample_tokens (elara_amd/csrc/sampling.hip) on
 host synchronisation.  The numbers are the caller's (torch.rand with a generator of its own), so a draw can be repeated; the same
 inputs give the same ids on every call.
 """
+import operator
 from typing import NamedTuple
 
 import torch
@@ -21,12 +22,16 @@ class Sample(NamedTuple):
 
 
 def _setting(v, u, name, dtypes, low, high):
-    """(value, None) for a number in [low, high], (0, tensor) for one value a row."""
+    """(value, None) for a number in [low, high] (a whole one for integer types), (0, tensor) for one value a row."""
     if torch.is_tensor(v):
         if not (v.is_cuda and v.device == u.device and v.dtype in dtypes and v.shape == u.shape):
             raise RuntimeError(f'{name} must be a number or a cuda {" or ".join(map(str, dtypes))} tensor of shape '
                                f'{tuple(u.shape)} on {u.device}')
         return 0, v.contiguous()
+    try:
+        v = float(v) if dtypes == (torch.float32,) else operator.index(v)
+    except (TypeError, ValueError):
+        raise RuntimeError(f'{name} must be {"a number" if dtypes == (torch.float32,) else "a whole number"}, got {v!r}') from None
     if not low <= v <= high:
         raise RuntimeError(f'{name} must lie in [{low}, {high}], got {v}')
     return v, None
@@ -65,7 +70,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if n:
         with _lib.on_device(dev):
             rc = _lib.lib().elr_sample_tokens(
-                x.data_ptr(), _lib.ETYPE[x.dtype], n, V, _ld(x), un.data_ptr(), temp, _lib.ptr(temps), int(k), _lib.ptr(ks),
+                x.data_ptr(), _lib.ETYPE[x.dtype], n, V, _ld(x), un.data_ptr(), temp, _lib.ptr(temps), k, _lib.ptr(ks),
                 int(ks is not None and ks.dtype == torch.int64), p, _lib.ptr(ps), mp, _lib.ptr(mps), token.data_ptr(),
                 logprob.data_ptr(), _lib.raw_stream(dev))
         _lib.check(rc, 'elr_sample_tokens')

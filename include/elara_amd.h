@@ -804,18 +804,15 @@ int elr_dequantize_int8(const int8_t* q, int64_t n, int64_t D, int64_t q_ld, int
 /* y[i, j] = x_scale[i] w_scale[j] sum_k x[i, k] w[j, k]: the product of int8 rows x [n, K] with an int8 weight w [N, K], a
  * scale for each token and each channel.  The sum is exact (int32: K < 2^17, else ELR_EUNSUPPORTED), then widened to fp32,
  * multiplied by x_scale and by w_scale and rounded to `type`.  Rows of x and w x_ld and w_ld bytes apart; y [n, N]
- * contiguous, not overlapping x or w.  K = 0 gives zeros times the scales.  scratch of
- * elr_int8_linear_scratch_bytes(n, N, K) bytes, 16-byte aligned (may be 0; -1: bad argument). */
-int64_t elr_int8_linear_scratch_bytes(int64_t n, int64_t N, int64_t K);
+ * contiguous, not overlapping x or w.  K = 0 gives zeros times the scales. */
 int elr_int8_linear(const int8_t* x, int64_t n, int64_t K, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t N,
-                    int64_t w_ld, const float* w_scale, void* y, int type, void* scratch, int64_t scratch_bytes,
-                    void* stream);
+                    int64_t w_ld, const float* w_scale, void* y, int type, void* stream);
 
 /* The weight gradient of a linear layer from its input kept in 8-bit integers: dw[j, k] = sum_i dy[i, j] x[i, k], x = q scale
  * in bf16 (exact where the scales are powers of two), dy (of `type`) unrounded, sums in fp32 in an order that depends on the
  * sizes alone.  dw fp32 [N, K], or [K, N] with transposed, contiguous; n = 0 gives zeros.  Rows of dy dy_ld elements, of q
- * q_ld bytes apart; scales as above, over K.  scratch of elr_int8_weight_grad_scratch_bytes bytes, 16-byte aligned (may be
- * 0; -1: bad argument). */
+ * q_ld bytes apart; scales as above, over K.  An infinity in dy makes its outputs NaN (fp32, fp16) or what the products give
+ * (bf16).  scratch of elr_int8_weight_grad_scratch_bytes bytes, 4-byte aligned (may be 0; -1: bad argument). */
 int64_t elr_int8_weight_grad_scratch_bytes(int64_t n, int64_t N, int64_t K, int type);
 int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t N, int64_t dy_ld, const int8_t* q, int64_t K,
                          int64_t q_ld, int64_t group, const float* scale, float* dw, int transposed, void* scratch,

@@ -196,7 +196,8 @@ def check_linear(dev, xq, wq, dtype, xs=None, ws=None):
 SHAPES = [(1, 1, 1), (1, 7, 16), (2, 64, 64), (3, 130, 17), (4, 256, 4096), (5, 33, 100), (8, 1000, 256), (15, 129, 1000),
           (16, 512, 2048), (17, 513, 333), (31, 65, 128), (33, 64, 15), (48, 200, 96), (64, 300, 512), (65, 257, 250),
           (100, 1024, 64), (127, 127, 127), (128, 128, 128), (129, 1000, 1000), (255, 256, 4096), (256, 300, 192),
-          (300, 20_011, 100), (513, 515, 1024), (1000, 700, 4097), (2048, 2048, 512)]
+          (300, 20_011, 100), (513, 515, 1024), (1000, 700, 4097), (2048, 2048, 512), (3000, 4100, 144), (12_001, 1027, 80),
+          (4099, 3333, 400)]
 
 
 @pytest.mark.gpu
@@ -209,7 +210,7 @@ def test_linear(dev, n, N, K, dtype):
 @pytest.mark.gpu
 def test_linear_places_of_every_product(dev):
     """One value a row at a place of its own: each output is one product, so a misplaced lane or column shows."""
-    for n, N, K in ((1, 300, 1024), (16, 272, 512), (64, 300, 320), (200, 260, 384), (300, 520, 1040)):
+    for n, N, K in ((1, 300, 1024), (16, 272, 512), (64, 300, 320), (200, 260, 384), (300, 520, 1040), (3300, 3900, 272)):
         xq = torch.zeros(n, K, dtype=torch.int8)
         xq[torch.arange(n), (torch.arange(n) * 37 + 5) % K] = (torch.arange(n) % 127 + 1).to(torch.int8)
         check_linear(dev, xq, _int_rows(3, N, K), torch.float32)
@@ -296,7 +297,8 @@ def check_wgrad(dev, dy, q, scale, group, transposed=False):
 
 
 WSHAPES = [(1, 1, 1), (1, 64, 64), (2, 3, 100), (7, 65, 33), (31, 64, 128), (32, 130, 64), (33, 127, 129), (64, 256, 256),
-           (100, 500, 100), (129, 96, 1000), (300, 513, 257), (1000, 64, 64), (2048, 256, 512), (5001, 100, 200), (9000, 64, 40)]
+           (100, 500, 100), (129, 96, 1000), (300, 513, 257), (1000, 64, 64), (2048, 256, 512), (5001, 100, 200), (9000, 64, 40), (200, 3500, 3601), (77, 4096, 3841),
+           (65, 12_300, 1030), (16_000, 16, 24)]
 
 
 @pytest.mark.gpu
@@ -317,7 +319,7 @@ def test_weight_grad(dev, n, N, K, dtype):
 def test_weight_grad_places(dev, dtype):
     """One token: an outer product, each of its values exact."""
     i8 = _i8()
-    for N, K, at, n in ((300, 260, 0, 1), (64, 70, 33, 40), (257, 129, 77, 300)):
+    for N, K, at, n in ((300, 260, 0, 1), (64, 70, 33, 40), (257, 129, 77, 300), (3600, 3590, 70, 130)):
         q = torch.zeros(n, K, dtype=torch.int8)
         q[at] = (torch.arange(K) % 127 + 1).to(torch.int8)
         dy = torch.zeros(n, N, dtype=dtype)
@@ -528,6 +530,45 @@ def test_streams_and_graphs(dev):
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls in flight together share nothing, workspaces included."""
+    i8 = _i8()
+    dy = [torch.randn(6000, 96, device=dev) for _ in range(2)]
+    k = [i8.quantize(torch.randn(6000, 200, device=dev), group=32, pow2=True) for _ in range(2)]
+    w = i8.quantize(torch.randn(150, 200, device=dev))
+    alone = [(i8.weight_grad(dy[i], k[i]), i8.linear(i8.quantize(dy[i].repeat(1, 3)[:, :200].contiguous()), w)) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((i8.weight_grad(dy[i], k[i]), i8.linear(i8.quantize(dy[i].repeat(1, 3)[:, :200].contiguous()), w)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, alone[i][0]) and torch.equal(b, alone[i][1])
+
+
+@pytest.mark.gpu
+def test_rows_of_one_dimension(dev):
+    """One row without a leading dimension, through every call."""
+    from elara_amd import norms
+    i8 = _i8()
+    x, dy = torch.randn(96, device=dev).bfloat16(), torch.randn(40, device=dev).bfloat16()
+    r, w = i8.quantize(x, group=32, pow2=True), i8.quantize(torch.randn(40, 96, device=dev))
+    y = i8.linear(i8.quantize(x), w)
+    assert y.shape == (40,) and torch.equal(y, i8.linear(i8.quantize(x[None]), w)[0])
+    dw = i8.weight_grad(dy, r)
+    assert torch.equal(dw, i8.weight_grad(dy[None], i8.Int8Rows(r.q[None], r.scale[None], 32))) and dw.shape == (40, 96)
+    g, rstd = torch.rand(96, device=dev), torch.tensor(0.7, device=dev)
+    dx, dg = norms.rms_norm_backward_int8(x, r, g, rstd)
+    two = norms.rms_norm_backward_int8(x[None], i8.Int8Rows(r.q[None], r.scale[None], 32), g, rstd[None])
+    assert torch.equal(dx, two[0][0]) and torch.equal(dg, two[1])
+
+
+@pytest.mark.gpu
 def test_repeats_are_bitwise_equal(dev):
     i8 = _i8()
     q, s = ref_quantize(_randn(1, 6000, 128), 64, True)
@@ -555,10 +596,9 @@ def test_refusals_of_the_c_entry_points():
     assert L.elr_dequantize_int8(p, 1, 8, -1, 0, p, p, 0, None) == -1
     assert L.elr_dequantize_int8(p, 1, 8, 8, 0, None, p, 0, None) == -1
     assert L.elr_dequantize_int8(None, 0, 8, 8, 0, None, None, 0, None) == 0
-    assert L.elr_int8_linear_scratch_bytes(-1, 1, 1) == -1 and L.elr_int8_linear_scratch_bytes(8, 8, 8) >= 0
-    lin = lambda n, K, N, x=p, y=p, t=0: L.elr_int8_linear(x, n, K, K, p, p, N, K, p, y, t, p, 1 << 40, None)  # noqa: E731
+    lin = lambda n, K, N, x=p, y=p, t=0: L.elr_int8_linear(x, n, K, K, p, p, N, K, p, y, t, None)  # noqa: E731
     assert lin(-1, 8, 8) == -1 and lin(1, -8, 8) == -1 and lin(1, 8, 8, t=3) == -1
-    assert lin(1, 1 << 17, 8) == -2
+    assert lin(1, 1 << 17, 8) == -2 and lin(1, 8, (1 << 30) + 1) == -2
     assert lin(1, 8, 8, x=None) == -1 and lin(1, 8, 8, y=None) == -1 and lin(1, 8, 8, y=ctypes.c_void_p(258)) == -1
     assert lin(0, 8, 8, x=None, y=None) == 0 and lin(1, 8, 0, y=None) == 0
     assert L.elr_int8_weight_grad_scratch_bytes(1, 1, 1, 7) == -1

@@ -251,6 +251,35 @@ def test_strides_shapes_and_empty(dev):
 
 
 @pytest.mark.gpu
+def test_numbers_of_other_types(dev):
+    import numpy as np
+    sp = _sp()
+    x, u = _logits(8, 5, 700, torch.float32).to(dev), torch.rand(5, device=dev)
+    a = sp.sample_tokens(x, u, temperature=0.5, top_k=9, top_p=0.75, min_p=0.25)
+    b = sp.sample_tokens(x, u, temperature=np.float32(0.5), top_k=np.int32(9), top_p=np.float64(0.75), min_p=np.float16(0.25))
+    assert torch.equal(a.token, b.token) and torch.equal(a.logprob, b.logprob)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls in flight together share nothing."""
+    sp = _sp()
+    xs = [_logits(20 + i, 300, 9000, torch.bfloat16).to(dev) for i in range(2)]
+    u = torch.rand(300, device=dev)
+    alone = [sp.sample_tokens(x, u, top_k=1000, top_p=0.9).token for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(sp.sample_tokens(xs[i], u, top_k=1000, top_p=0.9).token)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, alone[i]) for i in range(2) for t in got[i])
+
+
+@pytest.mark.gpu
 def test_streams_graphs_and_repeats(dev):
     sp = _sp()
     x = [_logits(7 + i, 20, 6000, torch.float16).to(dev) for i in range(2)]
@@ -334,6 +363,7 @@ def test_refusals(dev):
            lambda: sp.sample_tokens(x, u, temperature=float('nan')), lambda: sp.sample_tokens(x, u, temperature=float('inf')),
            lambda: sp.sample_tokens(x, u, top_k=-1), lambda: sp.sample_tokens(x, u, top_p=1.1),
            lambda: sp.sample_tokens(x, u, top_p=-0.1), lambda: sp.sample_tokens(x, u, min_p=1.5),
+           lambda: sp.sample_tokens(x, u, top_k=5.5), lambda: sp.sample_tokens(x, u, temperature='hot'),
            lambda: sp.sample_tokens(x, u, temperature=u.double()), lambda: sp.sample_tokens(x, u, top_k=u),
            lambda: sp.sample_tokens(x, u, top_p=u[:1]), lambda: sp.sample_tokens(x, u, min_p=u.cpu())]
     for i, call in enumerate(bad):
