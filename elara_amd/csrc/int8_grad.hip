@@ -4,6 +4,12 @@
 // x = q scale in bf16 is exact where the scale is a power of two (q has 7 bits, bf16 holds 8), else rounded once to it.  dy in bf16 goes
 // into the products as it is; fp16 values are the sum of two bf16 parts (8 and 3 bits), fp32 values of three (8 bits each), so the products
 // are exact and only the fp32 sums round.  (Bits of fp32 values below 2^-133 are lost; an infinity makes its outputs NaN.)
+//
+// Measured, tokens x N x K with groups of 128.  16,384 x 4,096 x 4,096 bf16 512-530 us, 1.05 PFLOP/s (torch's library product of two bf16
+// matrices that are already wide 470-475): the matrix units are busy 46 % of the cycles, a wave waits 29 % of its time for memory, LDS or
+// the barrier and 39 % for its turn to issue.  Fewer barriers (64 tokens a step instead of 32) and rows two steps ahead instead of one
+// changed nothing, LDS reads have no bank conflicts.  4,096 x 4,096 x 4,096 fp16 294 us, fp32 420-450 (two and three products).
+// 5,001 x 500 x 1,000 fp32 34 us: 30 for 512 blocks of ten steps and 7 to join 16 parts.  2,048 x 512 x 256 bf16 14 us.
 #include "elr_int8.h"
 
 #include <type_traits>
@@ -351,8 +357,11 @@ __global__ __launch_bounds__(256) void k_wgrad_join(const float* part, int split
 
 // ---- host side
 
-// Tiles and splits of the tokens.  256 x 256 where such tiles alone nearly fill the chip, else 128 x 128 with the tokens split so that
-// about two blocks a CU run, of 256 tokens at least.
+// Tiles and splits of the tokens.  256 x 256 where such tiles alone nearly fill the chip (4,096 x 4,096 x 4,096 bf16 1,000 TFLOP/s, 128 x
+// 128 about 690), bf16 gradients only: two or three parts of a step's rows do not fit the registers beside that tile's sums.  Else 128 x
+// 128 with the tokens split so that about two blocks a CU run, of 256 tokens at least (5,001 x 500 x 1,000 fp32 41 us so, 46 with one
+// block a CU; 20,480 x 512 x 1,024 86 and 104; 128 tokens at least: 512 x 512 x 1,024 fp32 16.5 instead of 18, 1,024 of them 22 instead
+// of 21).
 struct WgradPlan {
   int tile;
   int64_t tiles_m, tiles_n, splits;
