@@ -639,6 +639,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
     const int b = (int)sh.bin;
     const u64 above = sh.above, above_mass = sh.bin_mass;
     if (b == kBins) {
+      __syncthreads();      // (the next call writes what every wave has just read; the way below has barriers of its own)
       kept_mass = above_mass;
       return true;
     }

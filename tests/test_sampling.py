@@ -153,6 +153,53 @@ def test_many_rows_with_ties_at_the_threshold(dev):
         assert torch.equal(sp.sample_tokens(x, u, top_k=k).token, want)
 
 
+def _nucleus(x, u, top_p, min_p):
+    """(ids, log probabilities, whether u and top_p lie clear of every border) of all rows by top_p and min_p, in 64 bits on x's
+    device."""
+    x = x.double()
+    m = x.amax(-1, keepdim=True)
+    order = torch.sort(x, dim=-1, descending=True, stable=True).indices
+    e = (x - m).exp()
+    w = e.gather(1, order)
+    total, before = w.sum(-1, keepdim=True), w.cumsum(-1) - w
+    on = before < top_p * total
+    on[:, 0] = True
+    clear = (before - top_p * total).abs().amin(-1) > 2.0 ** -25 * total[:, 0]
+    if min_p > 0:
+        on &= x.gather(1, order) - m >= math.log(min_p)
+    kept = torch.zeros_like(e).scatter_(1, order, torch.where(on, w, 0.0))
+    cum = kept.cumsum(-1)
+    t = u.double()[:, None] * cum[:, -1:]
+    clear &= (cum - t).abs().amin(-1) > 2.0 ** -25 * cum[:, -1]
+    token = (cum <= t).sum(-1).clamp(max=x.shape[1] - 1)
+    return token, (kept.gather(1, token[:, None])[:, 0] / cum[:, -1]).log(), clear
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,V,top_k,dtype', [(3000, 5000, 1000, torch.bfloat16), (3000, 3000, 600, torch.float32),
+                                             (2000, 20_000, 4000, torch.bfloat16), (300, 20_000, 4000, torch.float16),
+                                             (600, 40_000, 9000, torch.bfloat16), (200, 50_000, 9000, torch.bfloat16),
+                                             (40, 140_000, 30_000, torch.bfloat16), (300, 150_000, 40_000, torch.float32)])
+def test_fewer_finite_ids_than_top_k(dev, n, V, top_k, dtype):
+    """Most ids banned, so that top_k (more than a bound's candidates) reaches past the last finite id and top_p has to look for
+    its place after a search that found none: in blocks of 4, 8 and 16 waves."""
+    sp = _sp()
+    g = torch.Generator(device=dev).manual_seed(V + n)
+    x = (torch.randn(n, V, generator=g, device=dev) * 2).to(dtype)
+    x.masked_fill_(torch.rand(n, V, generator=g, device=dev) < 0.9, NEG)
+    assert int((x > NEG).sum(-1).max()) < top_k < V
+    u = torch.rand(n, generator=g, device=dev)
+    for top_p, min_p in ((0.9, 0.0), (0.5, 0.0), (0.95, 1e-3)):
+        token, logp, clear = _nucleus(x, u, top_p, min_p)
+        assert float(clear.double().mean()) > 0.9
+        for k in (top_k, torch.full((n,), top_k, dtype=torch.int32, device=dev)):
+            for _ in range(3):
+                r = sp.sample_tokens(x, u, top_k=k, top_p=top_p, min_p=min_p)
+                assert torch.equal(r.token[clear], token[clear])
+                off = (r.logprob.double() - logp).abs()
+                assert bool((off <= 2.0 ** -24 * logp.abs() + 2.0 ** -25)[clear].all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('V', [50, 777, 4096, 33_000])
