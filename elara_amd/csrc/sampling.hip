@@ -252,7 +252,8 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 1) void k_sample(SampleArgs a) {
                   : a.top_k_64 ? ((const int64_t*)a.top_k_rows)[row] : ((const int32_t*)a.top_k_rows)[row];
   if (greedy) top_k = 1;
   const bool by_k = top_k > 0 && top_k < a.V, by_p = !greedy && top_p < 1.0;
-  const double inv_t = greedy ? 0.0 : 1.0 / temp, per_e = inv_t * 0x1.71547652b82fep+0;      // to powers of two
+  // (1 / T at most 2^1000: already there any smaller value has no weight, and the maximum's own difference times it stays 0)
+  const double inv_t = greedy ? 0.0 : __builtin_fmin(1.0 / temp, 0x1p1000), per_e = inv_t * 0x1.71547652b82fep+0;      // to powers of two
   const auto weight = [&](float v) -> u64 { return weight_of(((double)v - (double)m) * per_e, a.shift); };
   const double low = greedy || !(min_p > 0.0) ? -__builtin_inf() : log(min_p < 1.0 ? min_p : 1.0) * temp;
   // the smallest value that min_p lets through: m itself at most

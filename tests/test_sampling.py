@@ -236,6 +236,34 @@ def test_flat_and_steep_rows(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
+def test_smallest_temperatures(dev, dtype):
+    """Temperatures whose reciprocal fp64 does not hold, or just holds: the ids of the largest logit share the mass, nothing else
+    has any.  What the outputs' memory held before is no answer."""
+    sp = _sp()
+    for V in (1, 5, 900, 5000, 40_000):
+        x = _logits(V, 6, V, dtype)
+        if V > 4:
+            x[2:, V // 3] = x[2:, V - 2] = 100.0              # two of the largest
+            x[4, :] = -1.0                                    # all of them
+            x[5] = 0.0
+            x[5, 3] = torch.finfo(dtype).tiny                 # a neighbour
+        u = torch.tensor([0.1, 0.9, 0.25, 0.75, 0.6, 0.4])
+        ids = [torch.nonzero(r == r.max())[:, 0] for r in x]
+        for s in (dict(), dict(top_k=5), dict(top_k=700), dict(top_p=0.9), dict(min_p=0.1), dict(top_k=400, top_p=1.0, min_p=0.5)):
+            for T in (5e-324, 1e-310, 5e-309, 8e-309, 1e-300):
+                old = torch.full((6,), 777, device=dev), torch.full((6,), 777.0, device=dev)      # the memory of the outputs to come
+                del old
+                r = sp.sample_tokens(x.to(dev), u.to(dev), temperature=T, **s)
+                for i in range(6):
+                    kept = ids[i][:s['top_k']] if 0 < s.get('top_k', 0) < V else ids[i]
+                    if 'top_p' in s and s['top_p'] < 1:       # the first whose mass before is less than the part
+                        kept = kept[torch.arange(len(kept)).double() < s['top_p'] * len(kept)]
+                    assert int(r.token[i]) == int(kept[int(float(u[i].double()) * len(kept))]), (V, s, T, i)
+                    assert abs(float(r.logprob[i]) + math.log(len(kept))) <= 2.0 ** -24 * math.log(len(kept)) + 2.0 ** -25
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
 def test_rows_without_an_answer(dev, dtype):
     sp = _sp()
     for V in (5, 900, 50_000):
