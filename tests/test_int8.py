@@ -218,6 +218,18 @@ def test_linear_places_of_every_product(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_linear_few_steps_of_k(dev, dtype):
+    """Fewer steps of K than are started ahead, and as many or a few more, whole and ending inside: what was started past K does
+    not reach the outputs.  Every product is 127 x 100, so that a missing or a repeated step shows everywhere."""
+    for n, N in ((33, 64), (64, 200), (200, 190), (129, 33_000)):
+        for K in (16, 112, 128, 144, 256, 272, 384, 400, 496, 512, 528, 640, 1024):
+            y = check_linear(dev, torch.full((n, K), 127, dtype=torch.int8), torch.full((N, K), 100, dtype=torch.int8), dtype,
+                             xs=torch.full((n, 1), 2.0 ** -20), ws=torch.ones(N, 1))
+            assert bool((y == y[0, 0]).all())
+
+
+@pytest.mark.gpu
 def test_linear_largest_sums(dev):
     """Every product 2^14 at the largest K: the int32 sum is 2^31 - 2^14."""
     K = 131_071
