@@ -391,7 +391,12 @@ static void linear(const LinearArgs& b, hipStream_t st) {
     if (a.n <= 32) {
       a.n <= 16 ? few<O, 1>(a, st) : few<O, 2>(a, st);
     } else if (whole) {
-      if (tiles(a.n, 256) * (uint64_t)tiles(a.N, 256) >= 192) launch_tiles<O, 256, 2, 4, 2>(a, st);
+      // Tiles of 256 where they alone nearly fill the chip (160 x 4,096 x 131,072 150 us, with 128 176), but 128 for up to 128 tokens, which
+      // are half of one at most (64 x 4,096 x 49,152 48 us, with 256 57; 128 x 4,096 x 131,072 138 and 146; 64 x 1,024 x 65,536 18 and 22).
+      // Else 128 where there is one for each CU (300 x 4,096 x 16,384 37, with 64 73), else 64 (128 x 4,096 x 16,384 28, with 128 35; more
+      // than 512 of them wait for each other's LDS, two to a CU: 300 x 4,096 x 8,192 47, with 128 33).
+      if (tiles(a.n, 256) * (uint64_t)tiles(a.N, 256) >= 192)
+        a.n > 128 ? launch_tiles<O, 256, 2, 4, 2>(a, st) : launch_tiles<O, 128, 2, 2, 2>(a, st);
       else if (a.n > 64 && tiles(a.n, 128) * (uint64_t)tiles(a.N, 128) >= 256) launch_tiles<O, 128, 2, 2, 2>(a, st);
       else launch_tiles<O, 64, 2, 2, 4>(a, st);
     } else if (a.n <= 64) {

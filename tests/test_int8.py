@@ -219,6 +219,15 @@ def test_linear_places_of_every_product(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
+def test_linear_few_tokens_and_many_channels(dev, dtype):
+    """Where the size of the tiles changes with the tokens (128 and 129) and with the channels (48,896 and the next)."""
+    for n, N in ((33, 48_896), (64, 48_897), (65, 49_152), (128, 48_897), (128, 65_544), (129, 48_896), (129, 48_897)):
+        for K in (64, 400):
+            check_linear(dev, _int_rows(n, n, K), _int_rows(N, N, K), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
 def test_linear_few_steps_of_k(dev, dtype):
     """Fewer steps of K than are started ahead, and as many or a few more, whole and ending inside: what was started past K does
     not reach the outputs.  Every product is 127 x 100, so that a missing or a repeated step shows everywhere."""
