@@ -1,8 +1,9 @@
 // A linear layer's weight gradient from its input kept in 8-bit integers:  dW[j, k] = sum_i dy[i, j] x[i, k],  x = q scale, with a scale
 // for each row of x or each group of its columns; dW in fp32, [N, K] or transposed.  No counterpart in the reference.
 //
-// x = q scale in bf16 is exact where the scale is a power of two (q has 7 bits, bf16 holds 8), else rounded once to it.  dy in bf16 goes
-// into the products as it is; fp16 values are the sum of two bf16 parts (8 and 3 bits), fp32 values of three (8 bits each), so the products
+// x = q scale in bf16 is exact where the scale is a power of two (q has 7 bits, bf16 holds 8), else rounded once to it: by 2^-8 of |x| at most,
+// where q itself is off by up to half a step, max / 254, so by no more than x has lost already; a second part of x would double the
+// products.  dy in bf16 goes into the products as it is; fp16 values are the sum of two bf16 parts (8 and 3 bits), fp32 values of three (8 bits each), so the products
 // are exact and only the fp32 sums round.  (Bits of fp32 values below 2^-133 are lost; an infinity makes its outputs NaN.)
 //
 // Measured, tokens x N x K with groups of 128.  16,384 x 4,096 x 4,096 bf16 512-530 us, 1.05 PFLOP/s (torch's library product of two bf16

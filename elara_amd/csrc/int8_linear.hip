@@ -7,7 +7,7 @@
 // Measured (bf16 out but where said).  8,192 x 4,096 x 16,384 (tokens, K, channels) 515-527 us, 2.1 P operations/s, of which the outputs
 // through memory are about 50: a longer K adds 2.6 P/s (each 4,096 of it 0.42 ms), near what this card's clock leaves of the matrix units'
 // 5 P/s under that load; the library's own int8 product takes 550-575 us for the int32 sums alone.  Operands of zeros: 440 us, so the
-// clock is part of it.  128 tokens x 4,096 x 16,384 29 us; 301 x 1,000 x 20,011 (rows of no multiple of 16 bytes) into fp32 23 us, 1,024
+// clock is part of it.  64 tokens x 4,096 x 16,384 26-27 us, 128 28-29; 301 x 1,000 x 20,011 (rows of no multiple of 16 bytes) into fp32 23 us, 1,024
 // columns instead 16.  4 tokens x 4,096 x 16,384 15-18 us (67 MB of weight: 4.4 TB/s in turn over three weights), x 4,096 x 4,096 7, of
 // which a call and its launch are 4-5.
 #include "elr_int8.h"

@@ -21,7 +21,7 @@
 // 20,480 (2,048 of them) 66 us (5.1 TB/s), and 245 backward (1.4), which reads such rows twice; of 100,000 (1,024), read twice
 // either way, 256 (3.2) and 630 (1.3).  The backward from h kept in 8 bits (q s, a scale a row or for each group of columns, widened as
 // it is loaded): 16,384 of 4,096 bf16 with groups of 128 and dh (472 MB) 77 us and 4 for the weight's sum (5.8 TB/s), 2,048 of 256 6.7
-// and 3.5.
+// and 3.5; of 20,480 (2,048 of them, with dh) 245, of 100,000 (1,024) 643 (1.1-1.2 TB/s, read twice).
 #include "elr_int8.h"
 
 #include <type_traits>

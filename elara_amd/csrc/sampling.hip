@@ -10,7 +10,8 @@
 //
 // Exactness.  With one uniform number a row the draw is a search in a cumulative sum, and an error of 2^-24 of the mass moves it across
 // a border in one of a few hundred rows of 100,000 ids.  So the weights are integers: e in fp64, times 2^s and rounded to 64 bits, with
-// V 2^s < 2^63.  Their sums are exact in any order (atomics and splits included), and the same for every launch shape.
+// V 2^s < 2^63 and s at most 51.  Their sums are exact in any order (atomics and splits included), and the same for every launch shape; what
+// is below 2^-(s + 1) of the largest has no weight (2^-46 at 131,072 ids).
 //
 // A row is a block's: read once for its maximum and, in registers or by the maxima of its steps, for the few elements that can matter.
 // top_k of up to 192 (48 for a wave's short rows): the k-th largest of 256 threads' maxima bounds the k-th largest element from below;
@@ -20,7 +21,7 @@
 // of the kept weights in the order of ids.
 //
 // Measured (bf16 but where said; the floor is the row read once at 5.3 TB/s).  4,096 rows of 32,768 (51 us): T = 0 51, top_k 50 88-98,
-// with top_p 0.9 too 87-93, min_p 0.05 120, no restriction 170-176, top_k 1,000 265, top_p 0.9 alone 370-390, settings by row 178.  301 of
+// with top_p 0.9 too 87-93, min_p 0.05 119-132, no restriction 156-180, top_k 1,000 260-273, top_p 0.9 alone 360-405, settings by row 178.  301 of
 // 50,021 fp32 (11): none 47.  1,024 of 100,003 fp32 (77): T = 0 81, top_k 50 101, none 190.  1 of 131,072: T = 0 9, top_k 50 17-18, none 42,
 // top_p alone 106-110: one CU's work.  8,192 of 1,000 (3): 14, 39, none 25.  What bounds them: T = 0 memory; a bound's rows the
 // chain of barriers behind the reading, about 10 us a row on a CU with four at once; the others about 25 instructions of fp64 an
@@ -86,7 +87,7 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {
 }
 
 // 2^(z + shift) for z <= 0, rounded to an integer below 2^52.  2^f, |f| <= 1/2, by the polynomial through the ten Chebyshev points
-// (1.9e-14 of the value); the sum with 1.5 2^52 rounds z, the one with 2^52 the result.  About 20 instructions of fp64, which runs at
+// (within 3.8e-14 of the value, 2^-44.6, at the ends); the sum with 1.5 2^52 rounds z, the one with 2^52 the result.  About 20 instructions of fp64, which runs at
 // the rate of fp32 here; a NaN (0 times infinity: an infinite temperature) counts as no weight.
 __device__ __forceinline__ u64 weight_of(double z, int shift) {
   constexpr double kRound = 0x1.8p52;

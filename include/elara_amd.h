@@ -792,7 +792,8 @@ int elr_rms_norm_backward(const void* dy, int type, int64_t n, int64_t D, int64_
  * not divide D (scale [n, ceil(D / group)]).  With a = max|x| over a row or group:
  *   pow2 = 0: scale = a / 127 in fp32, 1 where that is 0;  pow2 = 1: the smallest power of two s with 127 s >= a, 2^-126 at
  *   least, 1 for a = 0;  q = x / scale rounded once to the nearest integer, ties to even, in [-127, 127].
- * A NaN or an infinity gives its row or group scale NaN and q = 0.
+ * A NaN or an infinity gives its row or group scale NaN and q = 0.  Near a type's end q scale can round past it: with pow2 values
+ * from 127 2^9 = 65,024 on in fp16, and from 127 2^121 on in fp32 and bf16, can come back infinite, else fp32's largest alone.
  *   x of `type`, rows x_ld elements apart; q [n, D] and scale contiguous and not overlapping x.
  * elr_dequantize_int8: x = q scale in fp32, rounded to `type`, contiguous; rows of q q_ld bytes apart.
  * ------------------------------------------------------------------------------------------------------- */
@@ -803,16 +804,17 @@ int elr_dequantize_int8(const int8_t* q, int64_t n, int64_t D, int64_t q_ld, int
 
 /* y[i, j] = x_scale[i] w_scale[j] sum_k x[i, k] w[j, k]: the product of int8 rows x [n, K] with an int8 weight w [N, K], a
  * scale for each token and each channel.  The sum is exact (int32: K < 2^17, else ELR_EUNSUPPORTED), then widened to fp32,
- * multiplied by x_scale and by w_scale and rounded to `type`.  Rows of x and w x_ld and w_ld bytes apart; y [n, N]
- * contiguous, not overlapping x or w.  K = 0 gives zeros times the scales. */
+ * multiplied by x_scale and by w_scale (in this order: a sum times x_scale past fp32's range is infinite) and rounded to
+ * `type`.  Rows of x and w x_ld and w_ld bytes apart; y [n, N] contiguous, not overlapping x or w.  K = 0 gives zeros times
+ * the scales. */
 int elr_int8_linear(const int8_t* x, int64_t n, int64_t K, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t N,
                     int64_t w_ld, const float* w_scale, void* y, int type, void* stream);
 
 /* The weight gradient of a linear layer from its input kept in 8-bit integers: dw[j, k] = sum_i dy[i, j] x[i, k], x = q scale
- * in bf16 (exact where the scales are powers of two), dy (of `type`) unrounded, sums in fp32 in an order that depends on the
- * sizes alone.  dw fp32 [N, K], or [K, N] with transposed, contiguous; n = 0 gives zeros.  Rows of dy dy_ld elements, of q
- * q_ld bytes apart; scales as above, over K.  An infinity in dy makes its outputs NaN (fp32, fp16) or what the products give
- * (bf16).  scratch of elr_int8_weight_grad_scratch_bytes bytes, 4-byte aligned (may be 0; -1: bad argument). */
+ * in bf16 (exact where the scales are powers of two, else rounded, 2^-8 of x at most), dy (of `type`) unrounded, sums in fp32
+ * in an order that depends on the sizes alone.  dw fp32 [N, K], or [K, N] with transposed, contiguous; n = 0 gives zeros.
+ * Rows of dy dy_ld elements, of q q_ld bytes apart; scales as above, over K.  An infinity in dy makes its outputs NaN (fp32,
+ * fp16) or what the products give (bf16).  scratch of elr_int8_weight_grad_scratch_bytes bytes, 4-byte aligned (may be 0; -1: bad argument). */
 int64_t elr_int8_weight_grad_scratch_bytes(int64_t n, int64_t N, int64_t K, int type);
 int elr_int8_weight_grad(const void* dy, int type, int64_t n, int64_t N, int64_t dy_ld, const int8_t* q, int64_t K,
                          int64_t q_ld, int64_t group, const float* scale, float* dw, int transposed, void* scratch,
@@ -833,9 +835,10 @@ int elr_rms_norm_backward_int8(const void* dy, int type, int64_t n, int64_t D, i
  *   their mass lies (1: all; the first always); of these, those with e >= min_p;
  *   token = the first kept id, in the order of ids, at which the sum of e over kept ids exceeds u times their whole sum S;
  *   logprob = log(e[token] / S).  temperature = 0: the first of the order, logprob 0.
- * Sums are of 64-bit integers (e in fp64 times a power of two): the same for every launch, and an e below 2^-44 or so of the
- * largest is never drawn.  A row of nothing but -inf: token -1, logprob -inf.  A NaN or +inf in a row, a negative or NaN
- * temperature or a NaN u: token -1, logprob NaN.  u outside [0, 1) counts as the nearest in it.
+ * Sums are of 64-bit integers (e in fp64 times 2^s, s = min(51, 62 - ceil(log2 V))): the same for every launch, and an e below
+ * 2^-(s + 1) of the largest is never drawn (2^-46 at V = 131,072, 2^-33 at 2^30).  A row of nothing but -inf: token -1,
+ * logprob -inf.  A NaN or +inf in a row, a negative or NaN temperature or a NaN u: token -1, logprob NaN.  u outside [0, 1)
+ * counts as the nearest in it.
  *   logits of `type`, row i at logits + i * ld elements; u fp32 [n]; each setting a value, or one for each row where its
  *   pointer is not NULL (fp32; top_k int32, or int64 with top_k_64; there values out of range count as the nearest in it,
  *   a NaN as no limit, and negative top_k as 0); token int64 [n], logprob fp32 [n].
