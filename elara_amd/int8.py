@@ -65,8 +65,8 @@ def quantize(x, group=0, pow2=False):
     """x [..., D] cuda float32/float16/bfloat16 (any row stride) -> Int8Rows.  Over each row (group=0) or each group of 32, 64, 128
     or 256 columns (the last one shorter where that does not divide D): scale = max|x| / 127 (1 where that is 0), or with pow2 the
     smallest power of two that is no less (2^-126 at least); q = x / scale rounded to nearest even.  A power of two costs up to one of
-    the 7 bits and makes q * scale exact in bfloat16 and float32, but for the largest values, which can come back infinite (float16 from
-    65,024 on, the others from 127 * 2^121).  A NaN or infinity makes its row or group NaN."""
+    the 7 bits and makes q * scale exact in bfloat16 and float32, but for the largest values, which can come back infinite
+    (float16 from 65,024 on, the others from 127 * 2^121).  A NaN or infinity makes its row or group NaN."""
     r = (_lib._host or _lib.host()).quantize(x, group, int(pow2))
     if r != _lib.NOT_TAKEN:
         _lib.check(r[0], 'elr_quantize_int8')
@@ -106,8 +106,8 @@ def dequantize(rows, dtype=torch.bfloat16):
 
 def linear(x, w, dtype=torch.bfloat16):
     """x: Int8Rows [..., K], a scale for each token; w: Int8Rows [N, K], a scale for each output channel (group=0 both).  Returns
-    [..., N] of dtype: sum_k x.q w.q, exact, times x.scale, times w.scale, rounded once to fp32 at each of these steps (infinite where one
-    passes its range) and then to dtype.  K is at most 131,071."""
+    [..., N] of dtype: sum_k x.q w.q, exact, times x.scale, times w.scale, rounded once to fp32 at each of these steps (infinite
+    where one passes its range) and then to dtype.  K is at most 131,071."""
     r = (_lib._host or _lib.host()).linear(*x, *w, _lib.ETYPE.get(dtype, -1))
     if r != _lib.NOT_TAKEN:
         _lib.check(r[0], 'elr_int8_linear')
@@ -137,8 +137,9 @@ def linear(x, w, dtype=torch.bfloat16):
 def weight_grad(dy, x, transposed=False):
     """dy [..., N] cuda float32/float16/bfloat16 (any row stride): the gradient of x W^T; x: Int8Rows [..., K], the layer's input
     as it was kept (scales by row or by group).  Returns dy^T x, float32 [N, K], or [K, N] with transposed (the gradient of a weight
-    that multiplies from the right).  dy is not rounded; x is q * scale in bfloat16, exact where the scales are powers of two (pow2=True), else
-    rounded: 2^-8 of each value at most, no more than quantizing has left.  Sums are float32 in an order that depends on the sizes alone.  An infinity in dy leaves NaN or infinities in its row of dy^T x."""
+    that multiplies from the right).  dy is not rounded; x is q * scale in bfloat16, exact where the scales are powers of two
+    (pow2=True), else rounded: by 2^-8 of each value at most, no more than quantizing took off it.  Sums are float32 in an order that
+    depends on the sizes alone.  An infinity in dy leaves NaN or infinities in its row of dy^T x."""
     r = (_lib._host or _lib.host()).weight_grad(dy, *x, int(transposed))
     if r != _lib.NOT_TAKEN:
         _lib.check(r[0], 'elr_int8_weight_grad')

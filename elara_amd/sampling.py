@@ -48,8 +48,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
     The token is the first kept id, by rising id, at which the running sum of e exceeds u times the whole; logprob is log(e / whole).
     temperature = 0 takes the first of the order, with logprob 0.  Sums are exact and the same for every launch; an e below
-    2^-(s + 1) of the largest, s = min(51, 62 - ceil(log2 V)), is never drawn (2^-46 at V = 131,072).  -inf marks banned ids: a row of nothing else has token -1 and logprob -inf.  A row with a
-    NaN or +inf, and one whose temperature (in a tensor) is negative or NaN or whose u is NaN, has token -1 and logprob NaN; other
+    2^-(s + 1) of the largest, s = min(51, 62 - ceil(log2 V)), is never drawn (2^-46 at V = 131,072).  -inf marks banned ids: a row
+    of nothing else has token -1 and logprob -inf.  A row with a NaN or +inf, and one whose temperature (in a tensor) is negative or NaN or whose u is NaN, has token -1 and logprob NaN; other
     per-row settings out of range count as the nearest in it, a NaN as no limit."""
     r = (_lib._host or _lib.host()).sample(logits, u, temperature, top_k, top_p, min_p)
     if r != _lib.NOT_TAKEN:
